@@ -549,3 +549,7 @@ def mul_mat_id_glu(qtype, w: torch.Tensor, w_gate: torch.Tensor, x: torch.Tensor
                                         ne11, n_tokens, K, _ptr(ids), n_ids, n_ids, op, alpha, limit, _ptr(out), nrows,
                                         _ptr(workspace), workspace.numel(), _stream()), "hip_qmm_mul_mat_id_glu")
     return out
+
+
+from .attn import (PagedKV, attn_paged, attn_paged_workspace_size, compact_pages, copy_pages, rope,  # noqa: E402,F401
+                   rope_kv_store, rope_steps)
