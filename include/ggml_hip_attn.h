@@ -30,8 +30,8 @@ extern "C" {
  * p*page_stride + h*head_stride + t*token_stride + d, in elements, the same in
  * both.  head_dim is a multiple of 8 up to 256, page_size a power of two from
  * 16 to 65536; k, v 16-byte aligned and the strides multiples of 8 elements;
- * pages, and the heads and tokens of a page, do not overlap.
- * At most 2^31 - 1 tokens in all.
+ * pages, and the heads and tokens of a page, do not overlap; token_stride is
+ * at most 2^27.  At most 2^31 - 1 tokens in all.
  */
 typedef struct hip_qmm_kv_cache {
     void *k, *v;
@@ -109,7 +109,7 @@ int hip_qmm_rope_kv_store(const float *q, int64_t n_heads, int64_t q_token_strid
  * cores as sums of f16 or bf16 parts that hold 22 bits and more.
  * q_starts ascends from 0 or more to n_tokens or less; max_q is at least the
  * largest m; max_kv, the largest length in the host's knowledge, only plans the
- * work (0: table_stride*page_size).  n_heads a multiple of n_kv_heads; q and
+ * work.  n_heads a multiple of n_kv_heads; q and
  * dst 16-byte aligned with strides that are multiples of 4 floats; window and
  * sinks in [0, 2^30].  Deterministic.  The workspace is scratch: its contents
  * do not matter before the call, and it serves one call at a time.

@@ -1,4 +1,24 @@
-// attn.hip -- attention over the paged key-value cache.
+// attn.hip -- attention over the paged key-value cache: one pass over the keys
+// and values of each sequence with the running maximum and sum of the softmax.
+//
+// The query rows of one key-value head are the (token, head) pairs of its
+// group, token first: row r is token r / group, so that the heads of a group
+// share every key and value that is read, for one token as for many.
+//
+// A wave contracts 32 rows with 32 tokens on 32x32x16 matrix instructions, all
+// transposed: scores S^T = K Q^T, results O^T = V^T P^T.  A row is then the
+// lane index (mod 32) of both accumulators: maximum, sum and rescaling stay in
+// the lane (but for one exchange of its halves), and the probabilities, as the
+// scores lie, are the second operand of the next product: slot e of lane half
+// h of its 16-token step holds token 8*(e/4) + 4*h + e%4, an order that the
+// transposing LDS reads of V follow.
+//
+// f32 results from 16-bit matrix cores: keys and values are what the cache
+// holds, exactly; queries and probabilities go in as sums of PARTS 16-bit
+// parts (two f16: 22 bits; three bf16: 24), each a product of its own into the
+// f32 accumulators.  A query row is scaled by a power of two that puts its
+// largest element near 2^13, so that f16's range does not matter; the
+// probabilities carry a factor of 2^12 for the same reason.
 #include <math.h>
 
 #include "kv_cache.h"
@@ -7,6 +27,24 @@ using namespace kvc;
 
 namespace {
 
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void *lds_ptr;
+typedef __attribute__((address_space(3))) v4s *lds_v4s;
+
+enum { PLAIN, EDGE, CARE };  // how a tile's hidden tokens are kept out
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LIFT = 12.0f;   // probabilities are held times 2^LIFT,
+constexpr float SLACK = 3.0f;   // and the running maximum may lag by 2^SLACK: 2^15 stays below f16's largest
+
 struct AttnArgs {
     Cache c;
     const float *q;
@@ -14,76 +52,754 @@ struct AttnArgs {
     int64_t q_token, q_head, dst_token, dst_head;
     const int32_t *q_starts, *table, *lens;
     int64_t table_stride;
-    int n_seqs, n_heads, group, max_q, n_tokens;
-    float scale;
+    int n_seqs, n_heads, group, n_tokens;
+    float scale;  // times log2(e)
     int window, sinks;
+    int per, splits;       // tiles per split, splits at most
+    int blocks;            // row blocks of a (sequence, key-value head)
+    float *part_o, *part_ml;
 };
 
-// The queries of sequence s: rows [*first, *first + count), the last at position n - 1.
-__device__ __forceinline__ int queries_of(const AttnArgs &a, int s, int *first, int *n) {
+// ---------------------------------------------------------------- 16-bit parts
+
+template <bool BF16>
+struct El;
+
+template <>
+struct El<false> {
+    static constexpr int PARTS = 2;
+    static constexpr uint32_t ONE = 0x3c00, EXP2 = 0x7c007c00, STEP2 = 0x04000400, SIGN = 0x8000, INF = 0x7c00;
+    static __device__ __forceinline__ v16f mma(v4u a, v4u b, v16f c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ void split(float x, float y, uint32_t *p) {
+        const v2h h = __builtin_convertvector((v2f){x, y}, v2h);
+        p[0] = __builtin_bit_cast(uint32_t, h);
+        const v2f r = {fmaf((float)h.x, -1.0f, x), fmaf((float)h.y, -1.0f, y)};
+        p[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, v2h));
+    }
+};
+
+template <>
+struct El<true> {
+    static constexpr int PARTS = 3;
+    static constexpr uint32_t ONE = 0x3f80, EXP2 = 0x7f807f80, STEP2 = 0x00800080, SIGN = 0x8000, INF = 0x7f80;
+    static __device__ __forceinline__ v16f mma(v4u a, v4u b, v16f c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ void split(float x, float y, uint32_t *p) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            p[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){x, y}, v2b));
+            x -= __uint_as_float(p[i] << 16);
+            y -= __uint_as_float(p[i] & 0xffff0000u);
+        }
+    }
+};
+
+// ---------------------------------------------------------------- what a block of rows sees
+
+struct Seq {
+    int first, m, n;  // its first row of q, its query count, its length
+};
+
+__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int s) {
     int lo = s, hi = s + 1;
     if (a.q_starts) {
         lo = max(a.q_starts[s], 0);
         hi = min(a.q_starts[s + 1], a.n_tokens);
     }
-    *first = lo;
     const int64_t most = a.table_stride << a.c.page_shift;
-    *n = (int)min((int64_t)max(a.lens[s], 0), most);
-    return max(hi - lo, 0);
+    return {lo, max(hi - lo, 0), (int)min((int64_t)max(a.lens[s], 0), most)};
+}
+
+// Rows [r0, r0 + rows) of a sequence's head group, their positions, and the
+// tiles of TN tokens that any of them sees (from token `low` on, or a first one): first `sink` tiles of the tokens
+// that stay visible, then those from tile `from` on; `count` in all, dealt to
+// the splits `per` at a time, `active` of which have some (the first always).
+template <int TN>
+struct Span {
+    int rows, p_first, p_last, low, sink, from, count, per, active;
+
+    __device__ __forceinline__ Span(const AttnArgs &a, const Seq &q, int r0, int block_rows) {
+        rows = min(block_rows, q.m * a.group - r0);
+        p_first = q.n - q.m + r0 / a.group;
+        p_last = q.n - q.m + (r0 + rows - 1) / a.group;
+        low = a.window ? max(0, p_first - a.window + 1) : 0;
+        sink = (min(a.sinks, low) + TN - 1) / TN;
+        from = max(low / TN, sink);
+        count = p_last < 0 ? 0 : sink + max(0, p_last / TN + 1 - from);
+        per = max(a.per, (count + a.splits - 1) / a.splits);
+        active = max(1, (count + per - 1) / per);
+    }
+    __device__ __forceinline__ int token(int u) const { return (u < sink ? u : from + u - sink) * TN; }
+};
+
+// ---------------------------------------------------------------- LDS tiles
+
+// A tile holds tokens as rows of DP elements in 16-byte chunks; chunk c of
+// token t sits at c ^ swizzle(t), so that 16 tokens' reads of one chunk column
+// meet all banks.
+template <int DP>
+__device__ __forceinline__ int swizzle(int t) { return DP == 64 ? (t >> 1) & 7 : t & 15; }
+
+// 16 bytes per lane from base + off to LDS at lds_base + 16 * lane (base and
+// lds_base wave-uniform).  Inline assembly, so that the compiler, which cannot
+// tell the stages of a ring apart, puts no vmcnt(0) of its own before the LDS
+// reads of another stage; every wait is wait_vm's.  M0 holds the LDS base, the s_nop
+// separates its write from the transfer.
+__device__ __forceinline__ void dma16(const uint16_t *base, uint32_t off, uint32_t lds_base) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds_base) : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    static_assert(N >= 0 && N <= 63, "vmcnt field");
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+    asm volatile("" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t lds_addr(const void *p) { return (uint32_t)(uintptr_t)(lds_ptr)p; }
+
+// The page numbers of 64 consecutive entries of a sequence's table row, one
+// per lane; an entry outside the pool or the row is -1.
+struct Pages {
+    const int32_t *row;
+    int64_t width;
+    int at, mine;
+
+    __device__ __forceinline__ void load(int n_pages) {
+        const int i = at + (threadIdx.x & 63);
+        const int e = i < width ? row[i] : -1;
+        mine = (uint32_t)e < (uint32_t)n_pages ? e : -1;
+    }
+    // Entry i, which like the `more` after it has to be among the 64 (wave-uniform).
+    __device__ __forceinline__ void hold(int i, int more, int n_pages) {
+        if (i < at || i + more > at + 63) {
+            at = i;
+            load(n_pages);
+        }
+    }
+    __device__ __forceinline__ int get(int i) const { return __builtin_amdgcn_readlane(mine, i - at); }
+};
+
+// Transfers i = first, first + step, .. of TN tokens' keys or values into a tile.  A transfer
+// covers 1024 bytes, 512 / DP tokens, inside 16 tokens and so inside one page.
+// Chunks past the head repeat its last one.
+template <int DP, int TN>
+__device__ __forceinline__ void load_tile(const AttnArgs &a, const uint16_t *pool, int64_t head_off, const Pages &pages,
+                                          int t0, uint32_t lds, int first, int step) {
+    constexpr int CH = DP / 8, PER = 64 / CH;  // chunks per token, tokens per transfer
+    const int lane = threadIdx.x & 63, mask = (1 << a.c.page_shift) - 1;
+    const int last = (a.c.head_dim >> 3) - 1;
+    const uint32_t stride = (uint32_t)a.c.token_stride;
+#pragma unroll
+    for (int i = first; i < TN / PER; i += step) {
+        const int g = i * PER;  // uniform: the transfer's first token
+        const int t = g + lane / CH;
+        const int chunk = min((lane % CH) ^ swizzle<DP>(t), last);
+        const int page = pages.get((t0 + g) >> a.c.page_shift);
+        const uint16_t *base = pool + (int64_t)max(page, 0) * a.c.page_stride + head_off +
+                               (int64_t)((t0 + g) & mask) * a.c.token_stride;
+        dma16(base, ((uint32_t)(lane / CH) * stride + chunk * 8) * 2, lds + i * 1024);
+    }
+}
+
+// ---------------------------------------------------------------- a wave's 32 rows
+
+template <bool BF16, int DP, bool FULL>
+struct Rows32 {
+    using E = El<BF16>;
+    static constexpr int KS = DP / 16, DT = DP / 32, P = E::PARTS;
+
+    v4u q[P][KS];
+    v16f o[DT];
+    float unit;      // what a score is to be multiplied with: a power of two
+    float top, sum;  // running maximum (log2), and this lane's share of the sum
+    int pos, low;    // the row's position (-1: none), the first token of its window
+
+    // Row `row` (its own index if `valid`) of the group at q.
+    __device__ __forceinline__ void load(const AttnArgs &a, const float *x, bool valid, int position) {
+        const int h = (threadIdx.x & 63) >> 5, D = a.c.head_dim;
+        pos = valid ? position : -1;
+        low = a.window ? pos - a.window + 1 : 0;
+        float big = 0.0f;
+        auto element8 = [&](int ks, float *v) {
+            const int d = ks * 16 + h * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+            if (valid && (FULL || d < D)) {
+                const float4 u = *reinterpret_cast<const float4 *>(x + d), w = *reinterpret_cast<const float4 *>(x + d + 4);
+                v[0] = u.x * a.scale, v[1] = u.y * a.scale, v[2] = u.z * a.scale, v[3] = u.w * a.scale;
+                v[4] = w.x * a.scale, v[5] = w.y * a.scale, v[6] = w.z * a.scale, v[7] = w.w * a.scale;
+            }
+        };
+        float v[8];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            element8(ks, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(v[e]));
+        }
+        big = fmaxf(big, __shfl_xor(big, 32));
+        const int ex = (int)(__float_as_uint(big) >> 23);  // biased; 255: not finite, left as it is
+        const int up = ex == 255 || ex == 0 ? 0 : min(13 - (ex - 127), 120);
+        unit = ldexpf(1.0f, -up);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            element8(ks, v);
+            uint32_t p[P];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                E::split(ldexpf(v[2 * e], up), ldexpf(v[2 * e + 1], up), p);
+#pragma unroll
+                for (int k = 0; k < P; ++k) q[k][ks][e] = p[k];
+            }
+        }
+        clear();
+    }
+
+    // Scores of tokens [t, t + 32) of the tile at lds.
+    __device__ __forceinline__ v16f scores(const AttnArgs &a, const uint8_t *tile, int t) const {
+        const int lane = threadIdx.x & 63, h = lane >> 5, tok = t + (lane & 31), sw = swizzle<DP>(tok);
+        const uint8_t *row = tile + tok * (DP * 2);
+        v16f s = {};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            v4u k = *reinterpret_cast<const v4u *>(row + (((2 * ks + h) ^ sw) << 4));
+            if (!FULL && ks * 16 + 8 * h >= a.c.head_dim) k = (v4u){};  // past the head: zeros, not its last chunk again
+#pragma unroll
+            for (int p = 0; p < P; ++p) s = E::mma(k, q[p][ks], s);
+        }
+        return s;
+    }
+
+    __device__ __forceinline__ bool sees(const AttnArgs &a, int t) const {
+        return t <= pos && (t >= low || t < a.sinks);
+    }
+
+    // The softmax's step over 32 tokens from t0 on: probabilities (times
+    // 2^(LIFT - top)) in parts, the running values.  Not PLAIN: some row may not see
+    // some token; ok0, ok1: whether the first and second 16 lie in the pool.
+    template <int MODE>
+    __device__ __forceinline__ void soften(const AttnArgs &a, v16f &s, int t0, bool ok0, bool ok1, v4u (&w)[P][2]) {
+        const int h = (threadIdx.x & 63) >> 5;
+        if constexpr (MODE != PLAIN) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (!((r < 8 ? ok0 : ok1) && sees(a, t0 + 8 * (r >> 2) + 4 * h + (r & 3)))) s[r] = -INFINITY;
+        }
+        float mx[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx[r] = fmaxf(fmaxf(s[r], s[r + 4]), fmaxf(s[r + 8], s[r + 12]));
+        float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        {
+            const v2u x = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+            m = fmaxf(__uint_as_float(x.x), __uint_as_float(x.y));
+        }
+        m *= unit;
+        const bool raise = m > top + SLACK;
+        if (__any(raise)) {
+            const float now = raise ? m : top;
+            const float shrink = raise ? __builtin_amdgcn_exp2f(top - now) : 1.0f;
+            top = now;
+            sum *= shrink;
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[t][r] *= shrink;
+        }
+        const float base = (top == -INFINITY ? 0.0f : top) - LIFT;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], unit, -base));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx[r] = (s[r] + s[r + 4]) + (s[r + 8] + s[r + 12]);
+        sum += (mx[0] + mx[1]) + (mx[2] + mx[3]);
+        uint32_t p[P];
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+            E::split(s[r], s[r + 1], p);
+#pragma unroll
+            for (int k = 0; k < P; ++k) w[k][r >> 3][(r & 7) >> 1] = p[k];
+        }
+    }
+
+    // The dwords of a V operand's lane (tokens of a 16-token step from t0 on)
+    // that hold tokens some row of the block sees.
+    __device__ __forceinline__ v4u seen_mask(const AttnArgs &a, int t0, int first, int last, bool ok) const {
+        const int h = (threadIdx.x & 63) >> 5;
+        v4u m = {};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int t = t0 + 8 * (e >> 2) + 4 * h + (e & 3);
+            if (ok && t <= last && (t >= first || t < a.sinks)) m[e >> 1] |= 0xffffu << (16 * (e & 1));
+        }
+        return m;
+    }
+
+    // O^T += V^T P^T over 32 tokens (t of the tile at lds, t0 of the sequence).
+    // EDGE: values that no row sees (m0, m1: masks of the two steps) are taken
+    // as zero, since they may be anything.  CARE: a value that is not finite must
+    // not reach rows that do not see it either, where its weight is 0, nor give
+    // inf - inf in the parts of a weight: such values are taken out of the
+    // product and counted, by kind, over the rows that see them.
+    template <int MODE>
+    __device__ __forceinline__ void gather(const AttnArgs &a, const uint8_t *tile, int t, int t0, bool ok0, bool ok1,
+                                           v4u m0, v4u m1, const v4u (&w)[P][2]) {
+        const int lane = threadIdx.x & 63, h = lane >> 5;
+        const int tok = t + 4 * h + ((lane & 15) >> 2);            // + 16 j + {0, 8}
+        const int sub = ((lane & 16) >> 3) + ((lane & 3) >> 1);    // chunk inside 32 dimensions
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int ta = tok + 16 * j, tb = ta + 8;
+            const uint8_t *ra = tile + ta * (DP * 2) + (lane & 1) * 8, *rb = ra + 8 * DP * 2;
+            const int sa = swizzle<DP>(ta), sb = swizzle<DP>(tb);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(ra + (((4 * d + sub) ^ sa) << 4)));
+                const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(rb + (((4 * d + sub) ^ sb) << 4)));
+                const v2u xu = __builtin_bit_cast(v2u, x), yu = __builtin_bit_cast(v2u, y);
+                v4u v = {xu.x, xu.y, yu.x, yu.y};
+                if constexpr (MODE != PLAIN) v &= j ? m1 : m0;
+                if constexpr (MODE == CARE) {
+                    uint32_t odd = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) odd |= (v[e] & E::EXP2) + E::STEP2;
+                    if (__any(odd & 0x80008000u)) {
+                        const v4u bad = v;
+                        v4u see = {};
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int sh = 16 * (e & 1);
+                            if ((bad[e >> 1] >> sh & E::INF) == E::INF) v[e >> 1] &= ~(0xffffu << sh);
+                            if ((j ? ok1 : ok0) && sees(a, t0 + 16 * j + 8 * (e >> 2) + 4 * h + (e & 3)))
+                                see[e >> 1] |= E::ONE << sh;
+                        }
+#pragma unroll 1
+                        for (int k = 0; k < 3; ++k) {  // inf, -inf, NaN
+                            v4u count = {};
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const int sh = 16 * (e & 1);
+                                const uint32_t b = bad[e >> 1] >> sh & 0xffffu;
+                                const int kind = b == E::INF ? 0 : b == (E::INF | E::SIGN) ? 1 : 2;
+                                if ((b & E::INF) == E::INF && kind == k) count[e >> 1] |= E::ONE << sh;
+                            }
+                            const v16f n = E::mma(count, see, (v16f){});
+                            const float what = k == 0 ? INFINITY : k == 1 ? -INFINITY : NAN;
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) o[d][r] += n[r] > 0.0f ? what : 0.0f;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < P; ++p) o[d] = E::mma(v, w[p][j], o[d]);
+            }
+        }
+    }
+
+    // Scores, softmax step and result of 32 tokens in one mode.
+    template <int MODE>
+    __device__ __forceinline__ void tile32(const AttnArgs &a, const uint8_t *k, const uint8_t *v, int t, int t0, bool ok0,
+                                           bool ok1, int first, int last) {
+        v4u w[P][2], m0 = {}, m1 = {};
+        v16f s = scores(a, k, t);
+        soften<MODE>(a, s, t0, ok0, ok1, w);
+        if constexpr (MODE != PLAIN) {
+            m0 = seen_mask(a, t0, first, last, ok0);
+            m1 = seen_mask(a, t0 + 16, first, last, ok1);
+        }
+        gather<MODE>(a, v, t, t0, ok0, ok1, m0, m1, w);
+    }
+
+    // Whether some result is NaN: by a value that CARE would have kept apart, or rightly.
+    __device__ __forceinline__ bool any_nan() const {
+        bool nan = false;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) nan |= o[t][r] != o[t][r];
+        return __any(nan);
+    }
+
+    __device__ __forceinline__ void clear() {
+        top = -INFINITY;
+        sum = 0.0f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[t] = (v16f){};
+    }
+
+    __device__ __forceinline__ float whole_sum() const { return sum + __shfl_xor(sum, 32); }
+};
+
+// Whether some row of the span may not see some token of [t0, t0 + TN).
+template <int TN>
+__device__ __forceinline__ bool is_edge(const AttnArgs &a, const Span<TN> &sp, int t0) {
+    return t0 + TN - 1 > sp.p_first || (a.window && t0 <= sp.p_last - a.window && t0 + TN > a.sinks);
+}
+
+// Row r of a block (a valid one): where its result goes.
+__device__ __forceinline__ float *result_row(const AttnArgs &a, const Seq &q, int kvh, int r) {
+    const int t = r / a.group, g = r - t * a.group;
+    return a.dst + (int64_t)(q.first + t) * a.dst_token + (int64_t)(kvh * a.group + g) * a.dst_head;
+}
+
+__device__ __forceinline__ int64_t part_row(const AttnArgs &a, const Seq &q, int kvh, int r, int split) {
+    const int t = r / a.group, g = r - t * a.group;
+    return ((int64_t)split * a.n_tokens + q.first + t) * a.n_heads + kvh * a.group + g;
+}
+
+// ---------------------------------------------------------------- few rows
+
+// Up to 32 rows (one token's heads, or a few tokens'): bound by the reads of K
+// and V.  Every wave has tiles of 32 tokens of its own, in a ring of two
+// stages whose K and V halves are refilled as soon as they have been read:
+// three of the four halves are in flight while one is contracted (96 KiB per
+// CU for head_dim 128), with no barrier.  At the end the waves' results are joined
+// in LDS.
+template <int DP>
+struct Few {
+    static constexpr int TN = 32, NW = DP == 256 ? 2 : 4, HALF = TN * DP * 2, RING = 4 * HALF;
+    static constexpr int NX = HALF / 1024;  // transfers per half
+};
+
+template <bool BF16, int DP, bool FULL>
+__global__ __launch_bounds__(Few<DP>::NW * 64, 1) void few_kernel(AttnArgs a) {
+    using F = Few<DP>;
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[F::NW][F::RING];
+    __shared__ float tops[F::NW][32], sums[F::NW][32];
+    const int split = blockIdx.x, kvh = blockIdx.y / a.blocks, block = blockIdx.y - kvh * a.blocks;
+    const Seq q = seq_of(a, blockIdx.z);
+    const int r0 = block * 32;
+    if (r0 >= q.m * a.group) return;
+    const Span<F::TN> sp(a, q, r0, 32);
+    if (split >= sp.active) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int row = r0 + (lane & 31), tok = row / a.group;
+
+    const int64_t head = (int64_t)kvh * a.c.head_stride;
+    const int begin = split * sp.per + wave, end = min(sp.count, (split + 1) * sp.per);
+    const int tiles = begin < end ? (end - begin + F::NW - 1) / F::NW : 0;
+    const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_addr(ring[wave]));
+    Pages pages = {a.table + blockIdx.z * a.table_stride, a.table_stride, 0, -1};
+    const int more = a.c.page_shift == 4 ? 1 : 0;  // a tile spans two pages of 16 tokens
+    uint32_t oks = 0;  // two bits per stage
+
+    // Half h of the ring's order: K and V of tile h / 2.
+    auto issue = [&](int i, bool keys) {
+        const int t0 = sp.token(begin + i * F::NW);
+        if (keys) {
+            pages.hold(t0 >> a.c.page_shift, more, a.c.n_pages);
+            const int p = t0 >> a.c.page_shift;
+            const uint32_t ok = (pages.get(p) >= 0 ? 1 : 0) | (pages.get(p + more) >= 0 ? 2 : 0);
+            oks = i & 1 ? (oks & 3) | ok << 2 : (oks & 12) | ok;
+        }
+        load_tile<DP, F::TN>(a, keys ? a.c.k : a.c.v, head, pages, t0, lds + ((i & 1) * 2 + !keys) * F::HALF, 0, 1);
+    };
+    auto start = [&] {
+        pages.at = sp.token(begin) >> a.c.page_shift;
+        pages.load(a.c.n_pages);
+        issue(0, true);
+        issue(0, false);
+    };
+    if (tiles > 0) start();
+    Rows32<BF16, DP, FULL> w;
+    w.load(a, a.q + (int64_t)(q.first + tok) * a.q_token + (int64_t)(kvh * a.group + row - tok * a.group) * a.q_head,
+           (lane & 31) < sp.rows, q.n - q.m + tok);
+    for (bool care = false;; care = true) {
+        if (tiles > 1) {
+            issue(1, true);
+            issue(1, false);
+        }
+        for (int i = 0; i < tiles; ++i) {
+            const int t0 = sp.token(begin + i * F::NW), ok = oks >> (2 * (i & 1)) & 3;
+            const bool ok0 = ok & 1, ok1 = ok & 2;
+            const uint8_t *k = ring[wave] + (i & 1) * 2 * F::HALF, *v = k + F::HALF;
+            const int left = 2 * (tiles - i) - 1;  // halves after this tile's keys
+            if (left >= 3) wait_vm<3 * F::NX>();
+            else wait_vm<F::NX>();
+            v4u p[El<BF16>::PARTS][2], m0 = {}, m1 = {};
+            v16f s = w.scores(a, k, 0);
+            const bool edge = care || is_edge<F::TN>(a, sp, t0) || ok != 3;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the keys have been read: their half may be refilled
+            if (i + 2 < tiles) issue(i + 2, true);
+            if (edge) {
+                w.template soften<EDGE>(a, s, t0, ok0, ok1, p);
+                m0 = w.seen_mask(a, t0, sp.low, sp.p_last, ok0);
+                m1 = w.seen_mask(a, t0 + 16, sp.low, sp.p_last, ok1);
+            } else {
+                w.template soften<PLAIN>(a, s, t0, true, true, p);
+            }
+            if (left >= 4) wait_vm<3 * F::NX>();
+            else if (left >= 3) wait_vm<2 * F::NX>();
+            else wait_vm<0>();
+            if (care) w.template gather<CARE>(a, v, 0, t0, ok0, ok1, m0, m1, p);
+            else if (edge) w.template gather<EDGE>(a, v, 0, t0, ok0, ok1, m0, m1, p);
+            else w.template gather<PLAIN>(a, v, 0, t0, true, true, m0, m1, p);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (i + 2 < tiles) issue(i + 2, false);
+        }
+        if (care || !w.any_nan()) break;
+        w.clear();  // again, and with care
+        start();
+    }
+
+    // Join the waves: every one's O in its own ring (its transfers are done).
+    constexpr int OS = DP + 4;  // floats per row, off the banks' period
+    const float l = w.whole_sum();
+    if (lane < 32) {
+        tops[wave][lane] = w.top;
+        sums[wave][lane] = l;
+    }
+    float *mine = reinterpret_cast<float *>(ring[wave]);
+    if ((lane & 31) < sp.rows) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4)
+                *reinterpret_cast<float4 *>(mine + (lane & 31) * OS + d * 32 + 2 * r + 4 * (lane >> 5)) =
+                    make_float4(w.o[d][r], w.o[d][r + 1], w.o[d][r + 2], w.o[d][r + 3]);
+    }
+    __syncthreads();
+    const int quads = a.c.head_dim >> 2;
+    for (int i = threadIdx.x; i < sp.rows * quads; i += F::NW * 64) {
+        const int r = i / quads, d = (i - r * quads) * 4;
+        float m = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < F::NW; ++k) m = fmaxf(m, tops[k][r]);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float total = 0.0f;
+#pragma unroll
+        for (int k = 0; k < F::NW; ++k) {
+            if (tops[k][r] == -INFINITY && sums[k][r] == 0.0f) continue;  // nothing seen
+            const float f = __builtin_amdgcn_exp2f(tops[k][r] - m);
+            const float4 u = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(ring[k]) + r * OS + d);
+            total = fmaf(f, sums[k][r], total);
+            o.x = fmaf(f, u.x, o.x), o.y = fmaf(f, u.y, o.y), o.z = fmaf(f, u.z, o.z), o.w = fmaf(f, u.w, o.w);
+        }
+        if (sp.active == 1) {
+            if (total == 0.0f) o = make_float4(0.f, 0.f, 0.f, 0.f);
+            else o.x /= total, o.y /= total, o.z /= total, o.w /= total;
+            *reinterpret_cast<float4 *>(result_row(a, q, kvh, r0 + r) + d) = o;
+        } else {
+            const int64_t at = part_row(a, q, kvh, r0 + r, split);
+            *reinterpret_cast<float4 *>(a.part_o + at * a.c.head_dim + d) = o;
+            if (d == 0) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = make_float2(m, total);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- many rows
+
+// 128 rows, 32 per wave, against tiles of 64 tokens that the four waves share:
+// bound by the matrix cores.  Two stages: the next tile's transfers are in
+// flight while one is contracted, one barrier per tile.
+template <int DP>
+struct Many {
+    static constexpr int TN = 64, NW = 4, HALF = TN * DP * 2, STAGE = 2 * HALF;
+    static constexpr int NX = HALF / 1024 / NW;  // transfers per wave and half
+};
+
+template <bool BF16, int DP, bool FULL>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a) {
+    using M = Many<DP>;
+    __shared__ __attribute__((aligned(1024))) uint8_t stage[2][M::STAGE];
+    const int split = blockIdx.y;
+    // Blocks of one (sequence, key-value head) share its keys and values: they
+    // go to one of the eight XCDs (workgroups are dealt to them in turn) as far
+    // as whole eights of pairs go.
+    const int pairs = a.n_seqs * a.c.n_kv_heads, whole = pairs & ~7;
+    int id = blockIdx.x, pair, block;
+    if (id < whole * a.blocks) {
+        pair = (id & 7) + 8 * ((id >> 3) / a.blocks);
+        block = (id >> 3) % a.blocks;
+    } else {
+        id -= whole * a.blocks;
+        pair = whole + id % (pairs - whole);
+        block = id / (pairs - whole);
+    }
+    const int s = pair / a.c.n_kv_heads, kvh = pair - s * a.c.n_kv_heads;
+    const Seq q = seq_of(a, s);
+    const int all = q.m * a.group, mine = (all + 127) / 128;
+    if (block >= mine) return;
+    const int r0 = (mine - 1 - block) * 128;  // the last rows see most: first
+    const Span<M::TN> sp(a, q, r0, 128);
+    if (split >= sp.active) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int in = wave * 32 + (lane & 31), row = r0 + in, tok = row / a.group;
+
+    const int64_t head = (int64_t)kvh * a.c.head_stride;
+    const int begin = split * sp.per, end = min(sp.count, begin + sp.per);
+    Pages pages = {a.table + s * a.table_stride, a.table_stride, 0, -1};
+    const int more = a.c.page_shift == 4 ? 3 : a.c.page_shift == 5 ? 1 : 0;
+    uint32_t oks = 0;  // four bits per stage
+    auto issue = [&](int u) {
+        const int t0 = sp.token(u), p = t0 >> a.c.page_shift;
+        pages.hold(p, more, a.c.n_pages);
+        uint32_t ok = 0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) ok |= pages.get((t0 + 16 * g) >> a.c.page_shift) >= 0 ? 1u << g : 0;
+        oks = u & 1 ? (oks & 15) | ok << 4 : (oks & 240) | ok;
+        const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_addr(stage[u & 1]));
+        load_tile<DP, M::TN>(a, a.c.k, head, pages, t0, lds, wave, M::NW);
+        load_tile<DP, M::TN>(a, a.c.v, head, pages, t0, lds + M::HALF, wave, M::NW);
+    };
+    auto start = [&] {
+        pages.at = sp.token(begin) >> a.c.page_shift;
+        pages.load(a.c.n_pages);
+        issue(begin);
+    };
+    if (begin < end) start();
+    Rows32<BF16, DP, FULL> w;
+    w.load(a, a.q + (int64_t)(q.first + tok) * a.q_token + (int64_t)(kvh * a.group + row - tok * a.group) * a.q_head,
+           in < sp.rows, q.n - q.m + tok);
+    const bool busy = wave * 32 < sp.rows;
+    for (bool care = false;; care = true) {
+        for (int u = begin; u < end; ++u) {
+            wait_vm<0>();
+            __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wave has read the stage that is refilled next
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            const int ok = oks >> (4 * (u & 1)) & 15, t0 = sp.token(u);
+            if (u + 1 < end) issue(u + 1);
+            if (!busy) continue;
+            const uint8_t *k = stage[u & 1], *v = k + M::HALF;
+            if (care) {
+#pragma unroll 1
+                for (int i = 0; i < 2; ++i)
+                    w.template tile32<CARE>(a, k, v, 32 * i, t0 + 32 * i, ok >> (2 * i) & 1, ok >> (2 * i + 1) & 1, sp.low,
+                                            sp.p_last);
+            } else if (is_edge<M::TN>(a, sp, t0) || ok != 15) {
+#pragma unroll 1
+                for (int i = 0; i < 2; ++i)
+                    w.template tile32<EDGE>(a, k, v, 32 * i, t0 + 32 * i, ok >> (2 * i) & 1, ok >> (2 * i + 1) & 1, sp.low,
+                                            sp.p_last);
+            } else {
+                w.template tile32<PLAIN>(a, k, v, 0, t0, true, true, 0, 0);
+                w.template tile32<PLAIN>(a, k, v, 32, t0 + 32, true, true, 0, 0);
+            }
+        }
+        if (care || !__syncthreads_or(w.any_nan())) break;  // (the barrier also frees both stages)
+        w.clear();
+        if (begin < end) start();
+    }
+
+    const float total = w.whole_sum();
+    if (in >= sp.rows) return;
+    float *out;
+    float f = 1.0f;
+    if (sp.active == 1) {
+        out = result_row(a, q, kvh, row);
+        f = total == 0.0f ? 0.0f : 1.0f / total;
+    } else {
+        const int64_t at = part_row(a, q, kvh, row, split);
+        out = a.part_o + at * a.c.head_dim;
+        if (lane < 32) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = make_float2(w.top, total);
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int e = d * 32 + 2 * r + 4 * (lane >> 5);
+            if (FULL || e < a.c.head_dim)
+                *reinterpret_cast<float4 *>(out + e) =
+                    make_float4(w.o[d][r] * f, w.o[d][r + 1] * f, w.o[d][r + 2] * f, w.o[d][r + 3] * f);
+        }
+}
+
+// ---------------------------------------------------------------- join of the splits
+
+// One wave per row, lanes over the head's dimensions, splits in order.
+template <int TN, int ROWS>
+__global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
+    const Seq q = seq_of(a, blockIdx.z);
+    const int kvh = blockIdx.y, r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (r >= q.m * a.group) return;
+    const Span<TN> sp(a, q, r / ROWS * ROWS, ROWS);
+    if (sp.active == 1) return;
+    const int64_t step = (int64_t)a.n_tokens * a.n_heads, at = part_row(a, q, kvh, r, 0);
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + at;
+    float m = -INFINITY;
+    for (int k = lane; k < sp.active; k += 64) m = fmaxf(m, ml[k * step].x);
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const int D = a.c.head_dim, d = lane * 4;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float total = 0.0f;
+    for (int k = 0; k < sp.active; ++k) {
+        const float2 p = ml[k * step];
+        if (p.x == -INFINITY && p.y == 0.0f) continue;
+        const float f = __builtin_amdgcn_exp2f(p.x - m);
+        total = fmaf(f, p.y, total);
+        if (d < D) {
+            const float4 u = *reinterpret_cast<const float4 *>(a.part_o + (at + k * step) * D + d);
+            o.x = fmaf(f, u.x, o.x), o.y = fmaf(f, u.y, o.y), o.z = fmaf(f, u.z, o.z), o.w = fmaf(f, u.w, o.w);
+        }
+    }
+    if (total == 0.0f) o = make_float4(0.f, 0.f, 0.f, 0.f);
+    else o.x /= total, o.y /= total, o.z /= total, o.w /= total;
+    if (d < D) *reinterpret_cast<float4 *>(result_row(a, q, kvh, r) + d) = o;
+}
+
+// ---------------------------------------------------------------- host
+
+constexpr int FEW_ROWS = 32, MANY_ROWS = 128;
+
+struct Plan {
+    bool few;
+    int blocks, per, splits;
+};
+
+// Which kernel, and how the tokens are split.  A split is worth it while the
+// grid leaves CUs idle; the few-row kernel's splits have a tile per wave at least.
+Plan plan_of(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t max_q, int64_t max_kv, int64_t window,
+             int64_t sinks) {
+    Plan p;
+    const int64_t rows = max_q * (n_heads / c.n_kv_heads);
+    p.few = rows <= FEW_ROWS;
+    const int64_t block_rows = p.few ? FEW_ROWS : MANY_ROWS, tn = p.few ? 32 : 64;
+    p.blocks = (int)((rows + block_rows - 1) / block_rows);
+    int64_t seen = max_kv;
+    if (window && window + max_q + sinks < seen) seen = window + max_q + sinks;
+    const int64_t tiles = (seen + tn - 1) / tn + 1;
+    const int64_t grid = (int64_t)p.blocks * c.n_kv_heads * n_seqs;
+    const int64_t want = p.few ? 1024 : 512, least = p.few ? 4 : 2;
+    int64_t splits = (want + grid - 1) / grid;
+    if (splits > (tiles + least - 1) / least) splits = (tiles + least - 1) / least;
+    if (splits > 256) splits = 256;
+    if (splits < 1 || grid >= want / 2) splits = 1;
+    int64_t per = (tiles + splits - 1) / splits;
+    per = (per + least - 1) / least * least;
+    p.per = (int)per;
+    p.splits = (int)((tiles + per - 1) / per);
+    return p;
+}
+
+bool fine_sizes(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t n_tokens, int64_t max_q, int64_t max_kv,
+                int64_t window, int64_t sinks) {
+    return n_heads >= 1 && n_heads <= 65535 && n_heads % c.n_kv_heads == 0 && n_seqs >= 0 && n_seqs <= 65535 &&
+           n_tokens >= 0 && n_tokens <= ((int64_t)1 << 23) && max_q >= 0 && max_q <= n_tokens && max_kv >= 0 &&
+           max_kv <= INT32_MAX && window >= 0 && sinks >= 0 && window <= (1 << 30) && sinks <= (1 << 30) &&
+           max_q * (n_heads / c.n_kv_heads) <= (1 << 30);
+}
+
+template <bool BF16, int DP, bool FULL>
+int launch(const AttnArgs &a, const Plan &p, hipStream_t s) {
+    if (p.few) {
+        const dim3 grid((unsigned)p.splits, (unsigned)(a.c.n_kv_heads * p.blocks), (unsigned)a.n_seqs);
+        hipLaunchKernelGGL((few_kernel<BF16, DP, FULL>), grid, dim3(Few<DP>::NW * 64), 0, s, a);
+    } else {
+        const dim3 grid((unsigned)(p.blocks * a.c.n_kv_heads * a.n_seqs), (unsigned)p.splits);
+        hipLaunchKernelGGL((many_kernel<BF16, DP, FULL>), grid, dim3(256), 0, s, a);
+    }
+    return (int)hipGetLastError();
 }
 
 template <bool BF16>
-__global__ __launch_bounds__(64) void simple_kernel(AttnArgs a) {
-    __shared__ float qs[256], ps[64];
-    const int head = blockIdx.y, s = blockIdx.z, lane = threadIdx.x;
-    int first, n;
-    const int m = queries_of(a, s, &first, &n);
-    const int D = a.c.head_dim, page = 1 << a.c.page_shift;
-    const int64_t hoff = (int64_t)(head / a.group) * a.c.head_stride;
-    for (int i = blockIdx.x; i < m; i += gridDim.x) {
-        const int p = n - m + i;
-        const float *q = a.q + (int64_t)(first + i) * a.q_token + head * a.q_head;
-        __syncthreads();
-        for (int d = lane; d < D; d += 64) qs[d] = q[d] * a.scale;
-        __syncthreads();
-        float top = -INFINITY, sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int j0 = 0; j0 <= p; j0 += 64) {
-            const int j = j0 + lane;
-            bool seen = j <= p && (a.window == 0 || p - j < a.window || j < a.sinks);
-            int64_t at = 0;
-            if (seen) {
-                const int e = a.table[s * a.table_stride + (j >> a.c.page_shift)];
-                seen = e >= 0 && e < a.c.n_pages;
-                at = e * a.c.page_stride + hoff + (int64_t)(j & (page - 1)) * a.c.token_stride;
-            }
-            float score = -INFINITY;
-            if (seen) {
-                score = 0.f;
-                for (int d = 0; d < D; ++d) score += qs[d] * from16<BF16>(a.c.k[at + d]);
-            }
-            float mx = score;
-            for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-            if (!__any(seen)) continue;
-            const float now = fmaxf(top, mx), base = now == -INFINITY ? 0.f : now;
-            const float shrink = expf(top - base), w = seen ? expf(score - base) : 0.f;
-            float t = w;
-            for (int o = 32; o; o >>= 1) t += __shfl_xor(t, o);
-            sum = sum * shrink + t;
-            top = now;
-            for (int v = 0; v < 4; ++v) acc[v] *= shrink;
-            for (int l = 0; l < 64; ++l) {
-                if (!__shfl((int)seen, l)) continue;
-                const float wl = __shfl(w, l);
-                const int64_t al = __shfl(at, l);
-                for (int v = 0; v < 4; ++v)
-                    if (v * 64 + lane < D) acc[v] += wl * from16<BF16>(a.c.v[al + v * 64 + lane]);
-            }
-        }
-        float *o = a.dst + (int64_t)(first + i) * a.dst_token + head * a.dst_head;
-        for (int v = 0; v < 4; ++v)
-            if (v * 64 + lane < D) o[v * 64 + lane] = sum == 0.f ? 0.f : acc[v] / sum;
-    }
-    (void)ps;
+int launch_dim(const AttnArgs &a, const Plan &p, hipStream_t s) {
+    const int D = a.c.head_dim;
+    if (D <= 64) return D == 64 ? launch<BF16, 64, true>(a, p, s) : launch<BF16, 64, false>(a, p, s);
+    if (D <= 128) return D == 128 ? launch<BF16, 128, true>(a, p, s) : launch<BF16, 128, false>(a, p, s);
+    return D == 256 ? launch<BF16, 256, true>(a, p, s) : launch<BF16, 256, false>(a, p, s);
 }
 
 }  // namespace
@@ -91,8 +807,12 @@ __global__ __launch_bounds__(64) void simple_kernel(AttnArgs a) {
 extern "C" size_t hip_qmm_attn_paged_workspace_size(const hip_qmm_kv_cache *cache, int64_t n_heads, int64_t n_seqs,
                                                     int64_t n_tokens, int64_t max_q, int64_t max_kv, int64_t window,
                                                     int64_t sinks) {
-    (void)cache, (void)n_heads, (void)n_seqs, (void)n_tokens, (void)max_q, (void)max_kv, (void)window, (void)sinks;
-    return 0;
+    Cache c;
+    if (!take(cache, &c) || !fine_sizes(c, n_heads, n_seqs, n_tokens, max_q, max_kv, window, sinks) || max_q == 0 ||
+        n_seqs == 0)
+        return 0;
+    const Plan p = plan_of(c, n_heads, n_seqs, max_q, max_kv, window, sinks);
+    return p.splits == 1 ? 0 : (size_t)p.splits * n_tokens * n_heads * (c.head_dim + 2) * sizeof(float);
 }
 
 extern "C" int hip_qmm_attn_paged(const hip_qmm_kv_cache *cache, const float *q, int64_t n_heads,
@@ -103,12 +823,10 @@ extern "C" int hip_qmm_attn_paged(const hip_qmm_kv_cache *cache, const float *q,
                                   int64_t dst_head_stride, void *workspace, size_t workspace_size, void *stream) {
     AttnArgs a = {};
     const int64_t lim = (int64_t)1 << 40;
-    if (!take(cache, &a.c)) return (int)hipErrorInvalidValue;
-    const int64_t H = a.c.n_kv_heads, D = a.c.head_dim;
-    if (n_heads < 1 || n_heads > 65535 || n_heads % H || n_seqs < 0 || n_seqs > 65535 || n_tokens < 0 ||
-        n_tokens > ((int64_t)1 << 23) || max_q < 0 || max_q > n_tokens || max_kv < 0 || !isfinite(scale) ||
-        window < 0 || sinks < 0 || window > (1 << 30) || sinks > (1 << 30) || table_stride < 0 || table_stride > INT32_MAX)
+    if (!take(cache, &a.c) || !fine_sizes(a.c, n_heads, n_seqs, n_tokens, max_q, max_kv, window, sinks) ||
+        !isfinite(scale) || table_stride < 0 || table_stride > INT32_MAX)
         return (int)hipErrorInvalidValue;
+    const int64_t H = a.c.n_kv_heads, D = a.c.head_dim;
     if (!q_starts && (n_tokens != n_seqs || (n_tokens > 0 && max_q < 1))) return (int)hipErrorInvalidValue;
     if (n_seqs == 0 || n_tokens == 0 || max_q == 0) return 0;
     if (!q || !dst || !kv_lens || (table_stride > 0 && !page_table)) return (int)hipErrorInvalidValue;
@@ -116,6 +834,13 @@ extern "C" int hip_qmm_attn_paged(const hip_qmm_kv_cache *cache, const float *q,
         q_token_stride < 0 || q_head_stride < 0 || dst_token_stride < 0 || dst_head_stride < 0 || q_token_stride > lim ||
         q_head_stride > lim || dst_token_stride > lim || dst_head_stride > lim || (n_heads > 1 && dst_head_stride < D) ||
         (n_tokens > 1 && dst_token_stride < (n_heads - 1) * dst_head_stride + D))
+        return (int)hipErrorInvalidValue;
+    const Plan p = plan_of(a.c, n_heads, n_seqs, max_q, max_kv, window, sinks);
+    const int64_t rows = (int64_t)p.splits * n_tokens * n_heads;
+    if ((int64_t)p.blocks * H > 65535 && p.few) return (int)hipErrorInvalidValue;
+    if ((int64_t)p.blocks * H * n_seqs > (1 << 23)) return (int)hipErrorInvalidValue;
+    if (p.splits > 1 && (!workspace || ((uintptr_t)workspace & 15) ||
+                         workspace_size < (size_t)rows * (D + 2) * sizeof(float)))
         return (int)hipErrorInvalidValue;
     a.q = q;
     a.dst = dst;
@@ -130,17 +855,20 @@ extern "C" int hip_qmm_attn_paged(const hip_qmm_kv_cache *cache, const float *q,
     a.n_seqs = (int)n_seqs;
     a.n_heads = (int)n_heads;
     a.group = (int)(n_heads / H);
-    a.max_q = (int)max_q;
     a.n_tokens = (int)n_tokens;
-    a.scale = scale;
+    a.scale = scale * LOG2E;
     a.window = (int)window;
     a.sinks = (int)sinks;
-    (void)max_kv, (void)workspace, (void)workspace_size;
+    a.per = p.per;
+    a.splits = p.splits;
+    a.blocks = p.blocks;
+    a.part_o = (float *)workspace;
+    a.part_ml = (float *)workspace + rows * D;
     hipStream_t s = (hipStream_t)stream;
-    const dim3 grid((unsigned)max_q, (unsigned)n_heads, (unsigned)n_seqs);
-    if (cache->type == HIP_QMM_TYPE_BF16)
-        hipLaunchKernelGGL(simple_kernel<true>, grid, dim3(64), 0, s, a);
-    else
-        hipLaunchKernelGGL(simple_kernel<false>, grid, dim3(64), 0, s, a);
+    const int e = cache->type == HIP_QMM_TYPE_BF16 ? launch_dim<true>(a, p, s) : launch_dim<false>(a, p, s);
+    if (e || p.splits == 1) return e;
+    const dim3 grid((unsigned)((max_q * a.group + 3) / 4), (unsigned)H, (unsigned)n_seqs);
+    if (p.few) hipLaunchKernelGGL((join_kernel<32, FEW_ROWS>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((join_kernel<64, MANY_ROWS>), grid, dim3(256), 0, s, a);
     return (int)hipGetLastError();
 }

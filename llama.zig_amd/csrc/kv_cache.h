@@ -26,7 +26,7 @@ inline bool take(const hip_qmm_kv_cache *c, Cache *out) {
     if (((uintptr_t)c->k | (uintptr_t)c->v) & 15) return false;
     const int64_t lim = (int64_t)1 << 40;
     if (c->page_stride < 0 || c->head_stride < 0 || c->token_stride < 0 || c->page_stride > lim ||
-        c->head_stride > lim || c->token_stride > lim || ((c->page_stride | c->head_stride | c->token_stride) & 7))
+        c->head_stride > lim || c->token_stride > (1 << 27) || ((c->page_stride | c->head_stride | c->token_stride) & 7))
         return false;
     if (c->page_stride > INT64_MAX / 4 / c->n_pages) return false;
     // Either order of heads and tokens inside a page, nothing overlapping.
