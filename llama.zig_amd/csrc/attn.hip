@@ -5,13 +5,13 @@
 // group, token first: row r is token r / group, so that the heads of a group
 // share every key and value that is read, for one token as for many.
 //
-// A wave contracts 32 rows with 32 tokens on 32x32x16 matrix instructions, all
-// transposed: scores S^T = K Q^T, results O^T = V^T P^T.  A row is then the
-// lane index (mod 32) of both accumulators: maximum, sum and rescaling stay in
-// the lane (but for one exchange of its halves), and the probabilities, as the
-// scores lie, are the second operand of the next product: slot e of lane half
-// h of its 16-token step holds token 8*(e/4) + 4*h + e%4, an order that the
-// transposing LDS reads of V follow.
+// A wave contracts 16 rows or a few times as many with 32 tokens on 16x16x32
+// matrix instructions, all transposed: scores S^T = K Q^T, results
+// O^T = V^T P^T.  A row is then the lane index (mod 16) of both accumulators:
+// maximum, sum and rescaling stay in the lane (but for one exchange among its four
+// quarters), and the probabilities, as the scores lie, are the second operand
+// of the next product: slot e of lane quarter g holds token
+// 16*(e/4) + 4*g + e%4, an order that the transposing LDS reads of V follow.
 //
 // f32 results from 16-bit matrix cores: keys and values are what the cache
 // holds, exactly; queries and probabilities go in as sums of PARTS 16-bit
@@ -28,7 +28,7 @@ using namespace kvc;
 namespace {
 
 typedef float v2f __attribute__((ext_vector_type(2)));
-typedef float v16f __attribute__((ext_vector_type(16)));
+typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
@@ -69,8 +69,8 @@ template <>
 struct El<false> {
     static constexpr int PARTS = 2;
     static constexpr uint32_t ONE = 0x3c00, EXP2 = 0x7c007c00, STEP2 = 0x04000400, SIGN = 0x8000, INF = 0x7c00;
-    static __device__ __forceinline__ v16f mma(v4u a, v4u b, v16f c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+    static __device__ __forceinline__ v4f mma(v4u a, v4u b, v4f c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ void split(float x, float y, uint32_t *p) {
         const v2h h = __builtin_convertvector((v2f){x, y}, v2h);
@@ -84,8 +84,8 @@ template <>
 struct El<true> {
     static constexpr int PARTS = 3;
     static constexpr uint32_t ONE = 0x3f80, EXP2 = 0x7f807f80, STEP2 = 0x00800080, SIGN = 0x8000, INF = 0x7f80;
-    static __device__ __forceinline__ v16f mma(v4u a, v4u b, v16f c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+    static __device__ __forceinline__ v4f mma(v4u a, v4u b, v4f c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ void split(float x, float y, uint32_t *p) {
 #pragma unroll
@@ -168,233 +168,276 @@ struct Pages {
     int64_t width;
     int at, mine;
 
-    __device__ __forceinline__ void load(int n_pages) {
+    __device__ __forceinline__ void load(int first, int n_pages) {
+        at = first;
         const int i = at + (threadIdx.x & 63);
         const int e = i < width ? row[i] : -1;
         mine = (uint32_t)e < (uint32_t)n_pages ? e : -1;
     }
-    // Entry i, which like the `more` after it has to be among the 64 (wave-uniform).
+    // Entries i to i + more will be asked for (wave-uniform, more < 64).
     __device__ __forceinline__ void hold(int i, int more, int n_pages) {
-        if (i < at || i + more > at + 63) {
-            at = i;
-            load(n_pages);
-        }
+        if (i < at || i + more > at + 63) load(i, n_pages);
     }
     __device__ __forceinline__ int get(int i) const { return __builtin_amdgcn_readlane(mine, i - at); }
 };
 
-// Transfers i = first, first + step, .. of TN tokens' keys or values into a tile.  A transfer
-// covers 1024 bytes, 512 / DP tokens, inside 16 tokens and so inside one page.
-// Chunks past the head repeat its last one.
-template <int DP, int TN>
-__device__ __forceinline__ void load_tile(const AttnArgs &a, const uint16_t *pool, int64_t head_off, const Pages &pages,
-                                          int t0, uint32_t lds, int first, int step) {
-    constexpr int CH = DP / 8, PER = 64 / CH;  // chunks per token, tokens per transfer
-    const int lane = threadIdx.x & 63, mask = (1 << a.c.page_shift) - 1;
-    const int last = (a.c.head_dim >> 3) - 1;
-    const uint32_t stride = (uint32_t)a.c.token_stride;
+// Transfers of 1024 bytes, PER tokens each, that fill tiles.  The lane's offset in
+// a transfer depends on the transfer's number modulo NV alone: its chunk is
+// its position XOR the token's swizzle, whose part from the lane and part from the
+// transfer do not meet.  Chunks past the head repeat its last one.
+template <int DP>
+struct Loader {
+    static constexpr int CH = DP / 8, PER = 64 / CH, NV = DP == 64 ? 2 : DP == 128 ? 4 : 8;
+    static constexpr int GROUP = 16 / PER;  // transfers of 16 tokens, which are in one page
+    uint32_t off[NV];
+
+    __device__ __forceinline__ Loader(const AttnArgs &a) {
+        const int lane = threadIdx.x & 63, t = lane / CH, last = (a.c.head_dim >> 3) - 1;
 #pragma unroll
-    for (int i = first; i < TN / PER; i += step) {
-        const int g = i * PER;  // uniform: the transfer's first token
-        const int t = g + lane / CH;
-        const int chunk = min((lane % CH) ^ swizzle<DP>(t), last);
-        const int page = pages.get((t0 + g) >> a.c.page_shift);
-        const uint16_t *base = pool + (int64_t)max(page, 0) * a.c.page_stride + head_off +
-                               (int64_t)((t0 + g) & mask) * a.c.token_stride;
-        dma16(base, ((uint32_t)(lane / CH) * stride + chunk * 8) * 2, lds + i * 1024);
+        for (int i = 0; i < NV; ++i) {
+            const int chunk = min((lane % CH) ^ swizzle<DP>(i * PER + t), last);
+            off[i] = ((uint32_t)t * (uint32_t)a.c.token_stride + chunk * 8) * 2;
+        }
     }
+    // 16 tokens from `base` to LDS; of a workgroup's transfers those of one wave in `step`, from `first` on.
+    __device__ __forceinline__ void group(const AttnArgs &a, const uint16_t *base, uint32_t lds, int first, int step) const {
+#pragma unroll
+        for (int i = 0; i < GROUP; ++i)
+            if (step == 1 || i % step == first)
+                dma16(base + (int64_t)(i * PER) * a.c.token_stride, off[i % NV], lds + i * 1024);
+    }
+};
+
+// Where tokens t0 to t0 + 15 of the held pages lie in a pool (a head's part added by the caller).
+__device__ __forceinline__ int64_t group_at(const AttnArgs &a, int page, int t0) {
+    return (int64_t)max(page, 0) * a.c.page_stride + (int64_t)(t0 & ((1 << a.c.page_shift) - 1)) * a.c.token_stride;
 }
 
-// ---------------------------------------------------------------- a wave's 32 rows
+// ---------------------------------------------------------------- a wave's rows
 
-template <bool BF16, int DP, bool FULL>
-struct Rows32 {
+// The larger of a value's four lane quarters, in all of them.
+__device__ __forceinline__ float quarter_max(float m) {
+    v2u x = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+    m = fmaxf(__uint_as_float(x.x), __uint_as_float(x.y));
+    x = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+    return fmaxf(__uint_as_float(x.x), __uint_as_float(x.y));
+}
+
+// 16 * RT rows.
+template <bool BF16, int DP, bool FULL, int RT>
+struct Rows {
     using E = El<BF16>;
-    static constexpr int KS = DP / 16, DT = DP / 32, P = E::PARTS;
+    static constexpr int KS = DP / 32, DT = DP / 16, P = E::PARTS;
 
-    v4u q[P][KS];
-    v16f o[DT];
-    float unit;      // what a score is to be multiplied with: a power of two
-    float top, sum;  // running maximum (log2), and this lane's share of the sum
-    int pos, low;    // the row's position (-1: none), the first token of its window
+    v4u q[RT][P][KS];
+    v4f o[RT][DT];
+    float unit[RT];           // what a score is to be multiplied with: a power of two
+    float top[RT], sum[RT];   // running maximum (log2), and this lane's share of the sum
+    int pos[RT], low[RT];     // the row's position (-1: none), the first token of its window
 
-    // Row `row` (its own index if `valid`) of the group at q.
-    __device__ __forceinline__ void load(const AttnArgs &a, const float *x, bool valid, int position) {
-        const int h = (threadIdx.x & 63) >> 5, D = a.c.head_dim;
-        pos = valid ? position : -1;
-        low = a.window ? pos - a.window + 1 : 0;
-        float big = 0.0f;
-        auto element8 = [&](int ks, float *v) {
-            const int d = ks * 16 + h * 8;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-            if (valid && (FULL || d < D)) {
-                const float4 u = *reinterpret_cast<const float4 *>(x + d), w = *reinterpret_cast<const float4 *>(x + d + 4);
-                v[0] = u.x * a.scale, v[1] = u.y * a.scale, v[2] = u.z * a.scale, v[3] = u.w * a.scale;
-                v[4] = w.x * a.scale, v[5] = w.y * a.scale, v[6] = w.z * a.scale, v[7] = w.w * a.scale;
-            }
-        };
-        float v[8];
+    // Row 16 * i + lane % 16 of the block, at x if it is valid.
+    __device__ __forceinline__ void load(const AttnArgs &a, int i, const float *x, bool valid, int position) {
+        const int g = (threadIdx.x & 63) >> 4, D = a.c.head_dim;
+        pos[i] = valid ? position : -1;
+        low[i] = a.window ? pos[i] - a.window + 1 : 0;
+        float v[KS][8], big = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            element8(ks, v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(v[e]));
+            const int d = ks * 32 + g * 8;
+            float4 u = make_float4(0.f, 0.f, 0.f, 0.f), w = u;
+            if (valid && (FULL || d < D)) {
+                u = *reinterpret_cast<const float4 *>(x + d);
+                w = *reinterpret_cast<const float4 *>(x + d + 4);
+            }
+            v[ks][0] = u.x, v[ks][1] = u.y, v[ks][2] = u.z, v[ks][3] = u.w;
+            v[ks][4] = w.x, v[ks][5] = w.y, v[ks][6] = w.z, v[ks][7] = w.w;
         }
-        big = fmaxf(big, __shfl_xor(big, 32));
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[ks][e] *= a.scale;
+                big = fmaxf(big, fabsf(v[ks][e]));
+            }
+        big = quarter_max(big);
         const int ex = (int)(__float_as_uint(big) >> 23);  // biased; 255: not finite, left as it is
         const int up = ex == 255 || ex == 0 ? 0 : min(13 - (ex - 127), 120);
-        unit = ldexpf(1.0f, -up);
+        unit[i] = ldexpf(1.0f, -up);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            element8(ks, v);
             uint32_t p[P];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                E::split(ldexpf(v[2 * e], up), ldexpf(v[2 * e + 1], up), p);
+                E::split(ldexpf(v[ks][2 * e], up), ldexpf(v[ks][2 * e + 1], up), p);
 #pragma unroll
-                for (int k = 0; k < P; ++k) q[k][ks][e] = p[k];
+                for (int k = 0; k < P; ++k) q[i][k][ks][e] = p[k];
             }
         }
-        clear();
     }
 
-    // Scores of tokens [t, t + 32) of the tile at lds.
-    __device__ __forceinline__ v16f scores(const AttnArgs &a, const uint8_t *tile, int t) const {
-        const int lane = threadIdx.x & 63, h = lane >> 5, tok = t + (lane & 31), sw = swizzle<DP>(tok);
-        const uint8_t *row = tile + tok * (DP * 2);
-        v16f s = {};
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            v4u k = *reinterpret_cast<const v4u *>(row + (((2 * ks + h) ^ sw) << 4));
-            if (!FULL && ks * 16 + 8 * h >= a.c.head_dim) k = (v4u){};  // past the head: zeros, not its last chunk again
+        for (int i = 0; i < RT; ++i) {
+            top[i] = -INFINITY;
+            sum[i] = 0.0f;
 #pragma unroll
-            for (int p = 0; p < P; ++p) s = E::mma(k, q[p][ks], s);
+            for (int d = 0; d < DT; ++d) o[i][d] = (v4f){};
         }
-        return s;
     }
 
-    __device__ __forceinline__ bool sees(const AttnArgs &a, int t) const {
-        return t <= pos && (t >= low || t < a.sinks);
+    // Scores of tokens [t, t + 32) of the tile: s[i][j] those of 16 j + 4 g + {0..3}.
+    __device__ __forceinline__ void scores(const AttnArgs &a, const uint8_t *tile, int t, v4f (&s)[RT][2]) const {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int tok = t + 16 * j + (lane & 15), sw = swizzle<DP>(tok);
+            const uint8_t *row = tile + tok * (DP * 2);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) s[i][j] = (v4f){};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                v4u k = *reinterpret_cast<const v4u *>(row + (((4 * ks + g) ^ sw) << 4));
+                if (!FULL && ks * 32 + g * 8 >= a.c.head_dim) k = (v4u){};  // past the head: zeros, not its last chunk again
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) s[i][j] = E::mma(k, q[i][p][ks], s[i][j]);
+            }
+        }
+    }
+
+    __device__ __forceinline__ bool sees(const AttnArgs &a, int i, int t) const {
+        return t <= pos[i] && (t >= low[i] || t < a.sinks);
     }
 
     // The softmax's step over 32 tokens from t0 on: probabilities (times
-    // 2^(LIFT - top)) in parts, the running values.  Not PLAIN: some row may not see
-    // some token; ok0, ok1: whether the first and second 16 lie in the pool.
+    // 2^(LIFT - top)) in parts, the running values.  Not PLAIN: some row may not
+    // see some token; ok0, ok1: whether the first and second 16 lie in the pool.
     template <int MODE>
-    __device__ __forceinline__ void soften(const AttnArgs &a, v16f &s, int t0, bool ok0, bool ok1, v4u (&w)[P][2]) {
-        const int h = (threadIdx.x & 63) >> 5;
-        if constexpr (MODE != PLAIN) {
+    __device__ __forceinline__ void soften(const AttnArgs &a, v4f (&s)[RT][2], int t0, bool ok0, bool ok1,
+                                           v4u (&w)[RT][P]) {
+        const int g = (threadIdx.x & 63) >> 4;
+        float m[RT];
+        bool raise = false;
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (!((r < 8 ? ok0 : ok1) && sees(a, t0 + 8 * (r >> 2) + 4 * h + (r & 3)))) s[r] = -INFINITY;
-        }
-        float mx[4];
+        for (int i = 0; i < RT; ++i) {
+            if constexpr (MODE != PLAIN) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) mx[r] = fmaxf(fmaxf(s[r], s[r + 4]), fmaxf(s[r + 8], s[r + 12]));
-        float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        {
-            const v2u x = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-            m = fmaxf(__uint_as_float(x.x), __uint_as_float(x.y));
+                for (int r = 0; r < 8; ++r)
+                    if (!((r < 4 ? ok0 : ok1) && sees(a, i, t0 + 16 * (r >> 2) + 4 * g + (r & 3))))
+                        s[i][r >> 2][r & 3] = -INFINITY;
+            }
+            float x = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x = fmaxf(x, fmaxf(s[i][0][r], s[i][1][r]));
+            m[i] = quarter_max(x) * unit[i];
+            raise |= m[i] > top[i] + SLACK;
         }
-        m *= unit;
-        const bool raise = m > top + SLACK;
         if (__any(raise)) {
-            const float now = raise ? m : top;
-            const float shrink = raise ? __builtin_amdgcn_exp2f(top - now) : 1.0f;
-            top = now;
-            sum *= shrink;
 #pragma unroll
-            for (int t = 0; t < DT; ++t)
+            for (int i = 0; i < RT; ++i) {
+                const bool mine = m[i] > top[i] + SLACK;
+                const float shrink = mine ? __builtin_amdgcn_exp2f(top[i] - m[i]) : 1.0f;
+                top[i] = mine ? m[i] : top[i];
+                sum[i] *= shrink;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[t][r] *= shrink;
+                for (int d = 0; d < DT; ++d) o[i][d] *= shrink;
+            }
         }
-        const float base = (top == -INFINITY ? 0.0f : top) - LIFT;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], unit, -base));
+        for (int i = 0; i < RT; ++i) {
+            const float base = (top[i] == -INFINITY ? 0.0f : top[i]) - LIFT;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) mx[r] = (s[r] + s[r + 4]) + (s[r + 8] + s[r + 12]);
-        sum += (mx[0] + mx[1]) + (mx[2] + mx[3]);
-        uint32_t p[P];
+            for (int j = 0; j < 2; ++j) {
 #pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-            E::split(s[r], s[r + 1], p);
+                for (int r = 0; r < 4; ++r) s[i][j][r] = __builtin_amdgcn_exp2f(fmaf(s[i][j][r], unit[i], -base));
+                sum[i] += (s[i][j][0] + s[i][j][1]) + (s[i][j][2] + s[i][j][3]);
+                uint32_t p[P];
 #pragma unroll
-            for (int k = 0; k < P; ++k) w[k][r >> 3][(r & 7) >> 1] = p[k];
+                for (int r = 0; r < 4; r += 2) {
+                    E::split(s[i][j][r], s[i][j][r + 1], p);
+#pragma unroll
+                    for (int k = 0; k < P; ++k) w[i][k][2 * j + (r >> 1)] = p[k];
+                }
+            }
         }
     }
 
-    // The dwords of a V operand's lane (tokens of a 16-token step from t0 on)
-    // that hold tokens some row of the block sees.
-    __device__ __forceinline__ v4u seen_mask(const AttnArgs &a, int t0, int first, int last, bool ok) const {
-        const int h = (threadIdx.x & 63) >> 5;
+    // The dwords of a V operand's lane (tokens from t0 on) that hold tokens
+    // some row of the block sees.
+    __device__ __forceinline__ v4u seen_mask(const AttnArgs &a, int t0, int first, int last, bool ok0, bool ok1) const {
+        const int g = (threadIdx.x & 63) >> 4;
         v4u m = {};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int t = t0 + 8 * (e >> 2) + 4 * h + (e & 3);
-            if (ok && t <= last && (t >= first || t < a.sinks)) m[e >> 1] |= 0xffffu << (16 * (e & 1));
+            const int t = t0 + 16 * (e >> 2) + 4 * g + (e & 3);
+            if ((e < 4 ? ok0 : ok1) && t <= last && (t >= first || t < a.sinks)) m[e >> 1] |= 0xffffu << (16 * (e & 1));
         }
         return m;
     }
 
-    // O^T += V^T P^T over 32 tokens (t of the tile at lds, t0 of the sequence).
-    // EDGE: values that no row sees (m0, m1: masks of the two steps) are taken
-    // as zero, since they may be anything.  CARE: a value that is not finite must
-    // not reach rows that do not see it either, where its weight is 0, nor give
-    // inf - inf in the parts of a weight: such values are taken out of the
-    // product and counted, by kind, over the rows that see them.
+    // Takes the values that are not finite out of a V operand v of dimension
+    // tile d, and adds them up by kind over the rows that see them.
+    __device__ __forceinline__ void odd_values(const AttnArgs &a, v4u &v, int d, int t0, bool ok0, bool ok1) {
+        const int g = (threadIdx.x & 63) >> 4;
+        const v4u bad = v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if ((bad[e >> 1] >> (16 * (e & 1)) & E::INF) == E::INF) v[e >> 1] &= ~(0xffffu << (16 * (e & 1)));
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            v4u see = {};
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if ((e < 4 ? ok0 : ok1) && sees(a, i, t0 + 16 * (e >> 2) + 4 * g + (e & 3)))
+                    see[e >> 1] |= E::ONE << (16 * (e & 1));
+#pragma unroll 1
+            for (int k = 0; k < 3; ++k) {  // inf, -inf, NaN
+                v4u count = {};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t b = bad[e >> 1] >> (16 * (e & 1)) & 0xffffu;
+                    const int kind = b == E::INF ? 0 : b == (E::INF | E::SIGN) ? 1 : 2;
+                    if ((b & E::INF) == E::INF && kind == k) count[e >> 1] |= E::ONE << (16 * (e & 1));
+                }
+                const v4f n = E::mma(count, see, (v4f){});
+                const float what = k == 0 ? INFINITY : k == 1 ? -INFINITY : NAN;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[i][d][r] += n[r] > 0.0f ? what : 0.0f;
+            }
+        }
+    }
+
+    // O^T += V^T P^T over 32 tokens (t of the tile, t0 of the sequence).
+    // EDGE: values that no row sees (mask) are taken as zero, since they may be
+    // anything.  CARE: a value that is not finite must not reach rows that do
+    // not see it either, where its weight is 0, nor give inf - inf in the parts
+    // of a weight (odd_values).
     template <int MODE>
     __device__ __forceinline__ void gather(const AttnArgs &a, const uint8_t *tile, int t, int t0, bool ok0, bool ok1,
-                                           v4u m0, v4u m1, const v4u (&w)[P][2]) {
-        const int lane = threadIdx.x & 63, h = lane >> 5;
-        const int tok = t + 4 * h + ((lane & 15) >> 2);            // + 16 j + {0, 8}
-        const int sub = ((lane & 16) >> 3) + ((lane & 3) >> 1);    // chunk inside 32 dimensions
+                                           v4u mask, const v4u (&w)[RT][P]) {
+        const int lane = threadIdx.x & 63;
+        const int ta = t + 4 * (lane >> 4) + ((lane & 15) >> 2), tb = ta + 16;
+        const int sub = (lane & 3) >> 1;  // chunk inside 16 dimensions
+        const uint8_t *ra = tile + ta * (DP * 2) + (lane & 1) * 8, *rb = ra + 16 * DP * 2;
+        const int sa = swizzle<DP>(ta), sb = swizzle<DP>(tb);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int ta = tok + 16 * j, tb = ta + 8;
-            const uint8_t *ra = tile + ta * (DP * 2) + (lane & 1) * 8, *rb = ra + 8 * DP * 2;
-            const int sa = swizzle<DP>(ta), sb = swizzle<DP>(tb);
+        for (int d = 0; d < DT; ++d) {
+            const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(ra + (((2 * d + sub) ^ sa) << 4)));
+            const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(rb + (((2 * d + sub) ^ sb) << 4)));
+            const v2u xu = __builtin_bit_cast(v2u, x), yu = __builtin_bit_cast(v2u, y);
+            v4u v = {xu.x, xu.y, yu.x, yu.y};
+            if constexpr (MODE != PLAIN) v &= mask;
+            if constexpr (MODE == CARE) {
+                uint32_t odd = 0;
 #pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(ra + (((4 * d + sub) ^ sa) << 4)));
-                const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(rb + (((4 * d + sub) ^ sb) << 4)));
-                const v2u xu = __builtin_bit_cast(v2u, x), yu = __builtin_bit_cast(v2u, y);
-                v4u v = {xu.x, xu.y, yu.x, yu.y};
-                if constexpr (MODE != PLAIN) v &= j ? m1 : m0;
-                if constexpr (MODE == CARE) {
-                    uint32_t odd = 0;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) odd |= (v[e] & E::EXP2) + E::STEP2;
-                    if (__any(odd & 0x80008000u)) {
-                        const v4u bad = v;
-                        v4u see = {};
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const int sh = 16 * (e & 1);
-                            if ((bad[e >> 1] >> sh & E::INF) == E::INF) v[e >> 1] &= ~(0xffffu << sh);
-                            if ((j ? ok1 : ok0) && sees(a, t0 + 16 * j + 8 * (e >> 2) + 4 * h + (e & 3)))
-                                see[e >> 1] |= E::ONE << sh;
-                        }
-#pragma unroll 1
-                        for (int k = 0; k < 3; ++k) {  // inf, -inf, NaN
-                            v4u count = {};
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const int sh = 16 * (e & 1);
-                                const uint32_t b = bad[e >> 1] >> sh & 0xffffu;
-                                const int kind = b == E::INF ? 0 : b == (E::INF | E::SIGN) ? 1 : 2;
-                                if ((b & E::INF) == E::INF && kind == k) count[e >> 1] |= E::ONE << sh;
-                            }
-                            const v16f n = E::mma(count, see, (v16f){});
-                            const float what = k == 0 ? INFINITY : k == 1 ? -INFINITY : NAN;
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) o[d][r] += n[r] > 0.0f ? what : 0.0f;
-                        }
-                    }
-                }
-#pragma unroll
-                for (int p = 0; p < P; ++p) o[d] = E::mma(v, w[p][j], o[d]);
+                for (int e = 0; e < 4; ++e) odd |= (v[e] & E::EXP2) + E::STEP2;
+                if (__any(odd & 0x80008000u)) odd_values(a, v, d, t0, ok0, ok1);
             }
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int i = 0; i < RT; ++i) o[i][d] = E::mma(v, w[i][p], o[i][d]);
         }
     }
 
@@ -402,34 +445,30 @@ struct Rows32 {
     template <int MODE>
     __device__ __forceinline__ void tile32(const AttnArgs &a, const uint8_t *k, const uint8_t *v, int t, int t0, bool ok0,
                                            bool ok1, int first, int last) {
-        v4u w[P][2], m0 = {}, m1 = {};
-        v16f s = scores(a, k, t);
+        v4f s[RT][2];
+        v4u w[RT][P], mask = {};
+        scores(a, k, t, s);
         soften<MODE>(a, s, t0, ok0, ok1, w);
-        if constexpr (MODE != PLAIN) {
-            m0 = seen_mask(a, t0, first, last, ok0);
-            m1 = seen_mask(a, t0 + 16, first, last, ok1);
-        }
-        gather<MODE>(a, v, t, t0, ok0, ok1, m0, m1, w);
+        if constexpr (MODE != PLAIN) mask = seen_mask(a, t0, first, last, ok0, ok1);
+        gather<MODE>(a, v, t, t0, ok0, ok1, mask, w);
     }
 
     // Whether some result is NaN: by a value that CARE would have kept apart, or rightly.
     __device__ __forceinline__ bool any_nan() const {
         bool nan = false;
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
+        for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) nan |= o[t][r] != o[t][r];
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) nan |= o[i][d][r] != o[i][d][r];
         return __any(nan);
     }
 
-    __device__ __forceinline__ void clear() {
-        top = -INFINITY;
-        sum = 0.0f;
-#pragma unroll
-        for (int t = 0; t < DT; ++t) o[t] = (v16f){};
+    __device__ __forceinline__ float whole_sum(int i) const {
+        const float x = sum[i] + __shfl_xor(sum[i], 16);
+        return x + __shfl_xor(x, 32);
     }
-
-    __device__ __forceinline__ float whole_sum() const { return sum + __shfl_xor(sum, 32); }
 };
 
 // Whether some row of the span may not see some token of [t0, t0 + TN).
@@ -451,114 +490,126 @@ __device__ __forceinline__ int64_t part_row(const AttnArgs &a, const Seq &q, int
 
 // ---------------------------------------------------------------- few rows
 
-// Up to 32 rows (one token's heads, or a few tokens'): bound by the reads of K
-// and V.  Every wave has tiles of 32 tokens of its own, in a ring of two
-// stages whose K and V halves are refilled as soon as they have been read:
-// three of the four halves are in flight while one is contracted (96 KiB per
-// CU for head_dim 128), with no barrier.  At the end the waves' results are joined
-// in LDS.
-template <int DP>
+// 16 * RT rows (one token's heads, or a few tokens'): bound by the reads of K
+// and V.  Every wave has tiles of 32 tokens of its own, in a ring of ST stages
+// whose K and V halves are refilled as soon as they have been read, with no
+// barrier.  At the end the waves' results are joined in LDS.
+template <int DP, int RT>
 struct Few {
-    static constexpr int TN = 32, NW = DP == 256 ? 2 : 4, HALF = TN * DP * 2, RING = 4 * HALF;
-    static constexpr int NX = HALF / 1024;  // transfers per half
+    static constexpr int TN = 32, NW = 4, ST = DP == 64 ? 2 : 1, HALF = TN * DP * 2;
+    static constexpr int NX = HALF / 1024;     // transfers per half
+    static constexpr int OS = DP + 4;          // floats of a row of results, off the banks' period
+    static constexpr int RING = 2 * ST * HALF > 16 * RT * OS * 4 ? 2 * ST * HALF : 16 * RT * OS * 4;
 };
 
-template <bool BF16, int DP, bool FULL>
-__global__ __launch_bounds__(Few<DP>::NW * 64, 1) void few_kernel(AttnArgs a) {
-    using F = Few<DP>;
+template <bool BF16, int DP, bool FULL, int RT>
+__global__ __launch_bounds__(256, RT == 1 && DP < 256 ? 2 : 1) void few_kernel(AttnArgs a) {
+    using F = Few<DP, RT>;
     __shared__ __attribute__((aligned(1024))) uint8_t ring[F::NW][F::RING];
-    __shared__ float tops[F::NW][32], sums[F::NW][32];
+    __shared__ float tops[F::NW][16 * RT], sums[F::NW][16 * RT];
     const int split = blockIdx.x, kvh = blockIdx.y / a.blocks, block = blockIdx.y - kvh * a.blocks;
     const Seq q = seq_of(a, blockIdx.z);
-    const int r0 = block * 32;
+    const int r0 = block * (16 * RT);
     if (r0 >= q.m * a.group) return;
-    const Span<F::TN> sp(a, q, r0, 32);
+    const Span<F::TN> sp(a, q, r0, 16 * RT);
     if (split >= sp.active) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int row = r0 + (lane & 31), tok = row / a.group;
 
     const int64_t head = (int64_t)kvh * a.c.head_stride;
     const int begin = split * sp.per + wave, end = min(sp.count, (split + 1) * sp.per);
     const int tiles = begin < end ? (end - begin + F::NW - 1) / F::NW : 0;
     const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_addr(ring[wave]));
     Pages pages = {a.table + blockIdx.z * a.table_stride, a.table_stride, 0, -1};
+    const Loader<DP> loader(a);
     const int more = a.c.page_shift == 4 ? 1 : 0;  // a tile spans two pages of 16 tokens
     uint32_t oks = 0;  // two bits per stage
+    int64_t at0 = 0, at1 = 0;  // where the tile last begun lies
 
-    // Half h of the ring's order: K and V of tile h / 2.
-    auto issue = [&](int i, bool keys) {
-        const int t0 = sp.token(begin + i * F::NW);
-        if (keys) {
-            pages.hold(t0 >> a.c.page_shift, more, a.c.n_pages);
-            const int p = t0 >> a.c.page_shift;
-            const uint32_t ok = (pages.get(p) >= 0 ? 1 : 0) | (pages.get(p + more) >= 0 ? 2 : 0);
-            oks = i & 1 ? (oks & 3) | ok << 2 : (oks & 12) | ok;
-        }
-        load_tile<DP, F::TN>(a, keys ? a.c.k : a.c.v, head, pages, t0, lds + ((i & 1) * 2 + !keys) * F::HALF, 0, 1);
+    auto issue_keys = [&](int i) {
+        const int t0 = sp.token(begin + i * F::NW), p = t0 >> a.c.page_shift, st = i % F::ST;
+        pages.hold(p, more, a.c.n_pages);
+        const int p0 = pages.get(p), p1 = pages.get(p + more);
+        const uint32_t ok = (p0 >= 0 ? 1 : 0) | (p1 >= 0 ? 2 : 0);
+        oks = (oks & ~(3u << (2 * st))) | ok << (2 * st);
+        at0 = head + group_at(a, p0, t0);
+        at1 = head + group_at(a, p1, t0 + 16);
+        loader.group(a, a.c.k + at0, lds + st * 2 * F::HALF, 0, 1);
+        loader.group(a, a.c.k + at1, lds + st * 2 * F::HALF + F::HALF / 2, 0, 1);
+    };
+    auto issue_values = [&](int i) {  // of the tile that issue_keys last began
+        const int st = i % F::ST;
+        loader.group(a, a.c.v + at0, lds + (st * 2 + 1) * F::HALF, 0, 1);
+        loader.group(a, a.c.v + at1, lds + (st * 2 + 1) * F::HALF + F::HALF / 2, 0, 1);
+    };
+    // At most n halves issued after the one wanted may be outstanding.
+    auto wait_halves = [&](int n) {
+        if (F::ST > 1 && n >= 3) wait_vm<3 * F::NX>();
+        else if (F::ST > 1 && n == 2) wait_vm<2 * F::NX>();
+        else if (n >= 1) wait_vm<F::NX>();
+        else wait_vm<0>();
     };
     auto start = [&] {
-        pages.at = sp.token(begin) >> a.c.page_shift;
-        pages.load(a.c.n_pages);
-        issue(0, true);
-        issue(0, false);
+        pages.load(sp.token(begin) >> a.c.page_shift, a.c.n_pages);
+#pragma unroll
+        for (int i = 0; i < F::ST; ++i)
+            if (i < tiles) {
+                issue_keys(i);
+                issue_values(i);
+            }
     };
-    if (tiles > 0) start();
-    Rows32<BF16, DP, FULL> w;
-    w.load(a, a.q + (int64_t)(q.first + tok) * a.q_token + (int64_t)(kvh * a.group + row - tok * a.group) * a.q_head,
-           (lane & 31) < sp.rows, q.n - q.m + tok);
+    Rows<BF16, DP, FULL, RT> w;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const int in = 16 * i + (lane & 15), row = r0 + in, tok = row / a.group;
+        w.load(a, i, a.q + (int64_t)(q.first + tok) * a.q_token + (int64_t)(kvh * a.group + row - tok * a.group) * a.q_head,
+               in < sp.rows, q.n - q.m + tok);
+    }
     for (bool care = false;; care = true) {
-        if (tiles > 1) {
-            issue(1, true);
-            issue(1, false);
-        }
+        w.clear();
+        if (tiles > 0) start();
         for (int i = 0; i < tiles; ++i) {
-            const int t0 = sp.token(begin + i * F::NW), ok = oks >> (2 * (i & 1)) & 3;
-            const bool ok0 = ok & 1, ok1 = ok & 2;
-            const uint8_t *k = ring[wave] + (i & 1) * 2 * F::HALF, *v = k + F::HALF;
-            const int left = 2 * (tiles - i) - 1;  // halves after this tile's keys
-            if (left >= 3) wait_vm<3 * F::NX>();
-            else wait_vm<F::NX>();
-            v4u p[El<BF16>::PARTS][2], m0 = {}, m1 = {};
-            v16f s = w.scores(a, k, 0);
-            const bool edge = care || is_edge<F::TN>(a, sp, t0) || ok != 3;
+            const int t0 = sp.token(begin + i * F::NW), st = i % F::ST;
+            const bool ok0 = oks >> (2 * st) & 1, ok1 = oks >> (2 * st) & 2;
+            const uint8_t *k = ring[wave] + st * 2 * F::HALF, *v = k + F::HALF;
+            const int after = 2 * (tiles - i) - 1;  // halves to come after this tile's keys, those not yet issued too
+            wait_halves(min(after, 2 * F::ST - 1));
+            v4f s[RT][2];
+            v4u p[RT][El<BF16>::PARTS], mask = {};
+            w.scores(a, k, 0, s);
+            const bool edge = care || is_edge<F::TN>(a, sp, t0) || !(ok0 && ok1);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the keys have been read: their half may be refilled
-            if (i + 2 < tiles) issue(i + 2, true);
+            if (i + F::ST < tiles) issue_keys(i + F::ST);
             if (edge) {
                 w.template soften<EDGE>(a, s, t0, ok0, ok1, p);
-                m0 = w.seen_mask(a, t0, sp.low, sp.p_last, ok0);
-                m1 = w.seen_mask(a, t0 + 16, sp.low, sp.p_last, ok1);
+                mask = w.seen_mask(a, t0, sp.low, sp.p_last, ok0, ok1);
             } else {
                 w.template soften<PLAIN>(a, s, t0, true, true, p);
             }
-            if (left >= 4) wait_vm<3 * F::NX>();
-            else if (left >= 3) wait_vm<2 * F::NX>();
-            else wait_vm<0>();
-            if (care) w.template gather<CARE>(a, v, 0, t0, ok0, ok1, m0, m1, p);
-            else if (edge) w.template gather<EDGE>(a, v, 0, t0, ok0, ok1, m0, m1, p);
-            else w.template gather<PLAIN>(a, v, 0, t0, true, true, m0, m1, p);
+            wait_halves(min(after - 1, 2 * F::ST - 1));
+            if (care) w.template gather<CARE>(a, v, 0, t0, ok0, ok1, mask, p);
+            else if (edge) w.template gather<EDGE>(a, v, 0, t0, ok0, ok1, mask, p);
+            else w.template gather<PLAIN>(a, v, 0, t0, true, true, mask, p);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (i + 2 < tiles) issue(i + 2, false);
+            if (i + F::ST < tiles) issue_values(i + F::ST);
         }
-        if (care || !w.any_nan()) break;
-        w.clear();  // again, and with care
-        start();
+        if (care || !w.any_nan()) break;  // again, and with care
     }
 
     // Join the waves: every one's O in its own ring (its transfers are done).
-    constexpr int OS = DP + 4;  // floats per row, off the banks' period
-    const float l = w.whole_sum();
-    if (lane < 32) {
-        tops[wave][lane] = w.top;
-        sums[wave][lane] = l;
-    }
     float *mine = reinterpret_cast<float *>(ring[wave]);
-    if ((lane & 31) < sp.rows) {
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
+    for (int i = 0; i < RT; ++i) {
+        const int in = 16 * i + (lane & 15);
+        const float l = w.whole_sum(i);
+        if (lane < 16) {
+            tops[wave][in] = w.top[i];
+            sums[wave][in] = l;
+        }
+        if (in < sp.rows) {
 #pragma unroll
-            for (int r = 0; r < 16; r += 4)
-                *reinterpret_cast<float4 *>(mine + (lane & 31) * OS + d * 32 + 2 * r + 4 * (lane >> 5)) =
-                    make_float4(w.o[d][r], w.o[d][r + 1], w.o[d][r + 2], w.o[d][r + 3]);
+            for (int d = 0; d < DP / 16; ++d)
+                *reinterpret_cast<v4f *>(mine + in * F::OS + d * 16 + 4 * (lane >> 4)) = w.o[i][d];
+        }
     }
     __syncthreads();
     const int quads = a.c.head_dim >> 2;
@@ -567,23 +618,22 @@ __global__ __launch_bounds__(Few<DP>::NW * 64, 1) void few_kernel(AttnArgs a) {
         float m = -INFINITY;
 #pragma unroll
         for (int k = 0; k < F::NW; ++k) m = fmaxf(m, tops[k][r]);
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        v4f o = {};
         float total = 0.0f;
 #pragma unroll
         for (int k = 0; k < F::NW; ++k) {
             if (tops[k][r] == -INFINITY && sums[k][r] == 0.0f) continue;  // nothing seen
             const float f = __builtin_amdgcn_exp2f(tops[k][r] - m);
-            const float4 u = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(ring[k]) + r * OS + d);
+            const v4f u = *reinterpret_cast<const v4f *>(reinterpret_cast<const float *>(ring[k]) + r * F::OS + d);
             total = fmaf(f, sums[k][r], total);
-            o.x = fmaf(f, u.x, o.x), o.y = fmaf(f, u.y, o.y), o.z = fmaf(f, u.z, o.z), o.w = fmaf(f, u.w, o.w);
+            o += f * u;
         }
         if (sp.active == 1) {
-            if (total == 0.0f) o = make_float4(0.f, 0.f, 0.f, 0.f);
-            else o.x /= total, o.y /= total, o.z /= total, o.w /= total;
-            *reinterpret_cast<float4 *>(result_row(a, q, kvh, r0 + r) + d) = o;
+            o = total == 0.0f ? (v4f){} : o / total;
+            *reinterpret_cast<v4f *>(result_row(a, q, kvh, r0 + r) + d) = o;
         } else {
             const int64_t at = part_row(a, q, kvh, r0 + r, split);
-            *reinterpret_cast<float4 *>(a.part_o + at * a.c.head_dim + d) = o;
+            *reinterpret_cast<v4f *>(a.part_o + at * a.c.head_dim + d) = o;
             if (d == 0) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = make_float2(m, total);
         }
     }
@@ -596,8 +646,7 @@ __global__ __launch_bounds__(Few<DP>::NW * 64, 1) void few_kernel(AttnArgs a) {
 // flight while one is contracted, one barrier per tile.
 template <int DP>
 struct Many {
-    static constexpr int TN = 64, NW = 4, HALF = TN * DP * 2, STAGE = 2 * HALF;
-    static constexpr int NX = HALF / 1024 / NW;  // transfers per wave and half
+    static constexpr int TN = 64, NW = 4, RT = 2, HALF = TN * DP * 2, STAGE = 2 * HALF;
 };
 
 template <bool BF16, int DP, bool FULL>
@@ -626,13 +675,14 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
     const Span<M::TN> sp(a, q, r0, 128);
     if (split >= sp.active) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int in = wave * 32 + (lane & 31), row = r0 + in, tok = row / a.group;
 
     const int64_t head = (int64_t)kvh * a.c.head_stride;
     const int begin = split * sp.per, end = min(sp.count, begin + sp.per);
     Pages pages = {a.table + s * a.table_stride, a.table_stride, 0, -1};
+    const Loader<DP> loader(a);
     const int more = a.c.page_shift == 4 ? 3 : a.c.page_shift == 5 ? 1 : 0;
     uint32_t oks = 0;  // four bits per stage
+    // Wave w transfers tokens 16 w to 16 w + 15.
     auto issue = [&](int u) {
         const int t0 = sp.token(u), p = t0 >> a.c.page_shift;
         pages.hold(p, more, a.c.n_pages);
@@ -640,21 +690,27 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
 #pragma unroll
         for (int g = 0; g < 4; ++g) ok |= pages.get((t0 + 16 * g) >> a.c.page_shift) >= 0 ? 1u << g : 0;
         oks = u & 1 ? (oks & 15) | ok << 4 : (oks & 240) | ok;
-        const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_addr(stage[u & 1]));
-        load_tile<DP, M::TN>(a, a.c.k, head, pages, t0, lds, wave, M::NW);
-        load_tile<DP, M::TN>(a, a.c.v, head, pages, t0, lds + M::HALF, wave, M::NW);
+        const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_addr(stage[u & 1])) + wave * (M::HALF / 4);
+        const int t = t0 + 16 * wave;
+        const int64_t at = head + group_at(a, pages.get(t >> a.c.page_shift), t);
+        loader.group(a, a.c.k + at, lds, 0, 1);
+        loader.group(a, a.c.v + at, lds + M::HALF, 0, 1);
     };
     auto start = [&] {
-        pages.at = sp.token(begin) >> a.c.page_shift;
-        pages.load(a.c.n_pages);
+        pages.load(sp.token(begin) >> a.c.page_shift, a.c.n_pages);
         issue(begin);
     };
     if (begin < end) start();
-    Rows32<BF16, DP, FULL> w;
-    w.load(a, a.q + (int64_t)(q.first + tok) * a.q_token + (int64_t)(kvh * a.group + row - tok * a.group) * a.q_head,
-           in < sp.rows, q.n - q.m + tok);
+    Rows<BF16, DP, FULL, M::RT> w;
+#pragma unroll
+    for (int i = 0; i < M::RT; ++i) {
+        const int in = wave * 32 + 16 * i + (lane & 15), row = r0 + in, tok = row / a.group;
+        w.load(a, i, a.q + (int64_t)(q.first + tok) * a.q_token + (int64_t)(kvh * a.group + row - tok * a.group) * a.q_head,
+               in < sp.rows, q.n - q.m + tok);
+    }
     const bool busy = wave * 32 < sp.rows;
     for (bool care = false;; care = true) {
+        w.clear();
         for (int u = begin; u < end; ++u) {
             wait_vm<0>();
             __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wave has read the stage that is refilled next
@@ -680,73 +736,98 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
             }
         }
         if (care || !__syncthreads_or(w.any_nan())) break;  // (the barrier also frees both stages)
-        w.clear();
         if (begin < end) start();
     }
 
-    const float total = w.whole_sum();
-    if (in >= sp.rows) return;
-    float *out;
-    float f = 1.0f;
-    if (sp.active == 1) {
-        out = result_row(a, q, kvh, row);
-        f = total == 0.0f ? 0.0f : 1.0f / total;
-    } else {
-        const int64_t at = part_row(a, q, kvh, row, split);
-        out = a.part_o + at * a.c.head_dim;
-        if (lane < 32) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = make_float2(w.top, total);
-    }
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int e = d * 32 + 2 * r + 4 * (lane >> 5);
-            if (FULL || e < a.c.head_dim)
-                *reinterpret_cast<float4 *>(out + e) =
-                    make_float4(w.o[d][r] * f, w.o[d][r + 1] * f, w.o[d][r + 2] * f, w.o[d][r + 3] * f);
+    for (int i = 0; i < M::RT; ++i) {
+        const int in = wave * 32 + 16 * i + (lane & 15), row = r0 + in;
+        const float total = w.whole_sum(i);
+        if (in >= sp.rows) continue;
+        float *out;
+        float f = 1.0f;
+        if (sp.active == 1) {
+            out = result_row(a, q, kvh, row);
+            f = total == 0.0f ? 0.0f : 1.0f / total;
+        } else {
+            const int64_t at = part_row(a, q, kvh, row, split);
+            out = a.part_o + at * a.c.head_dim;
+            if (lane < 16) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = make_float2(w.top[i], total);
         }
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) {
+            const int e = d * 16 + 4 * (lane >> 4);
+            if (FULL || e < a.c.head_dim) *reinterpret_cast<v4f *>(out + e) = w.o[i][d] * f;
+        }
+    }
 }
 
 // ---------------------------------------------------------------- join of the splits
 
-// One wave per row, lanes over the head's dimensions, splits in order.
-template <int TN, int ROWS>
+// One workgroup per row.  The weights of the splits first (at most MAX_SPLITS,
+// in LDS), then their results: LANES threads hold a row, the groups of them
+// take the splits in turn, four loads of each in flight, and are added in
+// order.
+constexpr int MAX_SPLITS = 256;
+
+template <int TN, int ROWS, int LANES>
 __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
+    __shared__ float weight[MAX_SPLITS], part[8];
+    __shared__ float4 sums[256];
     const Seq q = seq_of(a, blockIdx.z);
-    const int kvh = blockIdx.y, r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int kvh = blockIdx.y, r = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
     if (r >= q.m * a.group) return;
     const Span<TN> sp(a, q, r / ROWS * ROWS, ROWS);
     if (sp.active == 1) return;
     const int64_t step = (int64_t)a.n_tokens * a.n_heads, at = part_row(a, q, kvh, r, 0);
-    const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + at;
-    float m = -INFINITY;
-    for (int k = lane; k < sp.active; k += 64) m = fmaxf(m, ml[k * step].x);
+    const float2 p = tid < sp.active ? reinterpret_cast<const float2 *>(a.part_ml)[at + tid * step]
+                                     : make_float2(-INFINITY, 0.0f);
+    float m = p.x;
     for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    const int D = a.c.head_dim, d = lane * 4;
+    if ((tid & 63) == 0) part[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    const float f = p.x == -INFINITY && p.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p.x - m);
+    float total = f == 0.0f ? 0.0f : f * p.y;
+    weight[tid] = f;
+    for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
+    if ((tid & 63) == 0) part[4 + wave] = total;
+    __syncthreads();
+    constexpr int GROUPS = 256 / LANES;
+    const int D = a.c.head_dim, d = tid % LANES * 4;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float total = 0.0f;
-    for (int k = 0; k < sp.active; ++k) {
-        const float2 p = ml[k * step];
-        if (p.x == -INFINITY && p.y == 0.0f) continue;
-        const float f = __builtin_amdgcn_exp2f(p.x - m);
-        total = fmaf(f, p.y, total);
-        if (d < D) {
-            const float4 u = *reinterpret_cast<const float4 *>(a.part_o + (at + k * step) * D + d);
-            o.x = fmaf(f, u.x, o.x), o.y = fmaf(f, u.y, o.y), o.z = fmaf(f, u.z, o.z), o.w = fmaf(f, u.w, o.w);
+    if (d < D) {
+        const float *src = a.part_o + at * D + d;
+#pragma unroll 4
+        for (int k = tid / LANES; k < sp.active; k += GROUPS) {
+            const float4 u = *reinterpret_cast<const float4 *>(src + k * step * D);
+            const float g = weight[k];
+            // a split that saw nothing has weight 0 and zeros
+            o.x = fmaf(g, u.x, o.x), o.y = fmaf(g, u.y, o.y), o.z = fmaf(g, u.z, o.z), o.w = fmaf(g, u.w, o.w);
         }
+    }
+    sums[tid] = o;
+    __syncthreads();
+    if (tid >= LANES || d >= D) return;
+    total = (part[4] + part[5]) + (part[6] + part[7]);
+#pragma unroll
+    for (int k = 1; k < GROUPS; ++k) {
+        const float4 u = sums[k * LANES + tid];
+        o.x += u.x, o.y += u.y, o.z += u.z, o.w += u.w;
     }
     if (total == 0.0f) o = make_float4(0.f, 0.f, 0.f, 0.f);
     else o.x /= total, o.y /= total, o.z /= total, o.w /= total;
-    if (d < D) *reinterpret_cast<float4 *>(result_row(a, q, kvh, r) + d) = o;
+    *reinterpret_cast<float4 *>(result_row(a, q, kvh, r) + d) = o;
 }
 
 // ---------------------------------------------------------------- host
 
-constexpr int FEW_ROWS = 32, MANY_ROWS = 128;
+constexpr int MANY_ROWS = 128;
 
 struct Plan {
-    bool few;
+    int rows;  // of a block: 16 or 32 (few), 128
     int blocks, per, splits;
+    bool few() const { return rows < MANY_ROWS; }
 };
 
 // Which kernel, and how the tokens are split.  A split is worth it while the
@@ -755,18 +836,18 @@ Plan plan_of(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t max_q, int
              int64_t sinks) {
     Plan p;
     const int64_t rows = max_q * (n_heads / c.n_kv_heads);
-    p.few = rows <= FEW_ROWS;
-    const int64_t block_rows = p.few ? FEW_ROWS : MANY_ROWS, tn = p.few ? 32 : 64;
-    p.blocks = (int)((rows + block_rows - 1) / block_rows);
+    p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : MANY_ROWS;
+    const int64_t tn = p.few() ? 32 : 64;
+    p.blocks = (int)((rows + p.rows - 1) / p.rows);
     int64_t seen = max_kv;
     if (window && window + max_q + sinks < seen) seen = window + max_q + sinks;
     const int64_t tiles = (seen + tn - 1) / tn + 1;
     const int64_t grid = (int64_t)p.blocks * c.n_kv_heads * n_seqs;
-    const int64_t want = p.few ? 1024 : 512, least = p.few ? 4 : 2;
+    const int64_t want = p.few() ? 1024 : 512, least = p.few() ? 4 : 2;
     int64_t splits = (want + grid - 1) / grid;
     if (splits > (tiles + least - 1) / least) splits = (tiles + least - 1) / least;
-    if (splits > 256) splits = 256;
-    if (splits < 1 || grid >= want / 2) splits = 1;
+    if (splits > MAX_SPLITS) splits = MAX_SPLITS;
+    if (splits < 1) splits = 1;
     int64_t per = (tiles + splits - 1) / splits;
     per = (per + least - 1) / least * least;
     p.per = (int)per;
@@ -784,14 +865,23 @@ bool fine_sizes(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t n_token
 
 template <bool BF16, int DP, bool FULL>
 int launch(const AttnArgs &a, const Plan &p, hipStream_t s) {
-    if (p.few) {
+    if (p.few()) {
         const dim3 grid((unsigned)p.splits, (unsigned)(a.c.n_kv_heads * p.blocks), (unsigned)a.n_seqs);
-        hipLaunchKernelGGL((few_kernel<BF16, DP, FULL>), grid, dim3(Few<DP>::NW * 64), 0, s, a);
+        if (p.rows == 16) hipLaunchKernelGGL((few_kernel<BF16, DP, FULL, 1>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((few_kernel<BF16, DP, FULL, 2>), grid, dim3(256), 0, s, a);
     } else {
         const dim3 grid((unsigned)(p.blocks * a.c.n_kv_heads * a.n_seqs), (unsigned)p.splits);
         hipLaunchKernelGGL((many_kernel<BF16, DP, FULL>), grid, dim3(256), 0, s, a);
     }
     return (int)hipGetLastError();
+}
+
+template <int LANES>
+void launch_join(const AttnArgs &a, int rows, int64_t max_q, hipStream_t s) {
+    const dim3 grid((unsigned)(max_q * a.group), (unsigned)a.c.n_kv_heads, (unsigned)a.n_seqs);
+    if (rows == 16) hipLaunchKernelGGL((join_kernel<32, 16, LANES>), grid, dim3(256), 0, s, a);
+    else if (rows == 32) hipLaunchKernelGGL((join_kernel<32, 32, LANES>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((join_kernel<64, MANY_ROWS, LANES>), grid, dim3(256), 0, s, a);
 }
 
 template <bool BF16>
@@ -837,7 +927,7 @@ extern "C" int hip_qmm_attn_paged(const hip_qmm_kv_cache *cache, const float *q,
         return (int)hipErrorInvalidValue;
     const Plan p = plan_of(a.c, n_heads, n_seqs, max_q, max_kv, window, sinks);
     const int64_t rows = (int64_t)p.splits * n_tokens * n_heads;
-    if ((int64_t)p.blocks * H > 65535 && p.few) return (int)hipErrorInvalidValue;
+    if ((int64_t)p.blocks * H > 65535 && p.few()) return (int)hipErrorInvalidValue;
     if ((int64_t)p.blocks * H * n_seqs > (1 << 23)) return (int)hipErrorInvalidValue;
     if (p.splits > 1 && (!workspace || ((uintptr_t)workspace & 15) ||
                          workspace_size < (size_t)rows * (D + 2) * sizeof(float)))
@@ -867,8 +957,8 @@ extern "C" int hip_qmm_attn_paged(const hip_qmm_kv_cache *cache, const float *q,
     hipStream_t s = (hipStream_t)stream;
     const int e = cache->type == HIP_QMM_TYPE_BF16 ? launch_dim<true>(a, p, s) : launch_dim<false>(a, p, s);
     if (e || p.splits == 1) return e;
-    const dim3 grid((unsigned)((max_q * a.group + 3) / 4), (unsigned)H, (unsigned)n_seqs);
-    if (p.few) hipLaunchKernelGGL((join_kernel<32, FEW_ROWS>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((join_kernel<64, MANY_ROWS>), grid, dim3(256), 0, s, a);
+    if (D <= 64) launch_join<16>(a, p.rows, max_q, s);
+    else if (D <= 128) launch_join<32>(a, p.rows, max_q, s);
+    else launch_join<64>(a, p.rows, max_q, s);
     return (int)hipGetLastError();
 }
