@@ -39,8 +39,6 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void *lds_ptr;
 typedef __attribute__((address_space(3))) v4s *lds_v4s;
 
-enum { PLAIN, EDGE, CARE };  // how a tile's hidden tokens are kept out
-
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LIFT = 12.0f;   // probabilities are held times 2^LIFT,
 constexpr float SLACK = 3.0f;   // and the running maximum may lag by 2^SLACK: 2^15 stays below f16's largest
@@ -68,14 +66,16 @@ struct El;
 template <>
 struct El<false> {
     static constexpr int PARTS = 2;
-    static constexpr uint32_t ONE = 0x3c00, EXP2 = 0x7c007c00, STEP2 = 0x04000400, SIGN = 0x8000, INF = 0x7c00;
+    static constexpr uint32_t INF = 0x7c00;
     static __device__ __forceinline__ v4f mma(v4u a, v4u b, v4f c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ void split(float x, float y, uint32_t *p) {
         const v2h h = __builtin_convertvector((v2f){x, y}, v2h);
         p[0] = __builtin_bit_cast(uint32_t, h);
-        const v2f r = {fmaf((float)h.x, -1.0f, x), fmaf((float)h.y, -1.0f, y)};
+        v2f r;  // x - h.x, y - h.y, one mixed operation each
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(r.x) : "v"(p[0]), "v"(x));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r.y) : "v"(p[0]), "v"(y));
         p[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, v2h));
     }
 };
@@ -83,7 +83,7 @@ struct El<false> {
 template <>
 struct El<true> {
     static constexpr int PARTS = 3;
-    static constexpr uint32_t ONE = 0x3f80, EXP2 = 0x7f807f80, STEP2 = 0x00800080, SIGN = 0x8000, INF = 0x7f80;
+    static constexpr uint32_t INF = 0x7f80;
     static __device__ __forceinline__ v4f mma(v4u a, v4u b, v4f c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
     }
@@ -215,6 +215,13 @@ __device__ __forceinline__ int64_t group_at(const AttnArgs &a, int page, int t0)
 
 // ---------------------------------------------------------------- a wave's rows
 
+// The largest of three; a NaN is passed over.  (fmaxf would first quiet each matrix result by an operation of its own.)
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float m;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(x), "v"(y), "v"(z));
+    return m;
+}
+
 // The larger of a value's four lane quarters, in all of them.
 __device__ __forceinline__ float quarter_max(float m) {
     v2u x = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
@@ -306,31 +313,15 @@ struct Rows {
         }
     }
 
-    __device__ __forceinline__ bool sees(const AttnArgs &a, int i, int t) const {
-        return t <= pos[i] && (t >= low[i] || t < a.sinks);
-    }
-
     // The softmax's step over 32 tokens from t0 on: probabilities (times
-    // 2^(LIFT - top)) in parts, the running values.  Not PLAIN: some row may not
-    // see some token; ok0, ok1: whether the first and second 16 lie in the pool.
-    template <int MODE>
-    __device__ __forceinline__ void soften(const AttnArgs &a, v4f (&s)[RT][2], int t0, bool ok0, bool ok1,
-                                           v4u (&w)[RT][P]) {
-        const int g = (threadIdx.x & 63) >> 4;
+    // 2^(LIFT - top)) in parts, the running values.
+    __device__ __forceinline__ void soften(v4f (&s)[RT][2], v4u (&w)[RT][P]) {
         float m[RT];
         bool raise = false;
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
-            if constexpr (MODE != PLAIN) {
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    if (!((r < 4 ? ok0 : ok1) && sees(a, i, t0 + 16 * (r >> 2) + 4 * g + (r & 3))))
-                        s[i][r >> 2][r & 3] = -INFINITY;
-            }
-            float x = -INFINITY;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) x = fmaxf(x, fmaxf(s[i][0][r], s[i][1][r]));
-            m[i] = quarter_max(x) * unit[i];
+            const float x = max3(s[i][0][0], s[i][0][1], s[i][0][2]), y = max3(s[i][0][3], s[i][1][0], s[i][1][1]);
+            m[i] = quarter_max(max3(max3(s[i][1][2], s[i][1][3], x), y, y)) * unit[i];
             raise |= m[i] > top[i] + SLACK;
         }
         if (__any(raise)) {
@@ -363,59 +354,22 @@ struct Rows {
         }
     }
 
-    // The dwords of a V operand's lane (tokens from t0 on) that hold tokens
-    // some row of the block sees.
-    __device__ __forceinline__ v4u seen_mask(const AttnArgs &a, int t0, int first, int last, bool ok0, bool ok1) const {
+    // The scores of tokens (t0 on) that their rows do not see; ok0, ok1: whether
+    // the first and second 16 lie in the pool.
+    __device__ __forceinline__ void hide(const AttnArgs &a, v4f (&s)[RT][2], int t0, bool ok0, bool ok1) const {
         const int g = (threadIdx.x & 63) >> 4;
-        v4u m = {};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int t = t0 + 16 * (e >> 2) + 4 * g + (e & 3);
-            if ((e < 4 ? ok0 : ok1) && t <= last && (t >= first || t < a.sinks)) m[e >> 1] |= 0xffffu << (16 * (e & 1));
-        }
-        return m;
-    }
-
-    // Takes the values that are not finite out of a V operand v of dimension
-    // tile d, and adds them up by kind over the rows that see them.
-    __device__ __forceinline__ void odd_values(const AttnArgs &a, v4u &v, int d, int t0, bool ok0, bool ok1) {
-        const int g = (threadIdx.x & 63) >> 4;
-        const v4u bad = v;
+        for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if ((bad[e >> 1] >> (16 * (e & 1)) & E::INF) == E::INF) v[e >> 1] &= ~(0xffffu << (16 * (e & 1)));
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            v4u see = {};
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if ((e < 4 ? ok0 : ok1) && sees(a, i, t0 + 16 * (e >> 2) + 4 * g + (e & 3)))
-                    see[e >> 1] |= E::ONE << (16 * (e & 1));
-#pragma unroll 1
-            for (int k = 0; k < 3; ++k) {  // inf, -inf, NaN
-                v4u count = {};
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t b = bad[e >> 1] >> (16 * (e & 1)) & 0xffffu;
-                    const int kind = b == E::INF ? 0 : b == (E::INF | E::SIGN) ? 1 : 2;
-                    if ((b & E::INF) == E::INF && kind == k) count[e >> 1] |= E::ONE << (16 * (e & 1));
-                }
-                const v4f n = E::mma(count, see, (v4f){});
-                const float what = k == 0 ? INFINITY : k == 1 ? -INFINITY : NAN;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[i][d][r] += n[r] > 0.0f ? what : 0.0f;
+            for (int r = 0; r < 8; ++r) {
+                const int t = t0 + 16 * (r >> 2) + 4 * g + (r & 3);
+                const bool seen = (r < 4 ? ok0 : ok1) & (t <= pos[i]) & ((t >= low[i]) | (t < a.sinks));
+                s[i][r >> 2][r & 3] = seen ? s[i][r >> 2][r & 3] : -INFINITY;
             }
-        }
     }
 
-    // O^T += V^T P^T over 32 tokens (t of the tile, t0 of the sequence).
-    // EDGE: values that no row sees (mask) are taken as zero, since they may be
-    // anything.  CARE: a value that is not finite must not reach rows that do
-    // not see it either, where its weight is 0, nor give inf - inf in the parts
-    // of a weight (odd_values).
-    template <int MODE>
-    __device__ __forceinline__ void gather(const AttnArgs &a, const uint8_t *tile, int t, int t0, bool ok0, bool ok1,
-                                           v4u mask, const v4u (&w)[RT][P]) {
+    // O^T += V^T P^T over tokens [t, t + 32) of the tile.
+    __device__ __forceinline__ void gather(const uint8_t *tile, int t, const v4u (&w)[RT][P]) {
         const int lane = threadIdx.x & 63;
         const int ta = t + 4 * (lane >> 4) + ((lane & 15) >> 2), tb = ta + 16;
         const int sub = (lane & 3) >> 1;  // chunk inside 16 dimensions
@@ -426,14 +380,7 @@ struct Rows {
             const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(ra + (((2 * d + sub) ^ sa) << 4)));
             const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(rb + (((2 * d + sub) ^ sb) << 4)));
             const v2u xu = __builtin_bit_cast(v2u, x), yu = __builtin_bit_cast(v2u, y);
-            v4u v = {xu.x, xu.y, yu.x, yu.y};
-            if constexpr (MODE != PLAIN) v &= mask;
-            if constexpr (MODE == CARE) {
-                uint32_t odd = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) odd |= (v[e] & E::EXP2) + E::STEP2;
-                if (__any(odd & 0x80008000u)) odd_values(a, v, d, t0, ok0, ok1);
-            }
+            const v4u v = {xu.x, xu.y, yu.x, yu.y};
 #pragma unroll
             for (int p = 0; p < P; ++p)
 #pragma unroll
@@ -441,19 +388,7 @@ struct Rows {
         }
     }
 
-    // Scores, softmax step and result of 32 tokens in one mode.
-    template <int MODE>
-    __device__ __forceinline__ void tile32(const AttnArgs &a, const uint8_t *k, const uint8_t *v, int t, int t0, bool ok0,
-                                           bool ok1, int first, int last) {
-        v4f s[RT][2];
-        v4u w[RT][P], mask = {};
-        scores(a, k, t, s);
-        soften<MODE>(a, s, t0, ok0, ok1, w);
-        if constexpr (MODE != PLAIN) mask = seen_mask(a, t0, first, last, ok0, ok1);
-        gather<MODE>(a, v, t, t0, ok0, ok1, mask, w);
-    }
-
-    // Whether some result is NaN: by a value that CARE would have kept apart, or rightly.
+    // Whether some result is NaN: by a value that `Odd` would have kept apart, or rightly.
     __device__ __forceinline__ bool any_nan() const {
         bool nan = false;
 #pragma unroll
@@ -488,6 +423,69 @@ __device__ __forceinline__ int64_t part_row(const AttnArgs &a, const Seq &q, int
     return ((int64_t)split * a.n_tokens + q.first + t) * a.n_heads + kvh * a.group + g;
 }
 
+// Whether no row of the span sees some token of [t0, t0 + TN), `ok` aside.
+template <int TN>
+__device__ __forceinline__ bool has_unseen(const AttnArgs &a, const Span<TN> &sp, int t0) {
+    return t0 + TN - 1 > sp.p_last || (t0 < sp.low && t0 + TN > a.sinks);
+}
+
+// Zeros for the values of tokens that no row sees, which may hold anything (their
+// weight is 0, but 0 times infinity is not); by threads first, first + step, ...
+template <int DP, int TN>
+__device__ __forceinline__ void blank(const AttnArgs &a, const Span<TN> &sp, uint8_t *tile, int t0, int ok, int first,
+                                      int step) {
+    for (int i = first; i < TN * (DP / 8); i += step) {
+        const int t = t0 + i / (DP / 8);
+        if (!((ok >> ((t - t0) >> 4) & 1) && t <= sp.p_last && (t >= sp.low || t < a.sinks)))
+            *reinterpret_cast<v4u *>(tile + i * 16) = (v4u){};
+    }
+}
+
+// ---------------------------------------------------------------- values that are not finite
+
+// One that some rows of a block see and others do not must not reach the
+// others, where its weight is 0; and seen, it must not meet a weight's parts of
+// both signs.  No test for them is in the tiles' loops: a block whose results
+// hold a NaN is done again, and then each tile's values that are not finite
+// become zeros before it is contracted, and are noted by row and dimension: two
+// bits, inf and -inf, both for NaN and for a sum of the two.
+template <int DP, int ROWS>
+struct Odd {
+    static constexpr int WORDS = ROWS * DP / 16;
+    uint32_t *bits;
+
+    // The values of `tokens` tokens (t0 on) at lds, by threads first, first + step, ...
+    template <bool BF16>
+    __device__ __forceinline__ void sift(const AttnArgs &a, uint8_t *tile, int tokens, int t0, int ok, const int first_row,
+                                         const int rows, int first, int step, int p_first_row) const {
+        constexpr uint32_t INF = El<BF16>::INF;
+        for (int i = first; i < tokens * (DP / 2); i += step) {
+            uint32_t *w = reinterpret_cast<uint32_t *>(tile) + i;
+            const uint32_t pair = *w;
+            const bool lo = (pair & INF) == INF, hi = (pair >> 16 & INF) == INF;
+            if (!lo && !hi) continue;
+            *w = pair & (lo ? 0xffff0000u : ~0u) & (hi ? 0x0000ffffu : ~0u);
+            const int t = i / (DP / 2), d = (((i & (DP / 2 - 1)) >> 2) ^ swizzle<DP>(t)) * 8 + (i & 3) * 2;
+            if (!(ok >> (t >> 4) & 1)) continue;
+            for (int r = 0; r < rows; ++r) {
+                const int p = p_first_row + (first_row + r) / a.group, j = t0 + t;
+                if (!(j <= p && (!a.window || p - j < a.window || j < a.sinks))) continue;
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t b = pair >> (16 * e) & 0xffffu;
+                    if ((b & INF) != INF) continue;
+                    const uint32_t kind = b == INF ? 1 : b == (INF | 0x8000u) ? 2 : 3;
+                    atomicOr(&bits[r * (DP / 16) + (d >> 4)], kind << (2 * ((d & 15) + e)));
+                }
+            }
+        }
+    }
+    // Row r's dimension d, given its result without them.
+    __device__ __forceinline__ float apply(int r, int d, float x) const {
+        const uint32_t k = bits[r * (DP / 16) + (d >> 4)] >> (2 * (d & 15)) & 3;
+        return k == 0 ? x : x + (k == 1 ? INFINITY : k == 2 ? -INFINITY : NAN);
+    }
+};
+
 // ---------------------------------------------------------------- few rows
 
 // 16 * RT rows (one token's heads, or a few tokens'): bound by the reads of K
@@ -507,6 +505,8 @@ __global__ __launch_bounds__(256, RT == 1 && DP < 256 ? 2 : 1) void few_kernel(A
     using F = Few<DP, RT>;
     __shared__ __attribute__((aligned(1024))) uint8_t ring[F::NW][F::RING];
     __shared__ float tops[F::NW][16 * RT], sums[F::NW][16 * RT];
+    __shared__ uint32_t odd_bits[Odd<DP, 16 * RT>::WORDS];
+    const Odd<DP, 16 * RT> odd = {odd_bits};
     const int split = blockIdx.x, kvh = blockIdx.y / a.blocks, block = blockIdx.y - kvh * a.blocks;
     const Seq q = seq_of(a, blockIdx.z);
     const int r0 = block * (16 * RT);
@@ -564,78 +564,86 @@ __global__ __launch_bounds__(256, RT == 1 && DP < 256 ? 2 : 1) void few_kernel(A
         w.load(a, i, a.q + (int64_t)(q.first + tok) * a.q_token + (int64_t)(kvh * a.group + row - tok * a.group) * a.q_head,
                in < sp.rows, q.n - q.m + tok);
     }
-    for (bool care = false;; care = true) {
+    bool care = false;
+    for (;;) {
         w.clear();
         if (tiles > 0) start();
         for (int i = 0; i < tiles; ++i) {
             const int t0 = sp.token(begin + i * F::NW), st = i % F::ST;
             const bool ok0 = oks >> (2 * st) & 1, ok1 = oks >> (2 * st) & 2;
-            const uint8_t *k = ring[wave] + st * 2 * F::HALF, *v = k + F::HALF;
+            uint8_t *k = ring[wave] + st * 2 * F::HALF, *v = k + F::HALF;
             const int after = 2 * (tiles - i) - 1;  // halves to come after this tile's keys, those not yet issued too
             wait_halves(min(after, 2 * F::ST - 1));
             v4f s[RT][2];
-            v4u p[RT][El<BF16>::PARTS], mask = {};
+            v4u p[RT][El<BF16>::PARTS];
             w.scores(a, k, 0, s);
-            const bool edge = care || is_edge<F::TN>(a, sp, t0) || !(ok0 && ok1);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the keys have been read: their half may be refilled
             if (i + F::ST < tiles) issue_keys(i + F::ST);
-            if (edge) {
-                w.template soften<EDGE>(a, s, t0, ok0, ok1, p);
-                mask = w.seen_mask(a, t0, sp.low, sp.p_last, ok0, ok1);
-            } else {
-                w.template soften<PLAIN>(a, s, t0, true, true, p);
-            }
+            if (is_edge<F::TN>(a, sp, t0) || !(ok0 && ok1)) w.hide(a, s, t0, ok0, ok1);
+            w.soften(s, p);
             wait_halves(min(after - 1, 2 * F::ST - 1));
-            if (care) w.template gather<CARE>(a, v, 0, t0, ok0, ok1, mask, p);
-            else if (edge) w.template gather<EDGE>(a, v, 0, t0, ok0, ok1, mask, p);
-            else w.template gather<PLAIN>(a, v, 0, t0, true, true, mask, p);
+            if (care || has_unseen<F::TN>(a, sp, t0) || !(ok0 && ok1)) {
+                blank<DP, F::TN>(a, sp, v, t0, ok0 | ok1 << 1, lane, 64);
+                if (care) odd.template sift<BF16>(a, v, F::TN, t0, ok0 | ok1 << 1, r0, sp.rows, lane, 64, q.n - q.m);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            }
+            w.gather(v, 0, p);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (i + F::ST < tiles) issue_values(i + F::ST);
         }
-        if (care || !w.any_nan()) break;  // again, and with care
-    }
 
-    // Join the waves: every one's O in its own ring (its transfers are done).
-    float *mine = reinterpret_cast<float *>(ring[wave]);
+        // Join the waves: every one's O in its own ring (its transfers are done).
+        float *mine = reinterpret_cast<float *>(ring[wave]);
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        const int in = 16 * i + (lane & 15);
-        const float l = w.whole_sum(i);
-        if (lane < 16) {
-            tops[wave][in] = w.top[i];
-            sums[wave][in] = l;
-        }
-        if (in < sp.rows) {
+        for (int i = 0; i < RT; ++i) {
+            const int in = 16 * i + (lane & 15);
+            const float l = w.whole_sum(i);
+            if (lane < 16) {
+                tops[wave][in] = w.top[i];
+                sums[wave][in] = l;
+            }
+            if (in < sp.rows) {
 #pragma unroll
-            for (int d = 0; d < DP / 16; ++d)
-                *reinterpret_cast<v4f *>(mine + in * F::OS + d * 16 + 4 * (lane >> 4)) = w.o[i][d];
+                for (int d = 0; d < DP / 16; ++d)
+                    *reinterpret_cast<v4f *>(mine + in * F::OS + d * 16 + 4 * (lane >> 4)) = w.o[i][d];
+            }
         }
-    }
-    __syncthreads();
-    const int quads = a.c.head_dim >> 2;
-    for (int i = threadIdx.x; i < sp.rows * quads; i += F::NW * 64) {
-        const int r = i / quads, d = (i - r * quads) * 4;
-        float m = -INFINITY;
+        __syncthreads();
+        const int quads = a.c.head_dim >> 2;
+        bool nan = false;
+        for (int i = threadIdx.x; i < sp.rows * quads; i += F::NW * 64) {
+            const int r = i / quads, d = (i - r * quads) * 4;
+            float m = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < F::NW; ++k) m = fmaxf(m, tops[k][r]);
-        v4f o = {};
-        float total = 0.0f;
+            for (int k = 0; k < F::NW; ++k) m = fmaxf(m, tops[k][r]);
+            v4f o = {};
+            float total = 0.0f;
 #pragma unroll
-        for (int k = 0; k < F::NW; ++k) {
-            if (tops[k][r] == -INFINITY && sums[k][r] == 0.0f) continue;  // nothing seen
-            const float f = __builtin_amdgcn_exp2f(tops[k][r] - m);
-            const v4f u = *reinterpret_cast<const v4f *>(reinterpret_cast<const float *>(ring[k]) + r * F::OS + d);
-            total = fmaf(f, sums[k][r], total);
-            o += f * u;
+            for (int k = 0; k < F::NW; ++k) {
+                if (tops[k][r] == -INFINITY && sums[k][r] == 0.0f) continue;  // nothing seen
+                const float f = __builtin_amdgcn_exp2f(tops[k][r] - m);
+                const v4f u = *reinterpret_cast<const v4f *>(reinterpret_cast<const float *>(ring[k]) + r * F::OS + d);
+                total = fmaf(f, sums[k][r], total);
+                o += f * u;
+            }
+            if (care) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = odd.apply(r, d + e, o[e]);
+            }
+            nan |= o[0] != o[0] || o[1] != o[1] || o[2] != o[2] || o[3] != o[3];
+            if (sp.active == 1) {
+                o = total == 0.0f ? (v4f){} : o / total;
+                *reinterpret_cast<v4f *>(result_row(a, q, kvh, r0 + r) + d) = o;
+            } else {
+                const int64_t at = part_row(a, q, kvh, r0 + r, split);
+                *reinterpret_cast<v4f *>(a.part_o + at * a.c.head_dim + d) = o;
+                if (d == 0) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = make_float2(m, total);
+            }
         }
-        if (sp.active == 1) {
-            o = total == 0.0f ? (v4f){} : o / total;
-            *reinterpret_cast<v4f *>(result_row(a, q, kvh, r0 + r) + d) = o;
-        } else {
-            const int64_t at = part_row(a, q, kvh, r0 + r, split);
-            *reinterpret_cast<v4f *>(a.part_o + at * a.c.head_dim + d) = o;
-            if (d == 0) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = make_float2(m, total);
-        }
+        if (care || !__syncthreads_or(nan)) return;
+        for (int i = threadIdx.x; i < odd.WORDS; i += F::NW * 64) odd_bits[i] = 0;
+        __syncthreads();
+        care = true;
     }
 }
 
@@ -653,6 +661,8 @@ template <bool BF16, int DP, bool FULL>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a) {
     using M = Many<DP>;
     __shared__ __attribute__((aligned(1024))) uint8_t stage[2][M::STAGE];
+    __shared__ uint32_t odd_bits[Odd<DP, 128>::WORDS];
+    const Odd<DP, 128> odd = {odd_bits};
     const int split = blockIdx.y;
     // Blocks of one (sequence, key-value head) share its keys and values: they
     // go to one of the eight XCDs (workgroups are dealt to them in turn) as far
@@ -708,8 +718,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
         w.load(a, i, a.q + (int64_t)(q.first + tok) * a.q_token + (int64_t)(kvh * a.group + row - tok * a.group) * a.q_head,
                in < sp.rows, q.n - q.m + tok);
     }
-    const bool busy = wave * 32 < sp.rows;
-    for (bool care = false;; care = true) {
+    bool care = false;
+    for (;;) {
         w.clear();
         for (int u = begin; u < end; ++u) {
             wait_vm<0>();
@@ -718,24 +728,27 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
             asm volatile("" ::: "memory");
             const int ok = oks >> (4 * (u & 1)) & 15, t0 = sp.token(u);
             if (u + 1 < end) issue(u + 1);
-            if (!busy) continue;
-            const uint8_t *k = stage[u & 1], *v = k + M::HALF;
-            if (care) {
+            uint8_t *k = stage[u & 1], *v = k + M::HALF;
+            if (care || has_unseen<M::TN>(a, sp, t0) || ok != 15) {
+                blank<DP, M::TN>(a, sp, v, t0, ok, threadIdx.x, 256);
+                if (care) odd.template sift<BF16>(a, v, M::TN, t0, ok, r0, sp.rows, threadIdx.x, 256, q.n - q.m);
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            }
+            const bool edge = is_edge<M::TN>(a, sp, t0) || ok != 15;
 #pragma unroll 1
-                for (int i = 0; i < 2; ++i)
-                    w.template tile32<CARE>(a, k, v, 32 * i, t0 + 32 * i, ok >> (2 * i) & 1, ok >> (2 * i + 1) & 1, sp.low,
-                                            sp.p_last);
-            } else if (is_edge<M::TN>(a, sp, t0) || ok != 15) {
-#pragma unroll 1
-                for (int i = 0; i < 2; ++i)
-                    w.template tile32<EDGE>(a, k, v, 32 * i, t0 + 32 * i, ok >> (2 * i) & 1, ok >> (2 * i + 1) & 1, sp.low,
-                                            sp.p_last);
-            } else {
-                w.template tile32<PLAIN>(a, k, v, 0, t0, true, true, 0, 0);
-                w.template tile32<PLAIN>(a, k, v, 32, t0 + 32, true, true, 0, 0);
+            for (int i = 0; i < 2; ++i) {
+                v4f x[M::RT][2];
+                v4u p[M::RT][El<BF16>::PARTS];
+                w.scores(a, k, 32 * i, x);
+                if (edge) w.hide(a, x, t0 + 32 * i, ok >> (2 * i) & 1, ok >> (2 * i + 1) & 1);
+                w.soften(x, p);
+                w.gather(v, 32 * i, p);
             }
         }
-        if (care || !__syncthreads_or(w.any_nan())) break;  // (the barrier also frees both stages)
+        if (care || !__syncthreads_or(w.any_nan())) break;
+        for (int i = threadIdx.x; i < odd.WORDS; i += 256) odd_bits[i] = 0;
+        __syncthreads();  // (which also frees both stages)
+        care = true;
         if (begin < end) start();
     }
 
@@ -757,7 +770,12 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d) {
             const int e = d * 16 + 4 * (lane >> 4);
-            if (FULL || e < a.c.head_dim) *reinterpret_cast<v4f *>(out + e) = w.o[i][d] * f;
+            v4f x = w.o[i][d] * f;
+            if (care) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) x[c] = odd.apply(in, e + c, x[c]);
+            }
+            if (FULL || e < a.c.head_dim) *reinterpret_cast<v4f *>(out + e) = x;
         }
     }
 }
