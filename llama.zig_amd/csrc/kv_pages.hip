@@ -96,10 +96,26 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(const int32_t *__res
     const Plan p = plan_at(ws, n_pages);
     for (int w = threadIdx.x; w < words; w += PLAN_THREADS) used[w] = 0;
     __syncthreads();
-    for (int64_t i = threadIdx.x; i < n_seqs * width; i += PLAN_THREADS) {
-        const int64_t row = i / width;
-        const int e = entry_of(table, stride, lens, row, i - row * width, page_shift, n_pages);
-        if (e >= 0) atomicOr(&used[e >> 5], 1u << (e & 31));
+    // A wave takes ROWS rows at a time, whose loads are in flight together.
+    constexpr int ROWS = 4, WAVES = PLAN_THREADS / 64;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (int64_t row = wave * ROWS; row < n_seqs; row += WAVES * ROWS) {
+        int64_t n[ROWS], most = 0;
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const int64_t len = row + i < n_seqs ? lens[row + i] : 0;
+            n[i] = len <= 0 ? 0 : ((len - 1) >> page_shift) + 1;
+            if (n[i] > width) n[i] = width;
+            most = most > n[i] ? most : n[i];
+        }
+        for (int64_t col = lane; col < most; col += 64) {
+            int e[ROWS];
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) e[i] = col < n[i] ? table[(row + i) * stride + col] : -1;
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i)
+                if (e[i] >= 0 && e[i] < n_pages) atomicOr(&used[e[i] >> 5], 1u << (e[i] & 31));
+        }
     }
     __syncthreads();
     const int w0 = min(words, (int)threadIdx.x * per), w1 = min(words, w0 + per);

@@ -7,10 +7,11 @@
 // argument of sincospi in [-1, 1), so that small angles keep their relative
 // precision too.
 //
-// HBM bound: one pass, 16-byte loads and stores.  A workgroup takes rows
-// (heads of q, then k, then v) of one token; a thread eight elements of one
-// row: four pairs, whose turns it computes itself (four sincospi hide behind
-// the loads).
+// HBM bound: one pass, 16-byte loads.  A workgroup takes the rows (heads of q,
+// then k, then v) of one token; a thread eight elements of a row, four pairs,
+// and computes their turns once for all of its rows, while other workgroups
+// load.  8192 tokens of 32 + 8 + 8 heads of 128 (369 MB): 69 us, 5.3 TB/s, what
+// a large copy reaches on this card; one such token 2.5 us, a launch.
 #include <math.h>
 
 #include "kv_cache.h"
@@ -20,6 +21,7 @@ using namespace kvc;
 namespace {
 
 constexpr int THREADS = 256;
+constexpr int64_t FEW_TOKENS = 512;
 
 struct Rows {
     const float *src;
@@ -56,8 +58,7 @@ __device__ __forceinline__ void put(float *d, float x) { *d = x; }
 template <bool BF16>
 __device__ __forceinline__ void put(uint16_t *d, float x) { *d = to16<BF16>(x); }
 
-// Any head_dim, n_dims, alignment: one pair or one plain element per thread
-// and step.
+// One pair or one plain element per lane and step.
 template <int LAYOUT, bool BF16, class Out>
 __device__ __forceinline__ void row_any(const RopeArgs &a, const float *x, Out *d, int64_t pos, bool rotate, int lane,
                                         int lanes) {
@@ -73,33 +74,116 @@ __device__ __forceinline__ void row_any(const RopeArgs &a, const float *x, Out *
     for (int e = 2 * half + lane; e < a.head_dim; e += lanes) put<BF16>(d + e, x[e]);
 }
 
+// Where row r (of q, then k, then v) of token t comes from, and where it goes:
+// one of the two destinations, or none (false).
+struct Place {
+    const float *from;
+    float *to;
+    uint16_t *stored;
+    bool rotate;
+};
+
+__device__ __forceinline__ bool place_of(const RopeArgs &a, int64_t t, int r, int slot, Place *p) {
+    if (r < a.q.n) {
+        *p = {a.q.src + t * a.q.token + r * a.q.head, a.dst + t * a.dst_token + r * a.dst_head, nullptr, true};
+        return true;
+    }
+    if (slot < 0 || (slot >> a.cache.page_shift) >= a.cache.n_pages) return false;
+    const bool key = r < a.q.n + a.k.n;
+    const int h = key ? r - a.q.n : r - a.q.n - a.k.n;
+    const Rows &in = key ? a.k : a.v;
+    *p = {in.src + t * in.token + h * in.head, nullptr,
+          (key ? a.cache.k : a.cache.v) + (int64_t)(slot >> a.cache.page_shift) * a.cache.page_stride +
+              (int64_t)(slot & ((1 << a.cache.page_shift) - 1)) * a.cache.token_stride + h * a.cache.head_stride,
+          key};
+    return true;
+}
+
+// Any size and alignment: a wave per row.
 template <int LAYOUT, bool BF16>
-__global__ __launch_bounds__(THREADS) void rope_kernel(RopeArgs a) {
+__global__ __launch_bounds__(THREADS) void rope_any_kernel(RopeArgs a) {
     const int64_t t = blockIdx.x;
-    const int64_t pos = a.pos[t];
     const int rows = a.q.n + a.k.n + a.v.n, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int slot = a.slots ? a.slots[t] : -1;
     for (int r = blockIdx.y * (THREADS / 64) + wave; r < rows; r += gridDim.y * (THREADS / 64)) {
-        if (r < a.q.n) {
-            row_any<LAYOUT, BF16>(a, a.q.src + t * a.q.token + r * a.q.head, a.dst + t * a.dst_token + r * a.dst_head,
-                                  pos, true, lane, 64);
-            continue;
-        }
-        const int slot = a.slots[t];
-        if (slot < 0 || (slot >> a.cache.page_shift) >= a.cache.n_pages) continue;
-        const bool key = r < a.q.n + a.k.n;
-        const int h = key ? r - a.q.n : r - a.q.n - a.k.n;
-        const Rows &in = key ? a.k : a.v;
-        uint16_t *d = (key ? a.cache.k : a.cache.v) + (int64_t)(slot >> a.cache.page_shift) * a.cache.page_stride +
-                      (int64_t)(slot & ((1 << a.cache.page_shift) - 1)) * a.cache.token_stride + h * a.cache.head_stride;
-        row_any<LAYOUT, BF16>(a, in.src + t * in.token + h * in.head, d, pos, key, lane, 64);
+        Place p;
+        if (!place_of(a, t, r, slot, &p)) continue;
+        if (p.to) row_any<LAYOUT, BF16>(a, p.from, p.to, a.pos[t], p.rotate, lane, 64);
+        else row_any<LAYOUT, BF16>(a, p.from, p.stored, a.pos[t], p.rotate, lane, 64);
     }
 }
+
+// Eight elements of a row per thread, `units` threads a row, as many rows of
+// one token at a time as fit; a thread's rows share its four turns.  Needs
+// head_dim and n_dims multiples of 8 and 16-byte aligned rows.
+template <int LAYOUT, bool BF16>
+__global__ __launch_bounds__(THREADS) void rope_kernel(RopeArgs a, int units) {
+    const int64_t t = blockIdx.x;
+    const int unit = threadIdx.x % units, at_once = THREADS / units;
+    if (threadIdx.x >= at_once * units) return;
+    const int rows = a.q.n + a.k.n + a.v.n, slot = a.slots ? a.slots[t] : -1;
+    const bool turned = unit < a.half / 4;  // else a unit behind the rotated elements
+    const bool apart = LAYOUT == HIP_QMM_ROPE_HALF && turned;
+    const int e0 = apart ? 4 * unit : 8 * unit, e1 = apart ? e0 + a.half : e0 + 4;  // the unit's two quads
+    float c[4], s[4];
+    if (turned) {
+        const int64_t pos = a.pos[t];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) turn(a, pos, 4 * unit + i, &c[i], &s[i]);
+    }
+    for (int r = threadIdx.x / units + at_once * blockIdx.y; r < rows; r += at_once * gridDim.y) {
+        Place p;
+        if (!place_of(a, t, r, slot, &p)) continue;
+        const float4 x = *reinterpret_cast<const float4 *>(p.from + e0), y = *reinterpret_cast<const float4 *>(p.from + e1);
+        float u[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
+        if (turned && p.rotate) {
+            float f[4], g[4];  // first and second members of the four pairs
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f[j] = LAYOUT == HIP_QMM_ROPE_HALF ? u[j] : j < 2 ? u[2 * j] : v[2 * j - 4];
+                g[j] = LAYOUT == HIP_QMM_ROPE_HALF ? v[j] : j < 2 ? u[2 * j + 1] : v[2 * j - 3];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float h = fmaf(f[j], c[j], -(g[j] * s[j]));
+                g[j] = fmaf(f[j], s[j], g[j] * c[j]);
+                f[j] = h;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u[j] = LAYOUT == HIP_QMM_ROPE_HALF ? f[j] : j & 1 ? g[j >> 1] : f[j >> 1];
+                v[j] = LAYOUT == HIP_QMM_ROPE_HALF ? g[j] : j & 1 ? g[2 + (j >> 1)] : f[2 + (j >> 1)];
+            }
+        }
+        if (p.to) {
+            *reinterpret_cast<float4 *>(p.to + e0) = make_float4(u[0], u[1], u[2], u[3]);
+            *reinterpret_cast<float4 *>(p.to + e1) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+            *reinterpret_cast<ushort4 *>(p.stored + e0) =
+                make_ushort4(to16<BF16>(u[0]), to16<BF16>(u[1]), to16<BF16>(u[2]), to16<BF16>(u[3]));
+            *reinterpret_cast<ushort4 *>(p.stored + e1) =
+                make_ushort4(to16<BF16>(v[0]), to16<BF16>(v[1]), to16<BF16>(v[2]), to16<BF16>(v[3]));
+        }
+    }
+}
+
+bool aligned(const void *p, int64_t token, int64_t head) { return !((uintptr_t)p & 15) && !((token | head) & 3); }
 
 template <int LAYOUT, bool BF16>
 int launch(const RopeArgs &a, int64_t n_tokens, hipStream_t s) {
     const int rows = a.q.n + a.k.n + a.v.n;
-    const dim3 grid((unsigned)n_tokens, (unsigned)((rows + THREADS / 64 - 1) / (THREADS / 64)));
-    hipLaunchKernelGGL((rope_kernel<LAYOUT, BF16>), grid, dim3(THREADS), 0, s, a);
+    if (a.head_dim % 8 == 0 && a.half % 4 == 0 && aligned(a.q.src, a.q.token, a.q.head) &&
+        aligned(a.dst, a.dst_token, a.dst_head) && aligned(a.k.src, a.k.token, a.k.head) && aligned(a.v.src, a.v.token, a.v.head)) {
+        // A workgroup per token, or for few tokens one for each pass over its rows: of 8192, 1024 and 256 tokens'
+        // 48 rows of 128 a workgroup per token took 69.1, 9.4 and 4.4 us, three per token 72.1, 11.0 and 4.3.
+        const int units = a.head_dim / 8, at_once = THREADS / units;
+        const int passes = n_tokens < FEW_TOKENS ? (rows + at_once - 1) / at_once : 1;
+        hipLaunchKernelGGL((rope_kernel<LAYOUT, BF16>), dim3((unsigned)n_tokens, (unsigned)passes), dim3(THREADS), 0, s, a,
+                           units);
+    } else {
+        const dim3 grid((unsigned)n_tokens, (unsigned)((rows + THREADS / 64 - 1) / (THREADS / 64)));
+        hipLaunchKernelGGL((rope_any_kernel<LAYOUT, BF16>), grid, dim3(THREADS), 0, s, a);
+    }
     return (int)hipGetLastError();
 }
 
