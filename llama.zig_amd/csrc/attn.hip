@@ -103,15 +103,22 @@ struct Seq {
     int first, m, n;  // its first row of q, its query count, its length
 };
 
-__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int s) {
-    int lo = s, hi = s + 1;
-    if (a.q_starts) {
-        lo = max(a.q_starts[s], 0);
-        hi = min(a.q_starts[s + 1], a.n_tokens);
-    }
-    const int64_t most = a.table_stride << a.c.page_shift;
-    return {lo, max(hi - lo, 0), (int)min((int64_t)max(a.lens[s], 0), most)};
+struct Rowspan {
+    int first, m;
+};
+
+__device__ __forceinline__ Rowspan rows_of(const AttnArgs &a, int s) {
+    if (!a.q_starts) return {s, 1};
+    const int lo = max(a.q_starts[s], 0), hi = min(a.q_starts[s + 1], a.n_tokens);
+    return {lo, max(hi - lo, 0)};
 }
+
+__device__ __forceinline__ Seq seq_of(const AttnArgs &a, const Rowspan &r, int s) {
+    const int64_t most = a.table_stride << a.c.page_shift;
+    return {r.first, r.m, (int)min((int64_t)max(a.lens[s], 0), most)};
+}
+
+__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int s) { return seq_of(a, rows_of(a, s), s); }
 
 // Rows [r0, r0 + rows) of a sequence's head group, their positions, and the
 // tiles of TN tokens that any of them sees (from token `low` on, or a first one): first `sink` tiles of the tokens
@@ -242,12 +249,13 @@ struct Rows {
     float top[RT], sum[RT];   // running maximum (log2), and this lane's share of the sum
     int pos[RT], low[RT];     // the row's position (-1: none), the first token of its window
 
-    // Row 16 * i + lane % 16 of the block, at x if it is valid.
-    __device__ __forceinline__ void load(const AttnArgs &a, int i, const float *x, bool valid, int position) {
+    // Row 16 * i + lane % 16 of the block as it is, at x if it is valid.
+    struct Raw {
+        float v[KS][8];
+    };
+    static __device__ __forceinline__ Raw fetch(const AttnArgs &a, const float *x, bool valid) {
         const int g = (threadIdx.x & 63) >> 4, D = a.c.head_dim;
-        pos[i] = valid ? position : -1;
-        low[i] = a.window ? pos[i] - a.window + 1 : 0;
-        float v[KS][8], big = 0.0f;
+        Raw raw;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const int d = ks * 32 + g * 8;
@@ -256,9 +264,18 @@ struct Rows {
                 u = *reinterpret_cast<const float4 *>(x + d);
                 w = *reinterpret_cast<const float4 *>(x + d + 4);
             }
-            v[ks][0] = u.x, v[ks][1] = u.y, v[ks][2] = u.z, v[ks][3] = u.w;
-            v[ks][4] = w.x, v[ks][5] = w.y, v[ks][6] = w.z, v[ks][7] = w.w;
+            float *v = raw.v[ks];
+            v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w, v[4] = w.x, v[5] = w.y, v[6] = w.z, v[7] = w.w;
         }
+        return raw;
+    }
+
+    // Its position (-1: none), its scale and its parts.
+    __device__ __forceinline__ void take_row(const AttnArgs &a, int i, Raw &raw, int position) {
+        auto &v = raw.v;
+        float big = 0.0f;
+        pos[i] = position;
+        low[i] = a.window ? position - a.window + 1 : 0;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -508,18 +525,31 @@ __global__ __launch_bounds__(256, RT == 1 && DP < 256 ? 2 : 1) void few_kernel(A
     __shared__ uint32_t odd_bits[Odd<DP, 16 * RT>::WORDS];
     const Odd<DP, 16 * RT> odd = {odd_bits};
     const int split = blockIdx.x, kvh = blockIdx.y / a.blocks, block = blockIdx.y - kvh * a.blocks;
-    const Seq q = seq_of(a, blockIdx.z);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int r0 = block * (16 * RT);
-    if (r0 >= q.m * a.group) return;
+    // Three loads that do not wait for one another: the rows, the length, and
+    // the pages of the tile that is this wave's first where the length does
+    // not change the split and there is no window.
+    const Rowspan own = rows_of(a, blockIdx.z);
+    if (r0 >= own.m * a.group) return;
+    typename Rows<BF16, DP, FULL, RT>::Raw raw[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const int row = r0 + 16 * i + (lane & 15), tok = row / a.group;
+        raw[i] = Rows<BF16, DP, FULL, RT>::fetch(
+            a, a.q + (int64_t)(own.first + tok) * a.q_token + (int64_t)(kvh * a.group + row - tok * a.group) * a.q_head,
+            row < own.m * a.group);
+    }
+    Pages pages = {a.table + blockIdx.z * a.table_stride, a.table_stride, 0, -1};
+    pages.load((split * a.per + wave) * F::TN >> a.c.page_shift, a.c.n_pages);
+    const Seq q = seq_of(a, own, blockIdx.z);
     const Span<F::TN> sp(a, q, r0, 16 * RT);
     if (split >= sp.active) return;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
 
     const int64_t head = (int64_t)kvh * a.c.head_stride;
     const int begin = split * sp.per + wave, end = min(sp.count, (split + 1) * sp.per);
     const int tiles = begin < end ? (end - begin + F::NW - 1) / F::NW : 0;
     const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_addr(ring[wave]));
-    Pages pages = {a.table + blockIdx.z * a.table_stride, a.table_stride, 0, -1};
     const Loader<DP> loader(a);
     const int more = a.c.page_shift == 4 ? 1 : 0;  // a tile spans two pages of 16 tokens
     uint32_t oks = 0;  // two bits per stage
@@ -549,7 +579,6 @@ __global__ __launch_bounds__(256, RT == 1 && DP < 256 ? 2 : 1) void few_kernel(A
         else wait_vm<0>();
     };
     auto start = [&] {
-        pages.load(sp.token(begin) >> a.c.page_shift, a.c.n_pages);
 #pragma unroll
         for (int i = 0; i < F::ST; ++i)
             if (i < tiles) {
@@ -560,9 +589,8 @@ __global__ __launch_bounds__(256, RT == 1 && DP < 256 ? 2 : 1) void few_kernel(A
     Rows<BF16, DP, FULL, RT> w;
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-        const int in = 16 * i + (lane & 15), row = r0 + in, tok = row / a.group;
-        w.load(a, i, a.q + (int64_t)(q.first + tok) * a.q_token + (int64_t)(kvh * a.group + row - tok * a.group) * a.q_head,
-               in < sp.rows, q.n - q.m + tok);
+        const int in = 16 * i + (lane & 15);
+        w.take_row(a, i, raw[i], in < sp.rows ? q.n - q.m + (r0 + in) / a.group : -1);
     }
     bool care = false;
     for (;;) {
@@ -715,8 +743,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
 #pragma unroll
     for (int i = 0; i < M::RT; ++i) {
         const int in = wave * 32 + 16 * i + (lane & 15), row = r0 + in, tok = row / a.group;
-        w.load(a, i, a.q + (int64_t)(q.first + tok) * a.q_token + (int64_t)(kvh * a.group + row - tok * a.group) * a.q_head,
-               in < sp.rows, q.n - q.m + tok);
+        auto raw = w.fetch(
+            a, a.q + (int64_t)(q.first + tok) * a.q_token + (int64_t)(kvh * a.group + row - tok * a.group) * a.q_head,
+            in < sp.rows);
+        w.take_row(a, i, raw, in < sp.rows ? q.n - q.m + tok : -1);
     }
     bool care = false;
     for (;;) {
@@ -865,7 +895,7 @@ Plan plan_of(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t max_q, int
     int64_t splits = (want + grid - 1) / grid;
     if (splits > (tiles + least - 1) / least) splits = (tiles + least - 1) / least;
     if (splits > MAX_SPLITS) splits = MAX_SPLITS;
-    if (splits < 1) splits = 1;
+    if (splits < 1 || (p.few() && tiles <= 14)) splits = 1;
     int64_t per = (tiles + splits - 1) / splits;
     per = (per + least - 1) / least * least;
     p.per = (int)per;

@@ -12,7 +12,7 @@ import ctypes
 
 import torch
 
-from . import HipQmmError, _check, _stream
+from . import HipQmmError, _check
 from . import lib as _base_lib
 
 ROPE_LAYOUTS = {"interleaved": 0, "half": 2}
@@ -50,14 +50,19 @@ def _lib():
     return _bound
 
 
+# The checks build their messages only when they refuse: a step's call lasts a few microseconds.
 def _need(ok, what):
     if not ok:
         raise HipQmmError(what)
 
 
+def _raw_stream(t):
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
 def _int32(t, n, name):
-    _need(t.dtype == torch.int32 and t.is_cuda and t.is_contiguous() and t.numel() == n,
-          f"{name} must be {n} contiguous int32 values on the GPU")
+    if not (t.dtype is torch.int32 and t.is_cuda and t.numel() == n and t.is_contiguous()):
+        raise HipQmmError(f"{name} must be {n} contiguous int32 values on the GPU")
 
 
 class PagedKV:
@@ -94,30 +99,44 @@ def rope_steps(n_dims: int, freq_base=10000.0, freq_scale=1.0, ext_factor=0.0, a
 
 
 def _heads(t, name):
-    _need(t.is_cuda and t.dtype == torch.float32 and t.dim() == 3 and t.stride(2) == 1,
-          f"{name} must be f32 [n_tokens, n_heads, head_dim] on the GPU, head_dim contiguous")
+    """Token and head stride of f32 [n_tokens, n_heads, head_dim]."""
+    if not (t.is_cuda and t.dtype is torch.float32 and t.dim() == 3):
+        raise HipQmmError(f"{name} must be f32 [n_tokens, n_heads, head_dim] on the GPU")
+    st, sh, sd = t.stride()
+    if sd != 1:
+        raise HipQmmError(f"{name}'s head_dim must be contiguous")
+    return st, sh
+
+
+def _result(out, x):
+    """out, checked, or a new tensor of x's shape; with its strides."""
+    if out is None:
+        out = torch.empty(x.shape, dtype=torch.float32, device=x.device)
+        return out, out.shape[1] * out.shape[2], out.shape[2]
+    st, sh = _heads(out, "out")
+    _need(out.shape == x.shape, "out must have the shape of its input")
+    return out, st, sh
 
 
 def _rotation(pos, steps, n, layout):
     _int32(pos, n, "pos")
-    _need(steps.dtype == torch.int64 and steps.is_cuda and steps.dim() == 1 and steps.is_contiguous(),
-          "steps must be what rope_steps returns")
-    _need(layout in ROPE_LAYOUTS, f"layout must be one of {sorted(ROPE_LAYOUTS)}")
-    return ROPE_LAYOUTS[layout]
+    if not (steps.dtype is torch.int64 and steps.is_cuda and steps.dim() == 1 and steps.is_contiguous()):
+        raise HipQmmError("steps must be what rope_steps returns")
+    mode = ROPE_LAYOUTS.get(layout)
+    if mode is None:
+        raise HipQmmError(f"layout must be one of {sorted(ROPE_LAYOUTS)}")
+    return mode, 2 * steps.numel()
 
 
 def rope(x: torch.Tensor, pos: torch.Tensor, steps: torch.Tensor, layout="half", mscale=1.0, out=None):
     """x f32 [n_tokens, n_heads, head_dim] with the first 2 * len(steps)
     elements of each head rotated by pos int32 [n_tokens]; out may be x."""
-    _heads(x, "x")
-    mode = _rotation(pos, steps, x.shape[0], layout)
-    out = torch.empty(x.shape, dtype=torch.float32, device=x.device) if out is None else out
-    _heads(out, "out")
-    _need(out.shape == x.shape, "out must have x's shape")
+    xt, xh = _heads(x, "x")
     n, h, d = x.shape
-    _check(_lib().hip_qmm_rope_f32(x.data_ptr(), n, h, d, x.stride(0), x.stride(1), pos.data_ptr(), steps.data_ptr(),
-                                   2 * steps.numel(), mode, mscale, out.data_ptr(), out.stride(0), out.stride(1),
-                                   _stream()), "hip_qmm_rope_f32")
+    mode, n_dims = _rotation(pos, steps, n, layout)
+    out, ot, oh = _result(out, x)
+    _check(_lib().hip_qmm_rope_f32(x.data_ptr(), n, h, d, xt, xh, pos.data_ptr(), steps.data_ptr(), n_dims, mode, mscale,
+                                   out.data_ptr(), ot, oh, _raw_stream(x)), "hip_qmm_rope_f32")
     return out
 
 
@@ -126,27 +145,28 @@ def rope_kv_store(q, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, steps:
     """Rotates q and k f32 [n_tokens, heads, head_dim], stores the rotated k and
     the plain v at cache slots int32 [n_tokens] (page * page_size + token;
     outside the cache: not stored) and returns the rotated q.  q may be None."""
-    _heads(k, "k")
-    _heads(v, "v")
+    kt, kh = _heads(k, "k")
     n, h, d = k.shape
-    _need(v.shape == k.shape and v.stride() == k.stride(), "k and v must have the same shape and strides")
-    _need((h, d) == (kv.n_kv_heads, kv.head_dim), "k and v must have the cache's heads and head_dim")
-    mode = _rotation(pos, steps, n, layout)
+    if _heads(v, "v") != (kt, kh) or v.shape != k.shape:
+        raise HipQmmError("k and v must have the same shape and strides")
+    if h != kv.n_kv_heads or d != kv.head_dim:
+        raise HipQmmError("k and v must have the cache's heads and head_dim")
+    mode, n_dims = _rotation(pos, steps, n, layout)
     _int32(slots, n, "slots")
-    if q is None:
-        _check(_lib().hip_qmm_rope_kv_store(None, 0, 0, 0, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), n,
-                                            pos.data_ptr(), steps.data_ptr(), 2 * steps.numel(), mode, mscale, None, 0,
-                                            0, kv._p, slots.data_ptr(), _stream()), "hip_qmm_rope_kv_store")
-        return None
-    _heads(q, "q")
-    _need(q.shape[0] == n and q.shape[2] == d, "q and k disagree on the tokens or head_dim")
-    out = torch.empty(q.shape, dtype=torch.float32, device=q.device) if out is None else out
-    _heads(out, "out")
-    _need(out.shape == q.shape, "out must have q's shape")
-    _check(_lib().hip_qmm_rope_kv_store(q.data_ptr(), q.shape[1], q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(),
-                                        k.stride(0), k.stride(1), n, pos.data_ptr(), steps.data_ptr(),
-                                        2 * steps.numel(), mode, mscale, out.data_ptr(), out.stride(0), out.stride(1),
-                                        kv._p, slots.data_ptr(), _stream()), "hip_qmm_rope_kv_store")
+    qp = op = None
+    heads = qt = qh = ot = oh = 0
+    if q is not None:
+        qt, qh = _heads(q, "q")
+        nq, heads, dq = q.shape
+        if nq != n or dq != d:
+            raise HipQmmError("q and k disagree on the tokens or head_dim")
+        out, ot, oh = _result(out, q)
+        qp, op = q.data_ptr(), out.data_ptr()
+    else:
+        out = None
+    _check(_lib().hip_qmm_rope_kv_store(qp, heads, qt, qh, k.data_ptr(), v.data_ptr(), kt, kh, n, pos.data_ptr(),
+                                        steps.data_ptr(), n_dims, mode, mscale, op, ot, oh, kv._p, slots.data_ptr(),
+                                        _raw_stream(k)), "hip_qmm_rope_kv_store")
     return out
 
 
@@ -154,6 +174,12 @@ def attn_paged_workspace_size(kv: PagedKV, n_heads: int, n_seqs: int, n_tokens: 
                               window=0, sinks=0) -> int:
     return int(_lib().hip_qmm_attn_paged_workspace_size(kv._p, n_heads, n_seqs, n_tokens, max_q, max_kv, window,
                                                         sinks))
+
+
+def _table(t):
+    if not (t.dtype is torch.int32 and t.is_cuda and t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]):
+        raise HipQmmError("page_table must be int32 [n_seqs, width] on the GPU, its rows contiguous and apart")
+    return t.shape
 
 
 def attn_paged(q: torch.Tensor, kv: PagedKV, page_table: torch.Tensor, kv_lens: torch.Tensor, q_starts=None,
@@ -166,39 +192,40 @@ def attn_paged(q: torch.Tensor, kv: PagedKV, page_table: torch.Tensor, kv_lens: 
     window is 0, p - j < window or j < sinks; entries outside the pool hide
     their tokens; nothing seen gives zeros.  max_kv: the longest length that
     the host knows of.  scale: head_dim ** -0.5 by default."""
-    _heads(q, "q")
+    qt, qh = _heads(q, "q")
     n, h, d = q.shape
-    _need(d == kv.head_dim, "q must have the cache's head_dim")
-    _need(page_table.dtype == torch.int32 and page_table.is_cuda and page_table.dim() == 2 and
-          page_table.stride(1) == 1 and page_table.stride(0) >= page_table.shape[1],
-          "page_table must be int32 [n_seqs, width] on the GPU")
-    n_seqs, width = page_table.shape
+    if d != kv.head_dim:
+        raise HipQmmError("q must have the cache's head_dim")
+    n_seqs, width = _table(page_table)
     _int32(kv_lens, n_seqs, "kv_lens")
+    starts = None
     if q_starts is None:
-        _need(n == n_seqs, "one token per sequence without q_starts")
+        if n != n_seqs:
+            raise HipQmmError("one token per sequence without q_starts")
         max_q = 1 if n else 0
     else:
         _int32(q_starts, n_seqs + 1, "q_starts")
+        starts = q_starts.data_ptr()
         max_q = n if max_q is None else max_q
-    if page_table.stride(0) != width:  # the row stride is the width that lengths are cut to
+    if not page_table.is_contiguous():  # the row stride is the width that lengths are cut to
         page_table = page_table.contiguous()
-    if max_kv is None or max_kv > width * kv.page_size:
-        max_kv = width * kv.page_size
-    scale = d ** -0.5 if scale is None else scale
-    out = torch.empty(q.shape, dtype=torch.float32, device=q.device) if out is None else out
-    _heads(out, "out")
-    _need(out.shape == q.shape, "out must have q's shape")
+    most = width * kv.page_size
+    max_kv = most if max_kv is None or max_kv > most else max_kv
+    out, ot, oh = _result(out, q)
     L = _lib()
     need = L.hip_qmm_attn_paged_workspace_size(kv._p, h, n_seqs, n, max_q, max_kv, window, sinks)
     if workspace is None:
-        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
-    elif workspace.numel() < need:
-        raise HipQmmError(f"workspace too small: {workspace.numel()} < {need}")
-    _check(L.hip_qmm_attn_paged(kv._p, q.data_ptr(), h, q.stride(0), q.stride(1),
-                                None if q_starts is None else q_starts.data_ptr(), n_seqs, n, max_q,
-                                page_table.data_ptr(), width, kv_lens.data_ptr(), max_kv, scale, window, sinks,
-                                out.data_ptr(), out.stride(0), out.stride(1), workspace.data_ptr(),
-                                workspace.numel(), _stream()), "hip_qmm_attn_paged")
+        have, wp = need, None
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            wp = workspace.data_ptr()
+    else:
+        have, wp = workspace.numel(), workspace.data_ptr()
+        if have < need:
+            raise HipQmmError(f"workspace too small: {have} < {need}")
+    _check(L.hip_qmm_attn_paged(kv._p, q.data_ptr(), h, qt, qh, starts, n_seqs, n, max_q, page_table.data_ptr(), width,
+                                kv_lens.data_ptr(), max_kv, d ** -0.5 if scale is None else scale, window, sinks,
+                                out.data_ptr(), ot, oh, wp, have, _raw_stream(q)), "hip_qmm_attn_paged")
     return out
 
 
@@ -211,7 +238,7 @@ def copy_pages(kv: PagedKV, src: torch.Tensor, dst: torch.Tensor, n_tokens=None)
     if n_tokens is not None:
         _int32(n_tokens, n, "n_tokens")
     _check(_lib().hip_qmm_kv_copy_pages(kv._p, src.data_ptr(), dst.data_ptr(),
-                                        None if n_tokens is None else n_tokens.data_ptr(), n, _stream()),
+                                        None if n_tokens is None else n_tokens.data_ptr(), n, _raw_stream(kv.k)),
            "hip_qmm_kv_copy_pages")
 
 
@@ -220,13 +247,11 @@ def compact_pages(kv: PagedKV, page_table: torch.Tensor, kv_lens: torch.Tensor, 
     the pool: (the table with their new numbers and -1 elsewhere, int32; the
     count of pages in use, int32 [1]), both on the device.  out may be
     page_table."""
-    _need(page_table.dtype == torch.int32 and page_table.is_cuda and page_table.dim() == 2 and
-          page_table.stride(1) == 1, "page_table must be int32 [n_seqs, width] on the GPU")
-    n_seqs, width = page_table.shape
+    n_seqs, width = _table(page_table)
     _int32(kv_lens, n_seqs, "kv_lens")
-    out = torch.empty((n_seqs, width), dtype=torch.int32, device=page_table.device) if out is None else out
-    _need(out.dtype == torch.int32 and out.is_cuda and out.shape == page_table.shape and out.stride(1) == 1,
-          "out must be int32 of page_table's shape")
+    if out is None:
+        out = torch.empty((n_seqs, width), dtype=torch.int32, device=page_table.device)
+    _need(_table(out) == page_table.shape, "out must have page_table's shape")
     n_live = torch.empty(1, dtype=torch.int32, device=page_table.device)
     L = _lib()
     need = L.hip_qmm_kv_compact_workspace_size(kv._p)
@@ -236,5 +261,5 @@ def compact_pages(kv: PagedKV, page_table: torch.Tensor, kv_lens: torch.Tensor, 
         raise HipQmmError(f"workspace too small: {workspace.numel()} < {need}")
     _check(L.hip_qmm_kv_compact(kv._p, page_table.data_ptr(), page_table.stride(0), width, kv_lens.data_ptr(), n_seqs,
                                 out.data_ptr(), out.stride(0), n_live.data_ptr(), workspace.data_ptr(),
-                                workspace.numel(), _stream()), "hip_qmm_kv_compact")
+                                workspace.numel(), _raw_stream(out)), "hip_qmm_kv_compact")
     return out, n_live
