@@ -524,13 +524,17 @@ __global__ __launch_bounds__(256, RT == 1 && DP < 256 ? 2 : 1) void few_kernel(A
     __shared__ float tops[F::NW][16 * RT], sums[F::NW][16 * RT];
     __shared__ uint32_t odd_bits[Odd<DP, 16 * RT>::WORDS];
     const Odd<DP, 16 * RT> odd = {odd_bits};
-    const int split = blockIdx.x, kvh = blockIdx.y / a.blocks, block = blockIdx.y - kvh * a.blocks;
+    // Splits slowest: workgroups are dealt to the XCDs in turn, and the later splits of short sequences are
+    // empty (with splits first, four of them, XCDs 3 and 7 had only the longest sequences' last quarters).
+    const int per_seq = a.c.n_kv_heads * a.blocks, pairs = a.n_seqs * per_seq;
+    const int split = blockIdx.x / pairs, pair = blockIdx.x - split * pairs, seq = pair / per_seq;
+    const int kvh = (pair - seq * per_seq) / a.blocks, block = pair - seq * per_seq - kvh * a.blocks;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int r0 = block * (16 * RT);
     // Three loads that do not wait for one another: the rows, the length, and
     // the pages of the tile that is this wave's first where the length does
     // not change the split and there is no window.
-    const Rowspan own = rows_of(a, blockIdx.z);
+    const Rowspan own = rows_of(a, seq);
     if (r0 >= own.m * a.group) return;
     typename Rows<BF16, DP, FULL, RT>::Raw raw[RT];
 #pragma unroll
@@ -540,9 +544,9 @@ __global__ __launch_bounds__(256, RT == 1 && DP < 256 ? 2 : 1) void few_kernel(A
             a, a.q + (int64_t)(own.first + tok) * a.q_token + (int64_t)(kvh * a.group + row - tok * a.group) * a.q_head,
             row < own.m * a.group);
     }
-    Pages pages = {a.table + blockIdx.z * a.table_stride, a.table_stride, 0, -1};
+    Pages pages = {a.table + seq * a.table_stride, a.table_stride, 0, -1};
     pages.load((split * a.per + wave) * F::TN >> a.c.page_shift, a.c.n_pages);
-    const Seq q = seq_of(a, own, blockIdx.z);
+    const Seq q = seq_of(a, own, seq);
     const Span<F::TN> sp(a, q, r0, 16 * RT);
     if (split >= sp.active) return;
 
@@ -889,15 +893,25 @@ Plan plan_of(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t max_q, int
     p.blocks = (int)((rows + p.rows - 1) / p.rows);
     int64_t seen = max_kv;
     if (window && window + max_q + sinks < seen) seen = window + max_q + sinks;
-    const int64_t tiles = (seen + tn - 1) / tn + 1;
+    const int64_t tiles = (seen + tn - 1) / tn + (window > 0);
     const int64_t grid = (int64_t)p.blocks * c.n_kv_heads * n_seqs;
-    const int64_t want = p.few() ? 1024 : 512, least = p.few() ? 4 : 2;
-    int64_t splits = (want + grid - 1) / grid;
-    if (splits > (tiles + least - 1) / least) splits = (tiles + least - 1) / least;
-    if (splits > MAX_SPLITS) splits = MAX_SPLITS;
-    if (splits < 1 || (p.few() && tiles <= 14)) splits = 1;
-    int64_t per = (tiles + splits - 1) / splits;
-    per = (per + least - 1) / least * least;
+    int64_t per;
+    if (p.few()) {
+        // A workgroup per CU reads as fast as two do, and a split's cost is its start and the join: 8 heads of 131072
+        // tokens in splits of 16, 32, 64, 128, 256 and 512 tiles took 110, 106, 101, 99, 104 and 174 us, of 4096
+        // tokens in 4, 8, 16, 32 and 64 13.1, 13.5, 15.3, 20.2 and 30.0.  Sequences of unlike lengths leave some
+        // workgroups little, so no more than 64 tiles where there are several: 48 of up to 8191 in 32, 64, 192 and
+        // 256 took 105, 104, 110 and 109 us.  Up to 14 tiles the join costs more than it saves: 333 tokens in 4, 8
+        // and all at once 11.4, 12.0 and 10.5 us.
+        per = ((tiles * grid + 255) / 256 + 3) / 4 * 4;
+        if (n_seqs > 1 && per > 64) per = 64;
+        if (tiles <= 14) per = tiles;
+    } else {
+        int64_t splits = (512 + grid - 1) / grid;
+        if (splits > (tiles + 1) / 2) splits = (tiles + 1) / 2;
+        per = (tiles + splits - 1) / splits;
+    }
+    if (per * MAX_SPLITS < tiles) per = (tiles + MAX_SPLITS - 1) / MAX_SPLITS;
     p.per = (int)per;
     p.splits = (int)((tiles + per - 1) / per);
     return p;
@@ -914,7 +928,7 @@ bool fine_sizes(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t n_token
 template <bool BF16, int DP, bool FULL>
 int launch(const AttnArgs &a, const Plan &p, hipStream_t s) {
     if (p.few()) {
-        const dim3 grid((unsigned)p.splits, (unsigned)(a.c.n_kv_heads * p.blocks), (unsigned)a.n_seqs);
+        const dim3 grid((unsigned)(a.c.n_kv_heads * p.blocks * a.n_seqs * p.splits));
         if (p.rows == 16) hipLaunchKernelGGL((few_kernel<BF16, DP, FULL, 1>), grid, dim3(256), 0, s, a);
         else hipLaunchKernelGGL((few_kernel<BF16, DP, FULL, 2>), grid, dim3(256), 0, s, a);
     } else {
@@ -975,8 +989,7 @@ extern "C" int hip_qmm_attn_paged(const hip_qmm_kv_cache *cache, const float *q,
         return (int)hipErrorInvalidValue;
     const Plan p = plan_of(a.c, n_heads, n_seqs, max_q, max_kv, window, sinks);
     const int64_t rows = (int64_t)p.splits * n_tokens * n_heads;
-    if ((int64_t)p.blocks * H > 65535 && p.few()) return (int)hipErrorInvalidValue;
-    if ((int64_t)p.blocks * H * n_seqs > (1 << 23)) return (int)hipErrorInvalidValue;
+    if ((int64_t)p.blocks * H * n_seqs * p.splits > (1 << 23)) return (int)hipErrorInvalidValue;
     if (p.splits > 1 && (!workspace || ((uintptr_t)workspace & 15) ||
                          workspace_size < (size_t)rows * (D + 2) * sizeof(float)))
         return (int)hipErrorInvalidValue;
