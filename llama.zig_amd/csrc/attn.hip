@@ -21,6 +21,8 @@
 // probabilities carry a factor of 2^12 for the same reason.
 #include <math.h>
 
+#include <algorithm>
+
 #include "kv_cache.h"
 
 using namespace kvc;
@@ -232,9 +234,9 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
 // The larger of a value's four lane quarters, in all of them.
 __device__ __forceinline__ float quarter_max(float m) {
     v2u x = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-    m = fmaxf(__uint_as_float(x.x), __uint_as_float(x.y));
+    m = max3(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.y));
     x = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-    return fmaxf(__uint_as_float(x.x), __uint_as_float(x.y));
+    return max3(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.y));
 }
 
 // 16 * RT rows.
@@ -392,17 +394,20 @@ struct Rows {
         const int sub = (lane & 3) >> 1;  // chunk inside 16 dimensions
         const uint8_t *ra = tile + ta * (DP * 2) + (lane & 1) * 8, *rb = ra + 16 * DP * 2;
         const int sa = swizzle<DP>(ta), sb = swizzle<DP>(tb);
+        v4u v[DT];
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(ra + (((2 * d + sub) ^ sa) << 4)));
             const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(rb + (((2 * d + sub) ^ sb) << 4)));
             const v2u xu = __builtin_bit_cast(v2u, x), yu = __builtin_bit_cast(v2u, y);
-            const v4u v = {xu.x, xu.y, yu.x, yu.y};
+            v[d] = (v4u){xu.x, xu.y, yu.x, yu.y};
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int p = 0; p < P; ++p)
 #pragma unroll
-                for (int i = 0; i < RT; ++i) o[i][d] = E::mma(v, w[i][p], o[i][d]);
-        }
+                for (int i = 0; i < RT; ++i) o[i][d] = E::mma(v[d], w[i][p], o[i][d]);
     }
 
     // Whether some result is NaN: by a value that `Odd` would have kept apart, or rightly.
@@ -518,7 +523,7 @@ struct Few {
 };
 
 template <bool BF16, int DP, bool FULL, int RT>
-__global__ __launch_bounds__(256, RT == 1 && DP < 256 ? 2 : 1) void few_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, RT * DP <= 128 ? 2 : 1) void few_kernel(AttnArgs a) {
     using F = Few<DP, RT>;
     __shared__ __attribute__((aligned(1024))) uint8_t ring[F::NW][F::RING];
     __shared__ float tops[F::NW][16 * RT], sums[F::NW][16 * RT];
@@ -682,19 +687,22 @@ __global__ __launch_bounds__(256, RT == 1 && DP < 256 ? 2 : 1) void few_kernel(A
 // ---------------------------------------------------------------- many rows
 
 // 128 rows, 32 per wave, against tiles of 64 tokens that the four waves share:
-// bound by the matrix cores.  Two stages: the next tile's transfers are in
-// flight while one is contracted, one barrier per tile.
+// bound by the matrix cores and the softmax beside them, whose times add up.
+// Two stages: the next tile's transfers are in flight while one is contracted,
+// one barrier per tile.  With WT = 2 64 rows: two waves have the same rows and
+// half of the tokens each, and are joined at the end.
 template <int DP>
 struct Many {
     static constexpr int TN = 64, NW = 4, RT = 2, HALF = TN * DP * 2, STAGE = 2 * HALF;
 };
 
-template <bool BF16, int DP, bool FULL>
+template <bool BF16, int DP, bool FULL, int WT>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a) {
     using M = Many<DP>;
+    constexpr int ROWS = 128 / WT;
     __shared__ __attribute__((aligned(1024))) uint8_t stage[2][M::STAGE];
-    __shared__ uint32_t odd_bits[Odd<DP, 128>::WORDS];
-    const Odd<DP, 128> odd = {odd_bits};
+    __shared__ uint32_t odd_bits[Odd<DP, ROWS>::WORDS];
+    const Odd<DP, ROWS> odd = {odd_bits};
     const int split = blockIdx.y;
     // Blocks of one (sequence, key-value head) share its keys and values: they
     // go to one of the eight XCDs (workgroups are dealt to them in turn) as far
@@ -711,10 +719,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
     }
     const int s = pair / a.c.n_kv_heads, kvh = pair - s * a.c.n_kv_heads;
     const Seq q = seq_of(a, s);
-    const int all = q.m * a.group, mine = (all + 127) / 128;
+    const int all = q.m * a.group, mine = (all + ROWS - 1) / ROWS;
     if (block >= mine) return;
-    const int r0 = (mine - 1 - block) * 128;  // the last rows see most: first
-    const Span<M::TN> sp(a, q, r0, 128);
+    const int r0 = (mine - 1 - block) * ROWS;  // the last rows see most: first
+    const Span<M::TN> sp(a, q, r0, ROWS);
     if (split >= sp.active) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
 
@@ -746,7 +754,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
     Rows<BF16, DP, FULL, M::RT> w;
 #pragma unroll
     for (int i = 0; i < M::RT; ++i) {
-        const int in = wave * 32 + 16 * i + (lane & 15), row = r0 + in, tok = row / a.group;
+        const int in = wave % (M::NW / WT) * 32 + 16 * i + (lane & 15), row = r0 + in, tok = row / a.group;
         auto raw = w.fetch(
             a, a.q + (int64_t)(q.first + tok) * a.q_token + (int64_t)(kvh * a.group + row - tok * a.group) * a.q_head,
             in < sp.rows);
@@ -769,14 +777,23 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
                 asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             }
             const bool edge = is_edge<M::TN>(a, sp, t0) || ok != 15;
-#pragma unroll 1
-            for (int i = 0; i < 2; ++i) {
+            auto half = [&](int i) {
                 v4f x[M::RT][2];
                 v4u p[M::RT][El<BF16>::PARTS];
                 w.scores(a, k, 32 * i, x);
                 if (edge) w.hide(a, x, t0 + 32 * i, ok >> (2 * i) & 1, ok >> (2 * i + 1) & 1);
+                // Matrix instructions first where the SIMD's other wave is at its softmax (274 -> 267 us for a
+                // prompt of 4096 tokens in f16, 353 -> 340 in bf16).
+                __builtin_amdgcn_s_setprio(0);
                 w.soften(x, p);
+                __builtin_amdgcn_s_setprio(1);
                 w.gather(v, 32 * i, p);
+            };
+            if constexpr (WT == 2) {
+                half(wave >> 1);
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < 2; ++i) half(i);
             }
         }
         if (care || !__syncthreads_or(w.any_nan())) break;
@@ -785,10 +802,34 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
         care = true;
         if (begin < end) start();
     }
+    if constexpr (WT == 2) {  // the stages are free: the check above was a barrier
+        v4f *other = reinterpret_cast<v4f *>(stage[0]) + (wave & 1) * 64 * M::RT * (DP / 16 + 1) + lane;
+        if (wave >= 2) {
+#pragma unroll
+            for (int i = 0; i < M::RT; ++i) {
+#pragma unroll
+                for (int d = 0; d < DP / 16; ++d) other[(i * (DP / 16 + 1) + d) * 64] = w.o[i][d];
+                other[(i * (DP / 16 + 1) + DP / 16) * 64] = (v4f){w.top[i], w.sum[i], 0.0f, 0.0f};
+            }
+        }
+        __syncthreads();
+        if (wave >= 2) return;
+#pragma unroll
+        for (int i = 0; i < M::RT; ++i) {
+            const v4f ts = other[(i * (DP / 16 + 1) + DP / 16) * 64];
+            // A lane's share of a sum is 0 where its row saw nothing; the others' of the row then too.
+            const float top = fmaxf(w.top[i], ts[0]), base = top == -INFINITY ? 0.0f : top;
+            const float f = __builtin_amdgcn_exp2f(w.top[i] - base), g = __builtin_amdgcn_exp2f(ts[0] - base);
+            w.sum[i] = f * w.sum[i] + g * ts[1];
+            w.top[i] = top;
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) w.o[i][d] = f * w.o[i][d] + g * other[(i * (DP / 16 + 1) + d) * 64];
+        }
+    }
 
 #pragma unroll
     for (int i = 0; i < M::RT; ++i) {
-        const int in = wave * 32 + 16 * i + (lane & 15), row = r0 + in;
+        const int in = wave % (M::NW / WT) * 32 + 16 * i + (lane & 15), row = r0 + in;
         const float total = w.whole_sum(i);
         if (in >= sp.rows) continue;
         float *out;
@@ -816,16 +857,15 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
 
 // ---------------------------------------------------------------- join of the splits
 
-// One workgroup per row.  The weights of the splits first (at most MAX_SPLITS,
-// in LDS), then their results: LANES threads hold a row, the groups of them
-// take the splits in turn, four loads of each in flight, and are added in
-// order.
-constexpr int MAX_SPLITS = 256;
+// For many splits one workgroup per row.  The weights of the splits first (in
+// LDS), then their results: LANES threads hold a row, the groups of them take
+// the splits in turn, four loads of each in flight, and are added in order.
+constexpr int MAX_SPLITS = 256, SOME_SPLITS = 16;
 
 template <int TN, int ROWS, int LANES>
 __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
     __shared__ float weight[MAX_SPLITS], part[8];
-    __shared__ float4 sums[256];
+    __shared__ v4f sums[256];
     const Seq q = seq_of(a, blockIdx.z);
     const int kvh = blockIdx.y, r = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
     if (r >= q.m * a.group) return;
@@ -839,6 +879,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
     if ((tid & 63) == 0) part[wave] = m;
     __syncthreads();
     m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    // a split that saw nothing has weight 0 and zeros
     const float f = p.x == -INFINITY && p.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p.x - m);
     float total = f == 0.0f ? 0.0f : f * p.y;
     weight[tid] = f;
@@ -847,48 +888,64 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
     __syncthreads();
     constexpr int GROUPS = 256 / LANES;
     const int D = a.c.head_dim, d = tid % LANES * 4;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    v4f o = {};
     if (d < D) {
         const float *src = a.part_o + at * D + d;
 #pragma unroll 4
-        for (int k = tid / LANES; k < sp.active; k += GROUPS) {
-            const float4 u = *reinterpret_cast<const float4 *>(src + k * step * D);
-            const float g = weight[k];
-            // a split that saw nothing has weight 0 and zeros
-            o.x = fmaf(g, u.x, o.x), o.y = fmaf(g, u.y, o.y), o.z = fmaf(g, u.z, o.z), o.w = fmaf(g, u.w, o.w);
-        }
+        for (int k = tid / LANES; k < sp.active; k += GROUPS) o += weight[k] * *reinterpret_cast<const v4f *>(src + k * step * D);
     }
     sums[tid] = o;
     __syncthreads();
     if (tid >= LANES || d >= D) return;
     total = (part[4] + part[5]) + (part[6] + part[7]);
 #pragma unroll
-    for (int k = 1; k < GROUPS; ++k) {
-        const float4 u = sums[k * LANES + tid];
-        o.x += u.x, o.y += u.y, o.z += u.z, o.w += u.w;
+    for (int k = 1; k < GROUPS; ++k) o += sums[k * LANES + tid];
+    *reinterpret_cast<v4f *>(result_row(a, q, kvh, r) + d) = total == 0.0f ? (v4f){} : o / total;
+}
+
+// For at most SOME_SPLITS of them LANES threads per row and nothing shared.
+template <int TN, int ROWS, int LANES>
+__global__ __launch_bounds__(256) void join_some_kernel(AttnArgs a) {
+    const Seq q = seq_of(a, blockIdx.z);
+    const int kvh = blockIdx.y, r = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, d = threadIdx.x % LANES * 4;
+    if (r >= q.m * a.group) return;
+    const Span<TN> sp(a, q, r / ROWS * ROWS, ROWS);
+    const int D = a.c.head_dim;
+    if (sp.active == 1 || d >= D) return;
+    const int64_t step = (int64_t)a.n_tokens * a.n_heads, at = part_row(a, q, kvh, r, 0);
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + at;
+    float m = -INFINITY;
+#pragma unroll 4
+    for (int k = 0; k < sp.active; ++k) m = fmaxf(m, ml[k * step].x);
+    const float *src = a.part_o + at * D + d;
+    v4f o = {};
+    float total = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < sp.active; ++k) {
+        const float2 p = ml[k * step];
+        const v4f u = *reinterpret_cast<const v4f *>(src + k * step * D);
+        const float f = p.x == -INFINITY && p.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p.x - m);
+        total = fmaf(f, p.y, total);
+        o += f * u;
     }
-    if (total == 0.0f) o = make_float4(0.f, 0.f, 0.f, 0.f);
-    else o.x /= total, o.y /= total, o.z /= total, o.w /= total;
-    *reinterpret_cast<float4 *>(result_row(a, q, kvh, r) + d) = o;
+    *reinterpret_cast<v4f *>(result_row(a, q, kvh, r) + d) = total == 0.0f ? (v4f){} : o / total;
 }
 
 // ---------------------------------------------------------------- host
 
-constexpr int MANY_ROWS = 128;
-
 struct Plan {
-    int rows;  // of a block: 16 or 32 (few), 128
+    int rows;  // of a block: 16 or 32 (few), 64 or 128
     int blocks, per, splits;
-    bool few() const { return rows < MANY_ROWS; }
+    bool few() const { return rows <= 32; }
 };
 
 // Which kernel, and how the tokens are split.  A split is worth it while the
 // grid leaves CUs idle; the few-row kernel's splits have a tile per wave at least.
-Plan plan_of(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t max_q, int64_t max_kv, int64_t window,
-             int64_t sinks) {
+Plan plan_of(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t n_tokens, int64_t max_q, int64_t max_kv,
+             int64_t window, int64_t sinks) {
     Plan p;
     const int64_t rows = max_q * (n_heads / c.n_kv_heads);
-    p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : MANY_ROWS;
+    p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     const int64_t tn = p.few() ? 32 : 64;
     p.blocks = (int)((rows + p.rows - 1) / p.rows);
     int64_t seen = max_kv;
@@ -907,9 +964,18 @@ Plan plan_of(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t max_q, int
         if (n_seqs > 1 && per > 64) per = 64;
         if (tiles <= 14) per = tiles;
     } else {
-        int64_t splits = (512 + grid - 1) / grid;
-        if (splits > (tiles + 1) / 2) splits = (tiles + 1) / 2;
-        per = (tiles + splits - 1) / splits;
+        // Time of a workgroup's tiles (2.9 us each, alone on a CU), and of the splits' results, written and read once.
+        per = tiles;
+        double best = 2.9 * (double)tiles;
+        for (int64_t n = 2; n * grid <= 512 && n <= MAX_SPLITS; n *= 2) {
+            const int64_t each = (tiles + n - 1) / n;
+            const double t = 2.9 * (double)each + 8.0 + (double)(n_tokens * n_heads * n) * c.head_dim * 8 / 4e6;
+            if (each < 2 || t >= best) continue;
+            best = t;
+            per = each;
+        }
+        // The exact share of 512 workgroups, two a CU, rather than a power of two.
+        if (per < tiles) per = std::max((tiles * grid + 511) / 512, std::min(per, (int64_t)2));
     }
     if (per * MAX_SPLITS < tiles) per = (tiles + MAX_SPLITS - 1) / MAX_SPLITS;
     p.per = (int)per;
@@ -933,17 +999,30 @@ int launch(const AttnArgs &a, const Plan &p, hipStream_t s) {
         else hipLaunchKernelGGL((few_kernel<BF16, DP, FULL, 2>), grid, dim3(256), 0, s, a);
     } else {
         const dim3 grid((unsigned)(p.blocks * a.c.n_kv_heads * a.n_seqs), (unsigned)p.splits);
-        hipLaunchKernelGGL((many_kernel<BF16, DP, FULL>), grid, dim3(256), 0, s, a);
+        if (p.rows == 64) hipLaunchKernelGGL((many_kernel<BF16, DP, FULL, 2>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((many_kernel<BF16, DP, FULL, 1>), grid, dim3(256), 0, s, a);
     }
     return (int)hipGetLastError();
 }
 
+template <int TN, int ROWS, int LANES>
+void launch_join(const AttnArgs &a, int64_t max_q, hipStream_t s) {
+    const int64_t rows = max_q * a.group;
+    if (a.splits <= SOME_SPLITS) {
+        const dim3 grid((unsigned)((rows * LANES + 255) / 256), (unsigned)a.c.n_kv_heads, (unsigned)a.n_seqs);
+        hipLaunchKernelGGL((join_some_kernel<TN, ROWS, LANES>), grid, dim3(256), 0, s, a);
+    } else {
+        const dim3 grid((unsigned)rows, (unsigned)a.c.n_kv_heads, (unsigned)a.n_seqs);
+        hipLaunchKernelGGL((join_kernel<TN, ROWS, LANES>), grid, dim3(256), 0, s, a);
+    }
+}
+
 template <int LANES>
 void launch_join(const AttnArgs &a, int rows, int64_t max_q, hipStream_t s) {
-    const dim3 grid((unsigned)(max_q * a.group), (unsigned)a.c.n_kv_heads, (unsigned)a.n_seqs);
-    if (rows == 16) hipLaunchKernelGGL((join_kernel<32, 16, LANES>), grid, dim3(256), 0, s, a);
-    else if (rows == 32) hipLaunchKernelGGL((join_kernel<32, 32, LANES>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((join_kernel<64, MANY_ROWS, LANES>), grid, dim3(256), 0, s, a);
+    if (rows == 16) launch_join<32, 16, LANES>(a, max_q, s);
+    else if (rows == 32) launch_join<32, 32, LANES>(a, max_q, s);
+    else if (rows == 64) launch_join<64, 64, LANES>(a, max_q, s);
+    else launch_join<64, 128, LANES>(a, max_q, s);
 }
 
 template <bool BF16>
@@ -963,7 +1042,7 @@ extern "C" size_t hip_qmm_attn_paged_workspace_size(const hip_qmm_kv_cache *cach
     if (!take(cache, &c) || !fine_sizes(c, n_heads, n_seqs, n_tokens, max_q, max_kv, window, sinks) || max_q == 0 ||
         n_seqs == 0)
         return 0;
-    const Plan p = plan_of(c, n_heads, n_seqs, max_q, max_kv, window, sinks);
+    const Plan p = plan_of(c, n_heads, n_seqs, n_tokens, max_q, max_kv, window, sinks);
     return p.splits == 1 ? 0 : (size_t)p.splits * n_tokens * n_heads * (c.head_dim + 2) * sizeof(float);
 }
 
@@ -987,7 +1066,7 @@ extern "C" int hip_qmm_attn_paged(const hip_qmm_kv_cache *cache, const float *q,
         q_head_stride > lim || dst_token_stride > lim || dst_head_stride > lim || (n_heads > 1 && dst_head_stride < D) ||
         (n_tokens > 1 && dst_token_stride < (n_heads - 1) * dst_head_stride + D))
         return (int)hipErrorInvalidValue;
-    const Plan p = plan_of(a.c, n_heads, n_seqs, max_q, max_kv, window, sinks);
+    const Plan p = plan_of(a.c, n_heads, n_seqs, n_tokens, max_q, max_kv, window, sinks);
     const int64_t rows = (int64_t)p.splits * n_tokens * n_heads;
     if ((int64_t)p.blocks * H * n_seqs * p.splits > (1 << 23)) return (int)hipErrorInvalidValue;
     if (p.splits > 1 && (!workspace || ((uintptr_t)workspace & 15) ||
