@@ -111,8 +111,8 @@ def _heads(t, name):
 def _result(out, x):
     """out, checked, or a new tensor of x's shape; with its strides."""
     if out is None:
-        out = torch.empty(x.shape, dtype=torch.float32, device=x.device)
-        return out, out.shape[1] * out.shape[2], out.shape[2]
+        n, h, d = x.shape
+        return x.new_empty((n, h, d)), h * d, d
     st, sh = _heads(out, "out")
     _need(out.shape == x.shape, "out must have the shape of its input")
     return out, st, sh
@@ -217,7 +217,7 @@ def attn_paged(q: torch.Tensor, kv: PagedKV, page_table: torch.Tensor, kv_lens: 
     if workspace is None:
         have, wp = need, None
         if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            workspace = q.new_empty(need, dtype=torch.uint8)
             wp = workspace.data_ptr()
     else:
         have, wp = workspace.numel(), workspace.data_ptr()
@@ -250,13 +250,13 @@ def compact_pages(kv: PagedKV, page_table: torch.Tensor, kv_lens: torch.Tensor, 
     n_seqs, width = _table(page_table)
     _int32(kv_lens, n_seqs, "kv_lens")
     if out is None:
-        out = torch.empty((n_seqs, width), dtype=torch.int32, device=page_table.device)
+        out = page_table.new_empty((n_seqs, width))
     _need(_table(out) == page_table.shape, "out must have page_table's shape")
-    n_live = torch.empty(1, dtype=torch.int32, device=page_table.device)
+    n_live = page_table.new_empty(1)
     L = _lib()
     need = L.hip_qmm_kv_compact_workspace_size(kv._p)
     if workspace is None:
-        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=page_table.device)
+        workspace = page_table.new_empty(max(need, 1), dtype=torch.uint8)
     elif workspace.numel() < need:
         raise HipQmmError(f"workspace too small: {workspace.numel()} < {need}")
     _check(L.hip_qmm_kv_compact(kv._p, page_table.data_ptr(), page_table.stride(0), width, kv_lens.data_ptr(), n_seqs,
