@@ -939,47 +939,62 @@ struct Plan {
     bool few() const { return rows <= 32; }
 };
 
-// Which kernel, and how the tokens are split.  A split is worth it while the
-// grid leaves CUs idle; the few-row kernel's splits have a tile per wave at least.
+// Tiles per split of the few-row kernel.  A workgroup per CU reads as fast as
+// two do, and a split's cost is its start and the join: 8 heads of 131072 tokens
+// in splits of 16, 32, 64, 128, 256 and 512 tiles took 110, 106, 101, 99, 104
+// and 174 us, of 4096 tokens in 4, 8, 16, 32 and 64 13.1, 13.5, 15.3, 20.2 and
+// 30.0.  Sequences of unlike lengths leave some workgroups little, so no more
+// than 64 tiles where there are several: 48 of up to 8191 in 32, 64, 192 and 256
+// took 105, 104, 110 and 109 us.  Up to 14 tiles the join costs more than it
+// saves: 333 tokens in 4, 8 and all at once 11.4, 12.0 and 10.5 us.
+int64_t few_per(int64_t tiles, int64_t grid, int64_t n_seqs) {
+    if (tiles <= 14) return tiles;
+    const int64_t per = ((tiles * grid + 255) / 256 + 3) / 4 * 4;
+    return n_seqs > 1 && per > 64 ? 64 : per;
+}
+
+// Of the many-row kernel, whose tiles take 2.9 us each, alone on a CU: what
+// that is, and the splits' results written and read once, decide.  512
+// workgroups are two a CU; the share is exact rather than a power of two.
+int64_t many_per(int64_t tiles, int64_t grid, double result_bytes) {
+    int64_t per = tiles;
+    double best = 2.9 * (double)tiles;
+    for (int64_t n = 2; n * grid <= 512 && n <= MAX_SPLITS; n *= 2) {
+        const int64_t each = (tiles + n - 1) / n;
+        const double t = 2.9 * (double)each + 8.0 + result_bytes * (double)n / 4e6;
+        if (each < 2 || t >= best) continue;
+        best = t;
+        per = each;
+    }
+    return per < tiles ? std::max((tiles * grid + 511) / 512, std::min(per, (int64_t)2)) : tiles;
+}
+
+// Which kernel, its rows per workgroup, and how the tokens are split.
 Plan plan_of(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t n_tokens, int64_t max_q, int64_t max_kv,
              int64_t window, int64_t sinks) {
-    Plan p;
-    const int64_t rows = max_q * (n_heads / c.n_kv_heads);
-    p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-    const int64_t tn = p.few() ? 32 : 64;
-    p.blocks = (int)((rows + p.rows - 1) / p.rows);
+    const int64_t rows = max_q * (n_heads / c.n_kv_heads), pairs = c.n_kv_heads * n_seqs;
+    const double result_bytes = (double)(n_tokens * n_heads) * c.head_dim * 8;
     int64_t seen = max_kv;
     if (window && window + max_q + sinks < seen) seen = window + max_q + sinks;
-    const int64_t tiles = (seen + tn - 1) / tn + (window > 0);
-    const int64_t grid = (int64_t)p.blocks * c.n_kv_heads * n_seqs;
-    int64_t per;
-    if (p.few()) {
-        // A workgroup per CU reads as fast as two do, and a split's cost is its start and the join: 8 heads of 131072
-        // tokens in splits of 16, 32, 64, 128, 256 and 512 tiles took 110, 106, 101, 99, 104 and 174 us, of 4096
-        // tokens in 4, 8, 16, 32 and 64 13.1, 13.5, 15.3, 20.2 and 30.0.  Sequences of unlike lengths leave some
-        // workgroups little, so no more than 64 tiles where there are several: 48 of up to 8191 in 32, 64, 192 and
-        // 256 took 105, 104, 110 and 109 us.  Up to 14 tiles the join costs more than it saves: 333 tokens in 4, 8
-        // and all at once 11.4, 12.0 and 10.5 us.
-        per = ((tiles * grid + 255) / 256 + 3) / 4 * 4;
-        if (n_seqs > 1 && per > 64) per = 64;
-        if (tiles <= 14) per = tiles;
-    } else {
-        // Time of a workgroup's tiles (2.9 us each, alone on a CU), and of the splits' results, written and read once.
-        per = tiles;
-        double best = 2.9 * (double)tiles;
-        for (int64_t n = 2; n * grid <= 512 && n <= MAX_SPLITS; n *= 2) {
-            const int64_t each = (tiles + n - 1) / n;
-            const double t = 2.9 * (double)each + 8.0 + (double)(n_tokens * n_heads * n) * c.head_dim * 8 / 4e6;
-            if (each < 2 || t >= best) continue;
-            best = t;
-            per = each;
-        }
-        // The exact share of 512 workgroups, two a CU, rather than a power of two.
-        if (per < tiles) per = std::max((tiles * grid + 511) / 512, std::min(per, (int64_t)2));
-    }
-    if (per * MAX_SPLITS < tiles) per = (tiles + MAX_SPLITS - 1) / MAX_SPLITS;
+    auto tiles = [&](int64_t tn) { return std::max((seen + tn - 1) / tn, (int64_t)1) + (window > 0); };
+    auto blocks = [&](int64_t n) { return (rows + n - 1) / n; };
+    Plan p;
+    // More than 16 rows, but little to see and few enough blocks of 16: the few-row kernel has more workgroups
+    // (prompts of 50, 100 and 200 tokens 7.5, 7.9 and 11.4 us; blocks of 64 rows 9.8, 11.5 and 13.8).
+    if (rows <= 16 || (tiles(32) <= 32 && blocks(16) * pairs <= 512)) p.rows = 16;
+    else if (rows <= 32) p.rows = 32;
+    else if (rows <= 64) p.rows = 64;
+    // Blocks of 64 rows where those of 128 would leave CUs idle and the tokens stay whole: prompts of 333, 1000 and
+    // 2000 tokens 18.3, 39.4 and 87.3 us instead of 23.6, 54.3 and 100.7; of 3000 172.5, not 158.1.
+    else if (blocks(128) * pairs <= (c.head_dim > 128 ? 256 : 512) &&
+             many_per(tiles(64), blocks(128) * pairs, result_bytes) == tiles(64)) p.rows = 64;
+    else p.rows = 128;
+    p.blocks = (int)blocks(p.rows);
+    const int64_t n = tiles(p.few() ? 32 : 64), grid = p.blocks * pairs;
+    int64_t per = p.few() ? few_per(n, grid, n_seqs) : many_per(n, grid, result_bytes);
+    per = std::max(per, (n + MAX_SPLITS - 1) / MAX_SPLITS);
     p.per = (int)per;
-    p.splits = (int)((tiles + per - 1) / per);
+    p.splits = (int)((n + per - 1) / per);
     return p;
 }
 
