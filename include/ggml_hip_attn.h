@@ -124,6 +124,14 @@ int hip_qmm_attn_paged(const hip_qmm_kv_cache *cache, const float *q, int64_t n_
                        int64_t dst_token_stride, int64_t dst_head_stride, void *workspace, size_t workspace_size,
                        void *stream);
 
+/* What hip_qmm_attn_paged runs for these sizes, for measurement and tests:
+ * the rows (query tokens x heads of a key-value head) of a workgroup, 16 or 32
+ * in the few-row kernel and 64 or 128 in the many-row one, or 0 where the call
+ * would be refused or empty; *splits, if not NULL (host), the most workgroups
+ * that share a row's tokens. */
+int hip_qmm_attn_paged_rows(const hip_qmm_kv_cache *cache, int64_t n_heads, int64_t n_seqs, int64_t n_tokens,
+                            int64_t max_q, int64_t max_kv, int64_t window, int64_t sinks, int *splits);
+
 /*
  * Copies pages inside the cache, keys and values: of page src[i] the first
  * n_tokens[i] tokens (NULL: all; values are cut to the page) into page dst[i], the rest

@@ -953,12 +953,13 @@ int64_t few_per(int64_t tiles, int64_t grid, int64_t n_seqs) {
     return n_seqs > 1 && per > 64 ? 64 : per;
 }
 
-// Of the many-row kernel, whose tiles take 2.9 us each, alone on a CU: what
-// that is, and the splits' results written and read once, decide.  512
-// workgroups are two a CU; the share is exact rather than a power of two.
-int64_t many_per(int64_t tiles, int64_t grid, double result_bytes) {
+// Of the many-row kernel with 128 rows, and the time in us: a tile takes 2.9
+// alone on a CU, 4.2 beside another workgroup, and splits their results, written
+// and read once, and the join.  512 workgroups are two a CU; the share is exact
+// rather than a power of two.
+int64_t many_per(int64_t tiles, int64_t grid, double result_bytes, double *time) {
     int64_t per = tiles;
-    double best = 2.9 * (double)tiles;
+    double best = (grid <= 256 ? 2.9 : 4.2) * (double)tiles;
     for (int64_t n = 2; n * grid <= 512 && n <= MAX_SPLITS; n *= 2) {
         const int64_t each = (tiles + n - 1) / n;
         const double t = 2.9 * (double)each + 8.0 + result_bytes * (double)n / 4e6;
@@ -966,6 +967,7 @@ int64_t many_per(int64_t tiles, int64_t grid, double result_bytes) {
         best = t;
         per = each;
     }
+    *time = best;
     return per < tiles ? std::max((tiles * grid + 511) / 512, std::min(per, (int64_t)2)) : tiles;
 }
 
@@ -984,14 +986,21 @@ Plan plan_of(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t n_tokens, 
     if (rows <= 16 || (tiles(32) <= 32 && blocks(16) * pairs <= 512)) p.rows = 16;
     else if (rows <= 32) p.rows = 32;
     else if (rows <= 64) p.rows = 64;
-    // Blocks of 64 rows where those of 128 would leave CUs idle and the tokens stay whole: prompts of 333, 1000 and
-    // 2000 tokens 18.3, 39.4 and 87.3 us instead of 23.6, 54.3 and 100.7; of 3000 172.5, not 158.1.
-    else if (blocks(128) * pairs <= (c.head_dim > 128 ? 256 : 512) &&
-             many_per(tiles(64), blocks(128) * pairs, result_bytes) == tiles(64)) p.rows = 64;
     else p.rows = 128;
+    double time = 0.0;
+    int64_t per = 0;
+    if (p.rows == 128) {
+        per = many_per(tiles(64), blocks(128) * pairs, result_bytes, &time);
+        // Blocks of 64 rows, 2.1 us a tile, where those of 128 leave CUs idle and it costs no more: prompts of 333,
+        // 1000 and 2000 tokens 18.3, 39.4 and 87.3 us instead of 23.6, 54.3 and 100.7; of 3000 172.5, not 158.1.
+        if (blocks(128) * pairs <= (c.head_dim > 128 ? 256 : 512) &&
+            2.1 * (double)tiles(64) * std::max(1.0, (double)(blocks(64) * pairs) / 512.0) <= time)
+            p.rows = 64, per = tiles(64);
+    }
     p.blocks = (int)blocks(p.rows);
     const int64_t n = tiles(p.few() ? 32 : 64), grid = p.blocks * pairs;
-    int64_t per = p.few() ? few_per(n, grid, n_seqs) : many_per(n, grid, result_bytes);
+    if (p.few()) per = few_per(n, grid, n_seqs);
+    else if (per == 0) per = many_per(n, grid, result_bytes, &time);  // at most 64 rows
     per = std::max(per, (n + MAX_SPLITS - 1) / MAX_SPLITS);
     p.per = (int)per;
     p.splits = (int)((n + per - 1) / per);
@@ -1059,6 +1068,18 @@ extern "C" size_t hip_qmm_attn_paged_workspace_size(const hip_qmm_kv_cache *cach
         return 0;
     const Plan p = plan_of(c, n_heads, n_seqs, n_tokens, max_q, max_kv, window, sinks);
     return p.splits == 1 ? 0 : (size_t)p.splits * n_tokens * n_heads * (c.head_dim + 2) * sizeof(float);
+}
+
+extern "C" int hip_qmm_attn_paged_rows(const hip_qmm_kv_cache *cache, int64_t n_heads, int64_t n_seqs,
+                                       int64_t n_tokens, int64_t max_q, int64_t max_kv, int64_t window, int64_t sinks,
+                                       int *splits) {
+    Cache c;
+    if (!take(cache, &c) || !fine_sizes(c, n_heads, n_seqs, n_tokens, max_q, max_kv, window, sinks) || max_q == 0 ||
+        n_seqs == 0)
+        return 0;
+    const Plan p = plan_of(c, n_heads, n_seqs, n_tokens, max_q, max_kv, window, sinks);
+    if (splits) *splits = p.splits;
+    return p.rows;
 }
 
 extern "C" int hip_qmm_attn_paged(const hip_qmm_kv_cache *cache, const float *q, int64_t n_heads,

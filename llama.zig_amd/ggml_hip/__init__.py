@@ -551,5 +551,5 @@ def mul_mat_id_glu(qtype, w: torch.Tensor, w_gate: torch.Tensor, x: torch.Tensor
     return out
 
 
-from .attn import (PagedKV, attn_paged, attn_paged_workspace_size, compact_pages, copy_pages, rope,  # noqa: E402,F401
-                   rope_kv_store, rope_steps)
+from .attn import (PagedKV, attn_paged, attn_paged_plan, attn_paged_workspace_size, compact_pages,  # noqa: E402,F401
+                   copy_pages, rope, rope_kv_store, rope_steps)

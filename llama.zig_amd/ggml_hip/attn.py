@@ -42,6 +42,7 @@ def _lib():
         L.hip_qmm_attn_paged_workspace_size.argtypes = [vp, i64, i64, i64, i64, i64, i64, i64]
         L.hip_qmm_attn_paged.argtypes = [vp, vp, i64, i64, i64, vp, i64, i64, i64, vp, i64, vp, i64, f32, i64, i64, vp,
                                          i64, i64, vp, size, vp]
+        L.hip_qmm_attn_paged_rows.argtypes = [vp, i64, i64, i64, i64, i64, i64, i64, vp]
         L.hip_qmm_kv_copy_pages.argtypes = [vp, vp, vp, vp, i64, vp]
         L.hip_qmm_kv_compact_workspace_size.restype = size
         L.hip_qmm_kv_compact_workspace_size.argtypes = [vp]
@@ -174,6 +175,14 @@ def attn_paged_workspace_size(kv: PagedKV, n_heads: int, n_seqs: int, n_tokens: 
                               window=0, sinks=0) -> int:
     return int(_lib().hip_qmm_attn_paged_workspace_size(kv._p, n_heads, n_seqs, n_tokens, max_q, max_kv, window,
                                                         sinks))
+
+
+def attn_paged_plan(kv: PagedKV, n_heads: int, n_seqs: int, n_tokens: int, max_q: int, max_kv: int, window=0, sinks=0):
+    """(rows of a workgroup, splits of a row's tokens at most) that attn_paged runs, for measurement and tests."""
+    splits = ctypes.c_int()
+    rows = _lib().hip_qmm_attn_paged_rows(kv._p, n_heads, n_seqs, n_tokens, max_q, max_kv, window, sinks,
+                                          ctypes.addressof(splits))
+    return rows, splits.value
 
 
 def _table(t):

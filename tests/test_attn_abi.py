@@ -32,7 +32,7 @@ BAD_CACHES = [dict(k=None), dict(v=None), dict(k=P + 8), dict(v=P + 2), dict(typ
 
 def test_declared_entry_points_are_exported():
     names = set(re.findall(r"\b(hip_qmm_\w+)\(", HEADER.read_text()))
-    assert len(names) == 8
+    assert len(names) == 9
     L = A._lib()
     assert all(hasattr(L, n) for n in names)
 
@@ -132,6 +132,37 @@ def test_workspace_size_of_what_is_refused():
     assert f(C.addressof(_cache()), 32, -1, 1, 1, 100, 0, 0) == 0
 
 
+def test_plan():
+    """Every kernel form is reached, and what is refused has no plan."""
+    f = A._lib().hip_qmm_attn_paged_rows
+    splits = C.c_int()
+
+    def plan(n_seqs, new, kv, window=0, sinks=0, heads=32, **cache):
+        c = _cache(**cache)
+        rows = f(C.addressof(c), heads, n_seqs, n_seqs * new, new, kv, window, sinks, C.addressof(splits))
+        need = A._lib().hip_qmm_attn_paged_workspace_size(C.addressof(c), heads, n_seqs, n_seqs * new, new, kv, window, sinks)
+        assert (need > 0) == (splits.value > 1)
+        assert need == 0 or need == splits.value * n_seqs * new * heads * (c.head_dim + 2) * 4
+        assert 1 <= splits.value <= 256
+        return rows, splits.value
+
+    assert plan(1, 1, 333) == (16, 1)
+    assert plan(1, 1, 131072) == (16, 32)
+    assert plan(1, 1, 131072, 1024, 4)[1] < 16
+    assert plan(64, 1, 4096)[0] == 16
+    assert plan(1, 50, 50) == (16, 1)
+    assert plan(1, 7, 4000)[0] == 32
+    assert plan(2, 13, 20000)[0] == 64 and splits.value > 1
+    assert plan(1, 1000, 1000) == (64, 1)
+    assert plan(1, 4096, 4096) == (128, 1)
+    assert plan(1, 512, 32768)[0] == 128 and splits.value > 1
+    assert plan(1, 1, 1 << 30) == (16, 32)
+    assert plan(1, 1, 1 << 20, heads=1, n_kv_heads=1) == (16, 256)
+    assert f(None, 32, 1, 1, 1, 100, 0, 0, None) == 0
+    c = _cache()
+    assert f(C.addressof(c), 31, 1, 1, 1, 100, 0, 0, None) == 0 and f(C.addressof(c), 32, 1, 1, 0, 100, 0, 0, None) == 0
+
+
 def _compact(cache=None, **kw):
     f = dict(table=P, stride=10, width=10, lens=P, n_seqs=1, out=P, out_stride=10, live=P, ws=P, size=1 << 30)
     f.update(kw)
@@ -144,7 +175,7 @@ def test_page_refusals():
     L = A._lib()
     good = _cache()
     at = C.addressof(good)
-    assert L.hip_qmm_kv_copy_pages(at, P, P, None, 0, None) == 0
+    assert L.hip_qmm_kv_copy_pages(at, P, P, None, 0, None) == 0 and L.hip_qmm_kv_copy_pages(at, None, None, None, 0, None) == 0
     for a in ((None, P, P, None, 1), (at, None, P, None, 1), (at, P, None, None, 1), (at, P, P, None, -1)):
         assert L.hip_qmm_kv_copy_pages(*a, None) == BAD, a
     need = L.hip_qmm_kv_compact_workspace_size(at)

@@ -312,3 +312,42 @@ def test_offsets_past_32_bits():
     k[hold], v[hold] = d["k"], d["v"]
     far = dict(d, k=k, v=v, table=torch.where(d["table"] >= 0, pages - 1 - d["table"], -1).int())
     assert torch.equal(_run(far), _run(d))
+
+
+FORMS = [  # rows of a workgroup, whether the tokens are split, sequences, new tokens, length
+    (16, False, 2, 1, 300), (16, True, 2, 1, 3000), (16, False, 2, 40, 300), (16, True, 1, 20, 900),
+    (32, True, 2, 7, 3000), (64, False, 2, 300, 700), (64, True, 2, 15, 3000), (128, False, 5, 1000, 1100),
+    (128, True, 1, 150, 9000)]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 80, 128, 256])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (0, 3), (900, 5)])
+@pytest.mark.parametrize("form", FORMS)
+def test_every_kernel_form(form, window, sinks, dim, dtype):
+    import ggml_hip as G
+    rows, split, seqs, new, n = form
+    lens = [n] + [max(new, n * 2 // 3 + 7 * i) for i in range(1, seqs)]
+    c = _case(dtype, 32, 8, dim, page=32, lens=lens, new=[new] * seqs)
+    kv = G.PagedKV(c["k"], c["v"])
+    got, splits = G.attn_paged_plan(kv, 32, seqs, c["q"].shape[0], new, c["table"].shape[1] * 32, window, sinks)
+    if not window and dim <= 128:
+        assert (got, splits > 1) == (rows, split)
+    _check(c, window, sinks)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("form", FORMS)
+def test_values_that_are_not_finite_in_every_kernel_form(form, bad):
+    """One bad value of a late token of the first sequence: its dimension of the rows that see it, nothing else."""
+    rows, split, seqs, new, n = form
+    c = _case("f16", 32, 8, 128, page=32, lens=[n] * seqs, new=[new] * seqs)
+    clean = _run(c, decode=False)
+    at = n - 1 - new // 3
+    c["v"][int(c["table"][0, at // 32]), 3, at % 32, 77] = bad
+    got = _run(c, decode=False)
+    first = new - 1 - new // 3
+    hit = got[first:new, 12:16, 77]
+    assert bool((torch.isnan(hit) if math.isnan(bad) else hit == bad).all())
+    got[first:new, 12:16, 77] = clean[first:new, 12:16, 77]
+    assert torch.equal(got, clean)

@@ -189,3 +189,18 @@ def test_fork_compact_and_attend():
     want, top = R.attention(r, k, v, table, lens + 1, torch.arange(3), 128 ** -0.5)
     assert float((got.double() - want).norm() / want.norm()) <= R.tolerance(128, top)
     assert not torch.equal(got[0], got[1])
+
+
+@pytest.mark.parametrize("pages,width", [(8192, 60), (8193, 60), (300, 16384 // 3), (300, 16384 // 3 + 1)])
+def test_compact_at_the_limits_of_one_launch(pages, width):
+    """Up to 8192 pages and 16384 table entries it is one launch, above two."""
+    rng = random.Random(pages + width)
+    k, v = _cache(pages=pages, kv_heads=1, dim=8)
+    free = rng.sample(range(pages), pages)
+    lens = [16 * 60, 16 * 37 + 3, 16 * 50]
+    table = [[free.pop() if i * 16 < n else rng.choice((-1, 5, pages)) for i in range(width)] for n in lens]
+    got = _check_compact(k, v, table, lens, 16)
+    # the same in place, which takes two launches
+    k, v = _cache(pages=pages, kv_heads=1, dim=8)
+    t = _i32(table)
+    assert torch.equal(_check_compact(k, v, table, lens, 16, tensor=t, out=t), got)
