@@ -93,11 +93,12 @@ int hip_qmm_rope_kv_store(const float *q, int64_t n_heads, int64_t q_token_strid
 /*
  * Attention of the newest tokens of n_seqs sequences over the paged cache.
  * Sequence s holds n = kv_lens[s] tokens, token j in page
- * page_table[s*table_stride + j / page_size] (lengths are cut to
- * table_stride*page_size; negative ones count as 0), and its last m have
- * queries: rows q_starts[s] <= t < q_starts[s+1] of q, or row s alone
- * (m = 1) with q_starts NULL.  The keys and values of the new tokens are in the
- * cache already.  The query of position p sees token j if
+ * page_table[s*table_stride + j / page_size] (n_seqs rows of table_stride
+ * entries; lengths are cut to table_stride*page_size and to 2^30; negative ones
+ * count as 0), and its last m have queries: rows q_starts[s] <= t <
+ * q_starts[s+1] of q, or row s alone (m = 1) with q_starts NULL.  The keys and
+ * values of the new tokens are in the cache already.  The query of position p
+ * sees token j if
  *   j <= p  and  (window == 0  or  p - j < window  or  j < sinks)
  * and j's page lies in [0, n_pages): pages that fell out of the window may be
  * freed and their entries set to -1.  With head h's keys and values in
@@ -109,10 +110,11 @@ int hip_qmm_rope_kv_store(const float *q, int64_t n_heads, int64_t q_token_strid
  * cores as sums of f16 or bf16 parts that hold 22 bits and more.
  * q_starts ascends from 0 or more to n_tokens or less; max_q is at least the
  * largest m; max_kv, the largest length in the host's knowledge, only plans the
- * work.  n_heads a multiple of n_kv_heads; q and
- * dst 16-byte aligned with strides that are multiples of 4 floats; window and
- * sinks in [0, 2^30].  Deterministic.  The workspace is scratch: its contents
- * do not matter before the call, and it serves one call at a time.
+ * work.  n_heads a multiple of n_kv_heads; q and dst 16-byte aligned with strides
+ * that are multiples of 4 floats; dst does not overlap q; window, sinks and
+ * max_kv in [0, 2^30]; n_tokens at most 2^23, its product with
+ * n_heads / n_kv_heads at most 2^30.  Deterministic.  The workspace is scratch:
+ * its contents do not matter before the call, and it serves one call at a time.
  */
 size_t hip_qmm_attn_paged_workspace_size(const hip_qmm_kv_cache *cache, int64_t n_heads, int64_t n_seqs,
                                          int64_t n_tokens, int64_t max_q, int64_t max_kv, int64_t window,

@@ -8,17 +8,16 @@
 // A wave contracts 16 rows or a few times as many with 32 tokens on 16x16x32
 // matrix instructions, all transposed: scores S^T = K Q^T, results
 // O^T = V^T P^T.  A row is then the lane index (mod 16) of both accumulators:
-// maximum, sum and rescaling stay in the lane (but for one exchange among its four
-// quarters), and the probabilities, as the scores lie, are the second operand
-// of the next product: slot e of lane quarter g holds token
+// maximum, sum and rescaling stay in the lane (but for one exchange among the
+// four lane quarters that share a row), and the probabilities, as the scores
+// lie, are the second operand of the next product: slot e of quarter g holds token
 // 16*(e/4) + 4*g + e%4, an order that the transposing LDS reads of V follow.
 //
 // f32 results from 16-bit matrix cores: keys and values are what the cache
 // holds, exactly; queries and probabilities go in as sums of PARTS 16-bit
 // parts (two f16: 22 bits; three bf16: 24), each a product of its own into the
-// f32 accumulators.  A query row is scaled by a power of two that puts its
-// largest element near 2^13, so that f16's range does not matter; the
-// probabilities carry a factor of 2^12 for the same reason.
+// f32 accumulators.  A query row is scaled by a power of two, and the
+// probabilities carry another, so that the parts' range does not matter.
 #include <math.h>
 
 #include <algorithm>
@@ -42,8 +41,9 @@ typedef __attribute__((address_space(3))) void *lds_ptr;
 typedef __attribute__((address_space(3))) v4s *lds_v4s;
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LIFT = 12.0f;   // probabilities are held times 2^LIFT,
-constexpr float SLACK = 3.0f;   // and the running maximum may lag by 2^SLACK: 2^15 stays below f16's largest
+constexpr float SLACK = 3.0f;   // the running maximum may lag by 2^SLACK
+
+constexpr int MAX_LENGTH = 1 << 30;  // tokens of a sequence: sums of two positions fit 32 bits
 
 struct AttnArgs {
     Cache c;
@@ -69,6 +69,10 @@ template <>
 struct El<false> {
     static constexpr int PARTS = 2;
     static constexpr uint32_t INF = 0x7c00;
+    // A row of q is scaled to 2^QUERY and probabilities to 2^LIFT at the maximum: with SLACK both stay just below
+    // f16's largest, and second parts and small weights lie as high above its smallest as they can.
+    static constexpr int QUERY = 13;
+    static constexpr float LIFT = 12.0f;
     static __device__ __forceinline__ v4f mma(v4u a, v4u b, v4f c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
     }
@@ -86,6 +90,9 @@ template <>
 struct El<true> {
     static constexpr int PARTS = 3;
     static constexpr uint32_t INF = 0x7f80;
+    // Far below 1: sums over many of a cache's largest values (3e38) stay finite.
+    static constexpr int QUERY = -10;
+    static constexpr float LIFT = -16.0f;
     static __device__ __forceinline__ v4f mma(v4u a, v4u b, v4f c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
     }
@@ -116,16 +123,17 @@ __device__ __forceinline__ Rowspan rows_of(const AttnArgs &a, int s) {
 }
 
 __device__ __forceinline__ Seq seq_of(const AttnArgs &a, const Rowspan &r, int s) {
-    const int64_t most = a.table_stride << a.c.page_shift;
+    const int64_t most = min(a.table_stride << a.c.page_shift, (int64_t)MAX_LENGTH);
     return {r.first, r.m, (int)min((int64_t)max(a.lens[s], 0), most)};
 }
 
 __device__ __forceinline__ Seq seq_of(const AttnArgs &a, int s) { return seq_of(a, rows_of(a, s), s); }
 
 // Rows [r0, r0 + rows) of a sequence's head group, their positions, and the
-// tiles of TN tokens that any of them sees (from token `low` on, or a first one): first `sink` tiles of the tokens
-// that stay visible, then those from tile `from` on; `count` in all, dealt to
-// the splits `per` at a time, `active` of which have some (the first always).
+// tiles of TN tokens that any of them sees (from token `low` on, or one of the
+// first): first `sink` tiles of the tokens that stay visible, then those from
+// tile `from` on; `count` in all, dealt to the splits `per` at a time, `active`
+// of which have some (the first always).
 template <int TN>
 struct Span {
     int rows, p_first, p_last, low, sink, from, count, per, active;
@@ -208,12 +216,10 @@ struct Loader {
             off[i] = ((uint32_t)t * (uint32_t)a.c.token_stride + chunk * 8) * 2;
         }
     }
-    // 16 tokens from `base` to LDS; of a workgroup's transfers those of one wave in `step`, from `first` on.
-    __device__ __forceinline__ void group(const AttnArgs &a, const uint16_t *base, uint32_t lds, int first, int step) const {
+    // 16 tokens from `base` to LDS.
+    __device__ __forceinline__ void group(const AttnArgs &a, const uint16_t *base, uint32_t lds) const {
 #pragma unroll
-        for (int i = 0; i < GROUP; ++i)
-            if (step == 1 || i % step == first)
-                dma16(base + (int64_t)(i * PER) * a.c.token_stride, off[i % NV], lds + i * 1024);
+        for (int i = 0; i < GROUP; ++i) dma16(base + (int64_t)(i * PER) * a.c.token_stride, off[i % NV], lds + i * 1024);
     }
 };
 
@@ -224,19 +230,16 @@ __device__ __forceinline__ int64_t group_at(const AttnArgs &a, int page, int t0)
 
 // ---------------------------------------------------------------- a wave's rows
 
-// The largest of three; a NaN is passed over.  (fmaxf would first quiet each matrix result by an operation of its own.)
-__device__ __forceinline__ float max3(float x, float y, float z) {
-    float m;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(x), "v"(y), "v"(z));
-    return m;
-}
+// The larger of two, NaN if one is: unlike fmaxf it needs no operation that first quiets each matrix result.  (And no
+// inline assembly on those: the compiler does not count it among the readers that wait for a matrix instruction.)
+__device__ __forceinline__ float larger(float x, float y) { return __builtin_elementwise_maximum(x, y); }
 
-// The larger of a value's four lane quarters, in all of them.
+// The largest of a value's four lane quarters, in all of them.
 __device__ __forceinline__ float quarter_max(float m) {
     v2u x = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-    m = max3(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.y));
+    m = larger(__uint_as_float(x.x), __uint_as_float(x.y));
     x = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-    return max3(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.y));
+    return larger(__uint_as_float(x.x), __uint_as_float(x.y));
 }
 
 // 16 * RT rows.
@@ -287,7 +290,7 @@ struct Rows {
             }
         big = quarter_max(big);
         const int ex = (int)(__float_as_uint(big) >> 23);  // biased; 255: not finite, left as it is
-        const int up = ex == 255 || ex == 0 ? 0 : min(13 - (ex - 127), 120);
+        const int up = ex == 255 || ex == 0 ? 0 : min(E::QUERY - (ex - 127), 120);
         unit[i] = ldexpf(1.0f, -up);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -339,8 +342,10 @@ struct Rows {
         bool raise = false;
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
-            const float x = max3(s[i][0][0], s[i][0][1], s[i][0][2]), y = max3(s[i][0][3], s[i][1][0], s[i][1][1]);
-            m[i] = quarter_max(max3(max3(s[i][1][2], s[i][1][3], x), y, y)) * unit[i];
+            float x = larger(s[i][0][0], s[i][0][1]);
+#pragma unroll
+            for (int r = 2; r < 8; ++r) x = larger(x, s[i][r >> 2][r & 3]);
+            m[i] = quarter_max(x) * unit[i];  // NaN: not above top, and the row is NaN by its sum
             raise |= m[i] > top[i] + SLACK;
         }
         if (__any(raise)) {
@@ -356,7 +361,7 @@ struct Rows {
         }
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
-            const float base = (top[i] == -INFINITY ? 0.0f : top[i]) - LIFT;
+            const float base = (top[i] == -INFINITY ? 0.0f : top[i]) - E::LIFT;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -508,6 +513,12 @@ struct Odd {
     }
 };
 
+// What results under the maximum `top` count for under `m`: never 0, which would make a NaN of one that is infinite,
+// however small its share.
+__device__ __forceinline__ float weight_of(float top, float m) {
+    return fmaxf(__builtin_amdgcn_exp2f(top - m), 0x1p-126f);
+}
+
 // ---------------------------------------------------------------- few rows
 
 // 16 * RT rows (one token's heads, or a few tokens'): bound by the reads of K
@@ -572,13 +583,13 @@ __global__ __launch_bounds__(256, RT * DP <= 128 ? 2 : 1) void few_kernel(AttnAr
         oks = (oks & ~(3u << (2 * st))) | ok << (2 * st);
         at0 = head + group_at(a, p0, t0);
         at1 = head + group_at(a, p1, t0 + 16);
-        loader.group(a, a.c.k + at0, lds + st * 2 * F::HALF, 0, 1);
-        loader.group(a, a.c.k + at1, lds + st * 2 * F::HALF + F::HALF / 2, 0, 1);
+        loader.group(a, a.c.k + at0, lds + st * 2 * F::HALF);
+        loader.group(a, a.c.k + at1, lds + st * 2 * F::HALF + F::HALF / 2);
     };
     auto issue_values = [&](int i) {  // of the tile that issue_keys last began
         const int st = i % F::ST;
-        loader.group(a, a.c.v + at0, lds + (st * 2 + 1) * F::HALF, 0, 1);
-        loader.group(a, a.c.v + at1, lds + (st * 2 + 1) * F::HALF + F::HALF / 2, 0, 1);
+        loader.group(a, a.c.v + at0, lds + (st * 2 + 1) * F::HALF);
+        loader.group(a, a.c.v + at1, lds + (st * 2 + 1) * F::HALF + F::HALF / 2);
     };
     // At most n halves issued after the one wanted may be outstanding.
     auto wait_halves = [&](int n) {
@@ -743,8 +754,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
         const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_addr(stage[u & 1])) + wave * (M::HALF / 4);
         const int t = t0 + 16 * wave;
         const int64_t at = head + group_at(a, pages.get(t >> a.c.page_shift), t);
-        loader.group(a, a.c.k + at, lds, 0, 1);
-        loader.group(a, a.c.v + at, lds + M::HALF, 0, 1);
+        loader.group(a, a.c.k + at, lds);
+        loader.group(a, a.c.v + at, lds + M::HALF);
     };
     auto start = [&] {
         pages.load(sp.token(begin) >> a.c.page_shift, a.c.n_pages);
@@ -819,7 +830,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
             const v4f ts = other[(i * (DP / 16 + 1) + DP / 16) * 64];
             // A lane's share of a sum is 0 where its row saw nothing; the others' of the row then too.
             const float top = fmaxf(w.top[i], ts[0]), base = top == -INFINITY ? 0.0f : top;
-            const float f = __builtin_amdgcn_exp2f(w.top[i] - base), g = __builtin_amdgcn_exp2f(ts[0] - base);
+            const float f = weight_of(w.top[i], base), g = weight_of(ts[0], base);
             w.sum[i] = f * w.sum[i] + g * ts[1];
             w.top[i] = top;
 #pragma unroll
@@ -862,6 +873,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
 // the splits in turn, four loads of each in flight, and are added in order.
 constexpr int MAX_SPLITS = 256, SOME_SPLITS = 16;
 
+__device__ __forceinline__ float split_weight(float2 p, float m) {
+    return p.x == -INFINITY && p.y == 0.0f ? 0.0f : weight_of(p.x, m);  // a split that saw nothing: 0, and zeros
+}
+
 template <int TN, int ROWS, int LANES>
 __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
     __shared__ float weight[MAX_SPLITS], part[8];
@@ -879,8 +894,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
     if ((tid & 63) == 0) part[wave] = m;
     __syncthreads();
     m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-    // a split that saw nothing has weight 0 and zeros
-    const float f = p.x == -INFINITY && p.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p.x - m);
+    const float f = split_weight(p, m);
     float total = f == 0.0f ? 0.0f : f * p.y;
     weight[tid] = f;
     for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
@@ -924,7 +938,7 @@ __global__ __launch_bounds__(256) void join_some_kernel(AttnArgs a) {
     for (int k = 0; k < sp.active; ++k) {
         const float2 p = ml[k * step];
         const v4f u = *reinterpret_cast<const v4f *>(src + k * step * D);
-        const float f = p.x == -INFINITY && p.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p.x - m);
+        const float f = split_weight(p, m);
         total = fmaf(f, p.y, total);
         o += f * u;
     }
@@ -1011,8 +1025,8 @@ bool fine_sizes(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t n_token
                 int64_t window, int64_t sinks) {
     return n_heads >= 1 && n_heads <= 65535 && n_heads % c.n_kv_heads == 0 && n_seqs >= 0 && n_seqs <= 65535 &&
            n_tokens >= 0 && n_tokens <= ((int64_t)1 << 23) && max_q >= 0 && max_q <= n_tokens && max_kv >= 0 &&
-           max_kv <= INT32_MAX && window >= 0 && sinks >= 0 && window <= (1 << 30) && sinks <= (1 << 30) &&
-           max_q * (n_heads / c.n_kv_heads) <= (1 << 30);
+           max_kv <= MAX_LENGTH && window >= 0 && sinks >= 0 && window <= MAX_LENGTH && sinks <= MAX_LENGTH &&
+           n_tokens * (n_heads / c.n_kv_heads) <= (1 << 30);
 }
 
 template <bool BF16, int DP, bool FULL>
@@ -1091,7 +1105,7 @@ extern "C" int hip_qmm_attn_paged(const hip_qmm_kv_cache *cache, const float *q,
     AttnArgs a = {};
     const int64_t lim = (int64_t)1 << 40;
     if (!take(cache, &a.c) || !fine_sizes(a.c, n_heads, n_seqs, n_tokens, max_q, max_kv, window, sinks) ||
-        !isfinite(scale) || table_stride < 0 || table_stride > INT32_MAX)
+        !isfinite(scale * LOG2E) || table_stride < 0 || table_stride > INT32_MAX)
         return (int)hipErrorInvalidValue;
     const int64_t H = a.c.n_kv_heads, D = a.c.head_dim;
     if (!q_starts && (n_tokens != n_seqs || (n_tokens > 0 && max_q < 1))) return (int)hipErrorInvalidValue;

@@ -218,7 +218,7 @@ def attn_paged(q: torch.Tensor, kv: PagedKV, page_table: torch.Tensor, kv_lens: 
         max_q = n if max_q is None else max_q
     if not page_table.is_contiguous():  # the row stride is the width that lengths are cut to
         page_table = page_table.contiguous()
-    most = width * kv.page_size
+    most = min(width * kv.page_size, 1 << 30)
     max_kv = most if max_kv is None or max_kv > most else max_kv
     out, ot, oh = _result(out, q)
     L = _lib()

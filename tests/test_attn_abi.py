@@ -110,7 +110,8 @@ def test_attention_refusals():
     assert _attn() == 0
     one = dict(n_seqs=1, n=4, max_q=4)
     for kw in (dict(n_heads=0), dict(n_heads=31), dict(n_heads=-32), dict(n_seqs=-1), dict(n_seqs=70000), dict(n=-1),
-               dict(n=(1 << 23) + 1), dict(max_q=-1), dict(max_q=5), dict(max_kv=-1), dict(scale=math.nan),
+               dict(n=(1 << 23) + 1), dict(max_q=-1), dict(max_q=5), dict(max_kv=-1), dict(max_kv=(1 << 30) + 1), dict(scale=math.nan),
+               dict(scale=3e38),
                dict(scale=math.inf), dict(window=-1), dict(sinks=-1), dict(window=1 << 31), dict(sinks=1 << 31),
                dict(width=-1), dict(width=1 << 31), dict(starts=None), dict(q=None), dict(dst=None), dict(lens=None),
                dict(table=None), dict(q=P + 4), dict(dst=P + 8), dict(q_token=4098), dict(q_head=126),

@@ -197,6 +197,45 @@ def test_extreme_queries(dtype, new):
     _check(c, scale=0.0, decode=False)
 
 
+@pytest.mark.parametrize("dtype,up", [("f16", 13), ("bf16", 100)])
+@pytest.mark.parametrize("lens,new", [((300, 77), 1), ((300, 77), 40), ((5000,), 1), ((700, 400), 300), ((9000,), 150)])
+def test_large_cached_values(dtype, up, lens, new):
+    """Keys far over 1 that small queries meet, values up to the type's largest."""
+    c = _case(dtype, lens=lens, new=[new] * len(lens))
+    c["q"] *= 2.0 ** -up
+    c["k"] *= 2.0 ** up
+    most = torch.finfo(c["v"].dtype).max
+    gen = torch.Generator("cuda").manual_seed(3)
+    size = 0.5 + 0.5 * torch.rand(c["v"].shape, generator=gen, device="cuda")
+    c["v"].copy_(torch.copysign(size, c["v"].float()) * most)
+    assert torch.isfinite(c["k"]).all() and torch.isfinite(c["v"]).all()
+    _check(c, vmax=most)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n,new", [(300, 1), (20000, 1), (900, 20), (3000, 7), (3000, 15), (700, 300), (9000, 150)])
+def test_an_infinite_value_of_tiny_weight(dtype, n, new):
+    """A probability that f32 holds as 0 is above 0 all the same: times infinity it is infinity, not NaN."""
+    c = _case(dtype, lens=(n,), new=[new])
+    c["q"].abs_()
+    page = int(c["table"][0, 0])
+    c["k"][page, 3, 0] = -60.0  # scores near -500
+    c["v"][page, 3, 0, 77] = math.inf
+    got = _check(c)
+    assert bool((got[:, 12:16, 77] == math.inf).all())
+
+
+def test_longest_planning_length():
+    """The longest length that can be planned for, over a short table and over one as long."""
+    c = _case(lens=(333,))
+    want = _check(c)
+    _hold(_run(c, max_kv=1 << 30), want.double(), 8.0, 128)
+    wide = torch.full((1, (1 << 26) + 5), -1, dtype=torch.int32, device="cuda")
+    wide[:, :c["table"].shape[1]] = c["table"]
+    _hold(_run(dict(c, table=wide)), want.double(), 8.0, 128)
+    _hold(_run(dict(c, table=wide), max_kv=2 ** 31 - 1), want.double(), 8.0, 128)
+
+
 def test_nan_query_is_its_own_rows_matter():
     c = _case(lens=(100, 50), new=[20, 20])
     clean = _run(c)
