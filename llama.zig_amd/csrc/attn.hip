@@ -700,17 +700,23 @@ __global__ __launch_bounds__(256, RT * DP <= 128 ? 2 : 1) void few_kernel(AttnAr
 // 128 rows, 32 per wave, against tiles of 64 tokens that the four waves share:
 // bound by the matrix cores and the softmax beside them, whose times add up.
 // Two stages: the next tile's transfers are in flight while one is contracted,
-// one barrier per tile.  With WT = 2 64 rows: two waves have the same rows and
-// half of the tokens each, and are joined at the end.
-template <int DP>
+// one barrier per tile.  With 64 rows two waves have the same rows and half of
+// the tokens each, and are joined at the end (WT = 2).  For 256 dimensions only
+// 64 rows, 16 per wave, and tiles of 32 tokens: two workgroups fit a CU, in 256
+// registers a lane, none in memory.  (With 32 rows per wave and tiles of 64 one did:
+// 2048 tokens 183 us in f16 and 360 in bf16, not 151 and 177; 13 tokens on
+// 20000 102 and 265, not 67 and 75.)
+template <int DP, int ROWS>
 struct Many {
-    static constexpr int TN = 64, NW = 4, RT = 2, HALF = TN * DP * 2, STAGE = 2 * HALF;
+    static constexpr bool WIDE = DP == 256;
+    static constexpr int TN = WIDE ? 32 : 64, NW = 4, RT = WIDE ? 1 : 2, WT = NW * 16 * RT / ROWS;
+    static constexpr int GROUPS = TN / 16, ALL = (1 << GROUPS) - 1, HALF = TN * DP * 2, STAGE = 2 * HALF;
 };
 
-template <bool BF16, int DP, bool FULL, int WT>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a) {
-    using M = Many<DP>;
-    constexpr int ROWS = 128 / WT;
+template <bool BF16, int DP, bool FULL, int ROWS>
+__global__ __launch_bounds__(256, 2) void many_kernel(AttnArgs a) {
+    using M = Many<DP, ROWS>;
+    constexpr int WT = M::WT;
     __shared__ __attribute__((aligned(1024))) uint8_t stage[2][M::STAGE];
     __shared__ uint32_t odd_bits[Odd<DP, ROWS>::WORDS];
     const Odd<DP, ROWS> odd = {odd_bits};
@@ -741,21 +747,27 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
     const int begin = split * sp.per, end = min(sp.count, begin + sp.per);
     Pages pages = {a.table + s * a.table_stride, a.table_stride, 0, -1};
     const Loader<DP> loader(a);
-    const int more = a.c.page_shift == 4 ? 3 : a.c.page_shift == 5 ? 1 : 0;
-    uint32_t oks = 0;  // four bits per stage
-    // Wave w transfers tokens 16 w to 16 w + 15.
+    const int more = max((M::TN >> a.c.page_shift) - 1, 0);
+    uint32_t oks = 0;  // GROUPS bits per stage
+    // Wave w transfers tokens 16 w to 16 w + 15, of two groups either the keys or the values.
     auto issue = [&](int u) {
         const int t0 = sp.token(u), p = t0 >> a.c.page_shift;
         pages.hold(p, more, a.c.n_pages);
         uint32_t ok = 0;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) ok |= pages.get((t0 + 16 * g) >> a.c.page_shift) >= 0 ? 1u << g : 0;
-        oks = u & 1 ? (oks & 15) | ok << 4 : (oks & 240) | ok;
-        const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_addr(stage[u & 1])) + wave * (M::HALF / 4);
-        const int t = t0 + 16 * wave;
+        for (int g = 0; g < M::GROUPS; ++g) ok |= pages.get((t0 + 16 * g) >> a.c.page_shift) >= 0 ? 1u << g : 0;
+        oks = u & 1 ? (oks & M::ALL) | ok << M::GROUPS : (oks & M::ALL << M::GROUPS) | ok;
+        const int g = wave % M::GROUPS, t = t0 + 16 * g;
+        const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_addr(stage[u & 1])) + g * (M::HALF / M::GROUPS);
         const int64_t at = head + group_at(a, pages.get(t >> a.c.page_shift), t);
-        loader.group(a, a.c.k + at, lds);
-        loader.group(a, a.c.v + at, lds + M::HALF);
+        if constexpr (M::GROUPS == M::NW) {
+            loader.group(a, a.c.k + at, lds);
+            loader.group(a, a.c.v + at, lds + M::HALF);
+        } else if (wave < M::GROUPS) {
+            loader.group(a, a.c.k + at, lds);
+        } else {
+            loader.group(a, a.c.v + at, lds + M::HALF);
+        }
     };
     auto start = [&] {
         pages.load(sp.token(begin) >> a.c.page_shift, a.c.n_pages);
@@ -765,7 +777,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
     Rows<BF16, DP, FULL, M::RT> w;
 #pragma unroll
     for (int i = 0; i < M::RT; ++i) {
-        const int in = wave % (M::NW / WT) * 32 + 16 * i + (lane & 15), row = r0 + in, tok = row / a.group;
+        const int in = wave % (M::NW / WT) * (16 * M::RT) + 16 * i + (lane & 15), row = r0 + in, tok = row / a.group;
         auto raw = w.fetch(
             a, a.q + (int64_t)(q.first + tok) * a.q_token + (int64_t)(kvh * a.group + row - tok * a.group) * a.q_head,
             in < sp.rows);
@@ -779,15 +791,15 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
             __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wave has read the stage that is refilled next
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            const int ok = oks >> (4 * (u & 1)) & 15, t0 = sp.token(u);
+            const int ok = oks >> (M::GROUPS * (u & 1)) & M::ALL, t0 = sp.token(u);
             if (u + 1 < end) issue(u + 1);
             uint8_t *k = stage[u & 1], *v = k + M::HALF;
-            if (care || has_unseen<M::TN>(a, sp, t0) || ok != 15) {
+            if (care || has_unseen<M::TN>(a, sp, t0) || ok != M::ALL) {
                 blank<DP, M::TN>(a, sp, v, t0, ok, threadIdx.x, 256);
                 if (care) odd.template sift<BF16>(a, v, M::TN, t0, ok, r0, sp.rows, threadIdx.x, 256, q.n - q.m);
                 asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             }
-            const bool edge = is_edge<M::TN>(a, sp, t0) || ok != 15;
+            const bool edge = is_edge<M::TN>(a, sp, t0) || ok != M::ALL;
             auto half = [&](int i) {
                 v4f x[M::RT][2];
                 v4u p[M::RT][El<BF16>::PARTS];
@@ -804,7 +816,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
                 half(wave >> 1);
             } else {
 #pragma unroll 1
-                for (int i = 0; i < 2; ++i) half(i);
+                for (int i = 0; i < M::TN / 32; ++i) half(i);
             }
         }
         if (care || !__syncthreads_or(w.any_nan())) break;
@@ -840,7 +852,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void many_kernel(AttnArgs a
 
 #pragma unroll
     for (int i = 0; i < M::RT; ++i) {
-        const int in = wave % (M::NW / WT) * 32 + 16 * i + (lane & 15), row = r0 + in;
+        const int in = wave % (M::NW / WT) * (16 * M::RT) + 16 * i + (lane & 15), row = r0 + in;
         const float total = w.whole_sum(i);
         if (in >= sp.rows) continue;
         float *out;
@@ -948,7 +960,7 @@ __global__ __launch_bounds__(256) void join_some_kernel(AttnArgs a) {
 // ---------------------------------------------------------------- host
 
 struct Plan {
-    int rows;  // of a block: 16 or 32 (few), 64 or 128
+    int rows;  // of a block: 16 or 32 (few), 64 or 128; 16 or 64 for over 128 dimensions
     int blocks, per, splits;
     bool few() const { return rows <= 32; }
 };
@@ -994,10 +1006,14 @@ Plan plan_of(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t n_tokens, 
     if (window && window + max_q + sinks < seen) seen = window + max_q + sinks;
     auto tiles = [&](int64_t tn) { return std::max((seen + tn - 1) / tn, (int64_t)1) + (window > 0); };
     auto blocks = [&](int64_t n) { return (rows + n - 1) / n; };
+    const bool wide = c.head_dim > 128;
     Plan p;
     // More than 16 rows, but little to see and few enough blocks of 16: the few-row kernel has more workgroups
-    // (prompts of 50, 100 and 200 tokens 7.5, 7.9 and 11.4 us; blocks of 64 rows 9.8, 11.5 and 13.8).
-    if (rows <= 16 || (tiles(32) <= 32 && blocks(16) * pairs <= 512)) p.rows = 16;
+    // (prompts of 50, 100 and 200 tokens 7.5, 7.9 and 11.4 us; blocks of 64 rows 9.8, 11.5 and 13.8).  For 256
+    // dimensions, where one workgroup fills a CU, up to one a CU (128 and 200 tokens 13.3 and 26.4 us, blocks of 64
+    // rows 15.3 and 19.5).
+    if (rows <= 16 || (tiles(32) <= 32 && blocks(16) * pairs <= (wide ? 256 : 512))) p.rows = 16;
+    else if (wide) p.rows = 64;
     else if (rows <= 32) p.rows = 32;
     else if (rows <= 64) p.rows = 64;
     else p.rows = 128;
@@ -1007,12 +1023,12 @@ Plan plan_of(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t n_tokens, 
         per = many_per(tiles(64), blocks(128) * pairs, result_bytes, &time);
         // Blocks of 64 rows, 2.1 us a tile, where those of 128 leave CUs idle and it costs no more: prompts of 333,
         // 1000 and 2000 tokens 18.3, 39.4 and 87.3 us instead of 23.6, 54.3 and 100.7; of 3000 172.5, not 158.1.
-        if (blocks(128) * pairs <= (c.head_dim > 128 ? 256 : 512) &&
+        if (blocks(128) * pairs <= 512 &&
             2.1 * (double)tiles(64) * std::max(1.0, (double)(blocks(64) * pairs) / 512.0) <= time)
             p.rows = 64, per = tiles(64);
     }
     p.blocks = (int)blocks(p.rows);
-    const int64_t n = tiles(p.few() ? 32 : 64), grid = p.blocks * pairs;
+    const int64_t n = tiles(p.few() || wide ? 32 : 64), grid = p.blocks * pairs;
     if (p.few()) per = few_per(n, grid, n_seqs);
     else if (per == 0) per = many_per(n, grid, result_bytes, &time);  // at most 64 rows
     per = std::max(per, (n + MAX_SPLITS - 1) / MAX_SPLITS);
@@ -1031,14 +1047,13 @@ bool fine_sizes(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t n_token
 
 template <bool BF16, int DP, bool FULL>
 int launch(const AttnArgs &a, const Plan &p, hipStream_t s) {
-    if (p.few()) {
-        const dim3 grid((unsigned)(a.c.n_kv_heads * p.blocks * a.n_seqs * p.splits));
-        if (p.rows == 16) hipLaunchKernelGGL((few_kernel<BF16, DP, FULL, 1>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((few_kernel<BF16, DP, FULL, 2>), grid, dim3(256), 0, s, a);
-    } else {
-        const dim3 grid((unsigned)(p.blocks * a.c.n_kv_heads * a.n_seqs), (unsigned)p.splits);
-        if (p.rows == 64) hipLaunchKernelGGL((many_kernel<BF16, DP, FULL, 2>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((many_kernel<BF16, DP, FULL, 1>), grid, dim3(256), 0, s, a);
+    const dim3 few((unsigned)(a.c.n_kv_heads * p.blocks * a.n_seqs * p.splits));
+    const dim3 many((unsigned)(p.blocks * a.c.n_kv_heads * a.n_seqs), (unsigned)p.splits);
+    if (p.rows == 16) hipLaunchKernelGGL((few_kernel<BF16, DP, FULL, 1>), few, dim3(256), 0, s, a);
+    else if (p.rows == 64) hipLaunchKernelGGL((many_kernel<BF16, DP, FULL, 64>), many, dim3(256), 0, s, a);
+    else if constexpr (DP < 256) {
+        if (p.rows == 32) hipLaunchKernelGGL((few_kernel<BF16, DP, FULL, 2>), few, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((many_kernel<BF16, DP, FULL, 128>), many, dim3(256), 0, s, a);
     }
     return (int)hipGetLastError();
 }
@@ -1057,10 +1072,13 @@ void launch_join(const AttnArgs &a, int64_t max_q, hipStream_t s) {
 
 template <int LANES>
 void launch_join(const AttnArgs &a, int rows, int64_t max_q, hipStream_t s) {
+    constexpr int DP = LANES * 4;
     if (rows == 16) launch_join<32, 16, LANES>(a, max_q, s);
-    else if (rows == 32) launch_join<32, 32, LANES>(a, max_q, s);
-    else if (rows == 64) launch_join<64, 64, LANES>(a, max_q, s);
-    else launch_join<64, 128, LANES>(a, max_q, s);
+    else if (rows == 64) launch_join<Many<DP, 64>::TN, 64, LANES>(a, max_q, s);
+    else if constexpr (DP < 256) {
+        if (rows == 32) launch_join<32, 32, LANES>(a, max_q, s);
+        else launch_join<64, 128, LANES>(a, max_q, s);
+    }
 }
 
 template <bool BF16>

@@ -158,6 +158,9 @@ def test_plan():
     assert plan(1, 4096, 4096) == (128, 1)
     assert plan(1, 512, 32768)[0] == 128 and splits.value > 1
     assert plan(1, 1, 1 << 30) == (16, 32)
+    wide = dict(head_dim=256, token_stride=256, head_stride=4096, page_stride=32768)
+    assert plan(1, 7, 4000, **wide)[0] == plan(1, 1000, 1000, **wide)[0] == plan(1, 9000, 9000, **wide)[0] == 64
+    assert plan(1, 4, 4000, **wide)[0] == plan(1, 100, 100, **wide)[0] == 16 and plan(1, 200, 200, **wide)[0] == 64
     assert plan(1, 1, 1 << 20, heads=1, n_kv_heads=1) == (16, 256)
     assert f(None, 32, 1, 1, 1, 100, 0, 0, None) == 0
     c = _cache()
