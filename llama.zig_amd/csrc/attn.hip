@@ -540,11 +540,14 @@ __global__ __launch_bounds__(256, RT * DP <= 128 ? 2 : 1) void few_kernel(AttnAr
     __shared__ float tops[F::NW][16 * RT], sums[F::NW][16 * RT];
     __shared__ uint32_t odd_bits[Odd<DP, 16 * RT>::WORDS];
     const Odd<DP, 16 * RT> odd = {odd_bits};
-    // Splits slowest: workgroups are dealt to the XCDs in turn, and the later splits of short sequences are
-    // empty (with splits first, four of them, XCDs 3 and 7 had only the longest sequences' last quarters).
+    // Workgroups are dealt to the eight XCDs in turn, and the later splits of short sequences are empty: splits
+    // slowest (first, four of them, XCDs 3 and 7 had only the longest sequences' last quarters), and where that would
+    // leave all splits of a sequence to the same few XCDs each split begins with another sequence (48 of up to 8191
+    // tokens, 4 heads: 100.7 -> 97.8 us).
     const int per_seq = a.c.n_kv_heads * a.blocks, pairs = a.n_seqs * per_seq;
-    const int split = blockIdx.x / pairs, pair = blockIdx.x - split * pairs, seq = pair / per_seq;
-    const int kvh = (pair - seq * per_seq) / a.blocks, block = pair - seq * per_seq - kvh * a.blocks;
+    const int split = blockIdx.x / pairs, pair = blockIdx.x - split * pairs, turn = pair / per_seq;
+    const int seq = (pairs & 7) == 0 && (per_seq & 7) ? (turn + split) % a.n_seqs : turn;
+    const int kvh = (pair - turn * per_seq) / a.blocks, block = pair - turn * per_seq - kvh * a.blocks;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int r0 = block * (16 * RT);
     // Three loads that do not wait for one another: the rows, the length, and
@@ -721,20 +724,13 @@ __global__ __launch_bounds__(256, 2) void many_kernel(AttnArgs a) {
     __shared__ uint32_t odd_bits[Odd<DP, ROWS>::WORDS];
     const Odd<DP, ROWS> odd = {odd_bits};
     const int split = blockIdx.y;
-    // Blocks of one (sequence, key-value head) share its keys and values: they
-    // go to one of the eight XCDs (workgroups are dealt to them in turn) as far
-    // as whole eights of pairs go.
-    const int pairs = a.n_seqs * a.c.n_kv_heads, whole = pairs & ~7;
-    int id = blockIdx.x, pair, block;
-    if (id < whole * a.blocks) {
-        pair = (id & 7) + 8 * ((id >> 3) / a.blocks);
-        block = (id >> 3) % a.blocks;
-    } else {
-        id -= whole * a.blocks;
-        pair = whole + id % (pairs - whole);
-        block = id / (pairs - whole);
-    }
-    const int s = pair / a.c.n_kv_heads, kvh = pair - s * a.c.n_kv_heads;
+    // Workgroups are dealt to the eight XCDs in turn.  Blocks of one key-value head share its keys and values, so a
+    // head goes to one XCD, or to 8 / n of them in turn; and every sequence to all of them, as its length may be any
+    // (three windowed prompts of up to 2500 tokens, 4 heads: 178 us, 217 with each pair of both on one XCD; eight of
+    // up to 1000 with one head 97 and 153).
+    const int H = a.c.n_kv_heads, n = min(H & -H, 8), xcd = blockIdx.x & 7;
+    const int id = (blockIdx.x >> 3) * (8 / n) + xcd / n, pair = id / a.blocks, block = id - pair * a.blocks;
+    const int s = pair / (H / n), kvh = (pair - s * (H / n)) * n + xcd % n;
     const Seq q = seq_of(a, s);
     const int all = q.m * a.group, mine = (all + ROWS - 1) / ROWS;
     if (block >= mine) return;

@@ -375,6 +375,15 @@ def test_every_kernel_form(form, window, sinks, dim, dtype):
     _check(c, window, sinks)
 
 
+@pytest.mark.parametrize("kv_heads,seqs", [(1, 1), (1, 8), (2, 3), (2, 4), (3, 3), (4, 1), (4, 3), (4, 6), (6, 2),
+                                           (12, 3), (16, 1), (24, 2)])
+@pytest.mark.parametrize("new,n", [(1, 3000), (40, 300), (300, 700), (200, 1500)])
+def test_every_block_and_split_is_done_once(kv_heads, seqs, new, n):
+    """Workgroups are dealt out by head, sequence and split: every order of them, with sequences of unlike lengths."""
+    lens = [n if i == 0 else (n * (3 * i + 1)) // (4 * i + 2) for i in range(seqs)]
+    _check(_case("f16", 2 * kv_heads, kv_heads, 64, page=32, lens=lens, new=[min(new, m) for m in lens]))
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("form", FORMS)
 def test_values_that_are_not_finite_in_every_kernel_form(form, bad):
