@@ -198,10 +198,10 @@ struct Pages {
     __device__ __forceinline__ int get(int i) const { return __builtin_amdgcn_readlane(mine, i - at); }
 };
 
-// Transfers of 1024 bytes, PER tokens each, that fill tiles.  The lane's offset in
-// a transfer depends on the transfer's number modulo NV alone: its chunk is
-// its position XOR the token's swizzle, whose part from the lane and part from the
-// transfer do not meet.  Chunks past the head repeat its last one.
+// Transfers of 1024 bytes, PER tokens each, that fill tiles.  The lane's offset
+// in a transfer depends on the transfer's number modulo NV alone: its chunk is
+// its position XOR the token's swizzle, whose part from the lane and part from
+// the transfer do not meet.  Chunks past the head repeat its last one.
 template <int DP>
 struct Loader {
     static constexpr int CH = DP / 8, PER = 64 / CH, NV = DP == 64 ? 2 : DP == 128 ? 4 : 8;
@@ -522,9 +522,18 @@ __device__ __forceinline__ float weight_of(float top, float m) {
 // ---------------------------------------------------------------- few rows
 
 // 16 * RT rows (one token's heads, or a few tokens'): bound by the reads of K
-// and V.  Every wave has tiles of 32 tokens of its own, in a ring of ST stages
-// whose K and V halves are refilled as soon as they have been read, with no
-// barrier.  At the end the waves' results are joined in LDS.
+// and V, and where those are few by the chain of dependent loads (length, page
+// numbers, keys).  Every wave has tiles of 32 tokens of its own, in a ring of
+// ST stages whose K and V halves are refilled as soon as they have been read,
+// with no barrier.  At the end the waves' results are joined in LDS.
+//
+// 32 query heads on 8 of 128 dimensions, f16: 131072 tokens (537 MB) 98 us, 5.5
+// TB/s (a large copy: 5.3); 16384 18.4; 4096 11.7; 333 8.7, where a launch is
+// 2.5.  100 sequences of a 1024-token window with 32 heads of 64 (819 MB): 151
+// us, 5.4 TB/s.  48 of up to 8191 in bf16 (447 MB): 98 us, 4.6 TB/s, with the
+// join's 5 us.  Four waves with one stage leave room for two workgroups a CU:
+// two stages took 9.4, 11.8 and 108 us for 333 tokens, 4096 and the 48, eight
+// waves 8.0, 12.0 and 105.
 template <int DP, int RT>
 struct Few {
     static constexpr int TN = 32, NW = 4, ST = DP == 64 ? 2 : 1, HALF = TN * DP * 2;
@@ -701,13 +710,19 @@ __global__ __launch_bounds__(256, RT * DP <= 128 ? 2 : 1) void few_kernel(AttnAr
 // ---------------------------------------------------------------- many rows
 
 // 128 rows, 32 per wave, against tiles of 64 tokens that the four waves share:
-// bound by the matrix cores and the softmax beside them, whose times add up.
+// bound by the matrix cores and the softmax beside them, whose times add up on
+// this part (a prompt of 4096 tokens, 32 heads on 8 of 128 in f16: 262 us, 525
+// TFLOP/s of the one product that counts, 1050 of the two that run; matrix
+// instructions are 44 % of the cycles, vector ones 31).  A row takes 5 to 6
+// vector operations per score, of which the exponential counts for four, so
+// that 16 rows a wave, which would double the reads of LDS, or parts of P
+// passed through LDS gain nothing.
 // Two stages: the next tile's transfers are in flight while one is contracted,
 // one barrier per tile.  With 64 rows two waves have the same rows and half of
 // the tokens each, and are joined at the end (WT = 2).  For 256 dimensions only
 // 64 rows, 16 per wave, and tiles of 32 tokens: two workgroups fit a CU, in 256
-// registers a lane, none in memory.  (With 32 rows per wave and tiles of 64 one did:
-// 2048 tokens 183 us in f16 and 360 in bf16, not 151 and 177; 13 tokens on
+// registers a lane, none in memory.  (With 32 rows per wave and tiles of 64 one
+// did: 2048 tokens 183 us in f16 and 360 in bf16, not 151 and 177; 13 tokens on
 // 20000 102 and 265, not 67 and 75.)
 template <int DP, int ROWS>
 struct Many {
@@ -876,6 +891,9 @@ __global__ __launch_bounds__(256, 2) void many_kernel(AttnArgs a) {
 
 // ---------------------------------------------------------------- join of the splits
 
+// A launch of its own: bound by its latency, 4 to 6 us.  (Joined in the same
+// launch by the last workgroup of a row, the flags' release and acquire wrote
+// the XCDs' L2 back and took longer: 16384 tokens 73 us instead of 19.)
 // For many splits one workgroup per row.  The weights of the splits first (in
 // LDS), then their results: LANES threads hold a row, the groups of them take
 // the splits in turn, four loads of each in flight, and are added in order.
@@ -925,7 +943,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
     *reinterpret_cast<v4f *>(result_row(a, q, kvh, r) + d) = total == 0.0f ? (v4f){} : o / total;
 }
 
-// For at most SOME_SPLITS of them LANES threads per row and nothing shared.
+// For at most SOME_SPLITS of them LANES threads per row and nothing shared (48 sequences of 4 splits: 5.0 us).
 template <int TN, int ROWS, int LANES>
 __global__ __launch_bounds__(256) void join_some_kernel(AttnArgs a) {
     const Seq q = seq_of(a, blockIdx.z);
