@@ -533,20 +533,20 @@ __device__ __forceinline__ float weight_of(float top, float m) {
 // us, 5.4 TB/s.  48 of up to 8191 in bf16 (447 MB): 98 us, 4.6 TB/s, with the
 // join's 5 us.  Four waves with one stage leave room for two workgroups a CU:
 // two stages took 9.4, 11.8 and 108 us for 333 tokens, 4096 and the 48, eight
-// waves 8.0, 12.0 and 105.
-template <int DP, int RT>
+// waves 8.0, 12.0 and 105.  With many short sequences NW is 1 (`plan_of`).
+template <int DP, int RT, int NW>
 struct Few {
-    static constexpr int TN = 32, NW = 4, ST = DP == 64 ? 2 : 1, HALF = TN * DP * 2;
+    static constexpr int TN = 32, ST = DP == 64 ? 2 : 1, HALF = TN * DP * 2;
     static constexpr int NX = HALF / 1024;     // transfers per half
     static constexpr int OS = DP + 4;          // floats of a row of results, off the banks' period
     static constexpr int RING = 2 * ST * HALF > 16 * RT * OS * 4 ? 2 * ST * HALF : 16 * RT * OS * 4;
 };
 
-template <bool BF16, int DP, bool FULL, int RT>
-__global__ __launch_bounds__(256, RT * DP <= 128 ? 2 : 1) void few_kernel(AttnArgs a) {
-    using F = Few<DP, RT>;
-    __shared__ __attribute__((aligned(1024))) uint8_t ring[F::NW][F::RING];
-    __shared__ float tops[F::NW][16 * RT], sums[F::NW][16 * RT];
+template <bool BF16, int DP, bool FULL, int RT, int NW>
+__global__ __launch_bounds__(64 * NW, RT * DP <= 128 ? 2 : 1) void few_kernel(AttnArgs a) {
+    using F = Few<DP, RT, NW>;
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[NW][F::RING];
+    __shared__ float tops[NW][16 * RT], sums[NW][16 * RT];
     __shared__ uint32_t odd_bits[Odd<DP, 16 * RT>::WORDS];
     const Odd<DP, 16 * RT> odd = {odd_bits};
     // Workgroups are dealt to the eight XCDs in turn, and the later splits of short sequences are empty: splits
@@ -580,7 +580,7 @@ __global__ __launch_bounds__(256, RT * DP <= 128 ? 2 : 1) void few_kernel(AttnAr
 
     const int64_t head = (int64_t)kvh * a.c.head_stride;
     const int begin = split * sp.per + wave, end = min(sp.count, (split + 1) * sp.per);
-    const int tiles = begin < end ? (end - begin + F::NW - 1) / F::NW : 0;
+    const int tiles = begin < end ? (end - begin + NW - 1) / NW : 0;
     const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_addr(ring[wave]));
     const Loader<DP> loader(a);
     const int more = a.c.page_shift == 4 ? 1 : 0;  // a tile spans two pages of 16 tokens
@@ -588,7 +588,7 @@ __global__ __launch_bounds__(256, RT * DP <= 128 ? 2 : 1) void few_kernel(AttnAr
     int64_t at0 = 0, at1 = 0;  // where the tile last begun lies
 
     auto issue_keys = [&](int i) {
-        const int t0 = sp.token(begin + i * F::NW), p = t0 >> a.c.page_shift, st = i % F::ST;
+        const int t0 = sp.token(begin + i * NW), p = t0 >> a.c.page_shift, st = i % F::ST;
         pages.hold(p, more, a.c.n_pages);
         const int p0 = pages.get(p), p1 = pages.get(p + more);
         const uint32_t ok = (p0 >= 0 ? 1 : 0) | (p1 >= 0 ? 2 : 0);
@@ -629,7 +629,7 @@ __global__ __launch_bounds__(256, RT * DP <= 128 ? 2 : 1) void few_kernel(AttnAr
         w.clear();
         if (tiles > 0) start();
         for (int i = 0; i < tiles; ++i) {
-            const int t0 = sp.token(begin + i * F::NW), st = i % F::ST;
+            const int t0 = sp.token(begin + i * NW), st = i % F::ST;
             const bool ok0 = oks >> (2 * st) & 1, ok1 = oks >> (2 * st) & 2;
             uint8_t *k = ring[wave] + st * 2 * F::HALF, *v = k + F::HALF;
             const int after = 2 * (tiles - i) - 1;  // halves to come after this tile's keys, those not yet issued too
@@ -671,15 +671,15 @@ __global__ __launch_bounds__(256, RT * DP <= 128 ? 2 : 1) void few_kernel(AttnAr
         __syncthreads();
         const int quads = a.c.head_dim >> 2;
         bool nan = false;
-        for (int i = threadIdx.x; i < sp.rows * quads; i += F::NW * 64) {
+        for (int i = threadIdx.x; i < sp.rows * quads; i += NW * 64) {
             const int r = i / quads, d = (i - r * quads) * 4;
             float m = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < F::NW; ++k) m = fmaxf(m, tops[k][r]);
+            for (int k = 0; k < NW; ++k) m = fmaxf(m, tops[k][r]);
             v4f o = {};
             float total = 0.0f;
 #pragma unroll
-            for (int k = 0; k < F::NW; ++k) {
+            for (int k = 0; k < NW; ++k) {
                 if (tops[k][r] == -INFINITY && sums[k][r] == 0.0f) continue;  // nothing seen
                 const float f = __builtin_amdgcn_exp2f(tops[k][r] - m);
                 const v4f u = *reinterpret_cast<const v4f *>(reinterpret_cast<const float *>(ring[k]) + r * F::OS + d);
@@ -701,7 +701,7 @@ __global__ __launch_bounds__(256, RT * DP <= 128 ? 2 : 1) void few_kernel(AttnAr
             }
         }
         if (care || !__syncthreads_or(nan)) return;
-        for (int i = threadIdx.x; i < odd.WORDS; i += F::NW * 64) odd_bits[i] = 0;
+        for (int i = threadIdx.x; i < odd.WORDS; i += NW * 64) odd_bits[i] = 0;
         __syncthreads();
         care = true;
     }
@@ -976,6 +976,7 @@ __global__ __launch_bounds__(256) void join_some_kernel(AttnArgs a) {
 struct Plan {
     int rows;  // of a block: 16 or 32 (few), 64 or 128; 16 or 64 for over 128 dimensions
     int blocks, per, splits;
+    int waves;  // of a few-row workgroup: 1 or 4
     bool few() const { return rows <= 32; }
 };
 
@@ -1048,6 +1049,11 @@ Plan plan_of(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t n_tokens, 
     per = std::max(per, (n + MAX_SPLITS - 1) / MAX_SPLITS);
     p.per = (int)per;
     p.splits = (int)((n + per - 1) / per);
+    // Many short sequences: one wave each, which starts alone and has no join (8 key-value heads of 128, 256 sequences
+    // of 50, 100 and 300 tokens 13.3, 17.7 and 42.3 us, four waves 26.3, 27.7 and 46.9; 500 of 100 34.4 and 55.1; 128
+    // of 100 and 500 12.3 and 36.5, 15.6 and 36.7; but 64 of 100 10.8 and 9.1).  For 256 dimensions a CU holds one
+    // workgroup of four (64 of 50 and 200 12.8 and 21.9, 18.0 and 24.6).
+    p.waves = p.rows == 16 && (n == 1 || (n <= 12 && grid >= (wide ? 512 : 1024))) ? 1 : 4;
     return p;
 }
 
@@ -1063,10 +1069,11 @@ template <bool BF16, int DP, bool FULL>
 int launch(const AttnArgs &a, const Plan &p, hipStream_t s) {
     const dim3 few((unsigned)(a.c.n_kv_heads * p.blocks * a.n_seqs * p.splits));
     const dim3 many((unsigned)(p.blocks * a.c.n_kv_heads * a.n_seqs), (unsigned)p.splits);
-    if (p.rows == 16) hipLaunchKernelGGL((few_kernel<BF16, DP, FULL, 1>), few, dim3(256), 0, s, a);
+    if (p.rows == 16 && p.waves == 1) hipLaunchKernelGGL((few_kernel<BF16, DP, FULL, 1, 1>), few, dim3(64), 0, s, a);
+    else if (p.rows == 16) hipLaunchKernelGGL((few_kernel<BF16, DP, FULL, 1, 4>), few, dim3(256), 0, s, a);
     else if (p.rows == 64) hipLaunchKernelGGL((many_kernel<BF16, DP, FULL, 64>), many, dim3(256), 0, s, a);
     else if constexpr (DP < 256) {
-        if (p.rows == 32) hipLaunchKernelGGL((few_kernel<BF16, DP, FULL, 2>), few, dim3(256), 0, s, a);
+        if (p.rows == 32) hipLaunchKernelGGL((few_kernel<BF16, DP, FULL, 2, 4>), few, dim3(256), 0, s, a);
         else hipLaunchKernelGGL((many_kernel<BF16, DP, FULL, 128>), many, dim3(256), 0, s, a);
     }
     return (int)hipGetLastError();

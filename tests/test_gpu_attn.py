@@ -384,6 +384,23 @@ def test_every_block_and_split_is_done_once(kv_heads, seqs, new, n):
     _check(_case("f16", 2 * kv_heads, kv_heads, 64, page=32, lens=lens, new=[min(new, m) for m in lens]))
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 80, 128, 256])
+@pytest.mark.parametrize("most,window,sinks", [(30, 0, 0), (380, 0, 0), (380, 100, 5)])
+def test_many_short_sequences(dtype, dim, most, window, sinks):
+    """A wave for each: from empty ones to the longest, values that are hidden or seen and not finite among them."""
+    lens = [most, 0, 1, most - 1] + [(37 * i) % most for i in range(13)]
+    c = _case(dtype, 64, 64, dim, page=16, lens=lens)
+    clean = _check(c, window, sinks)
+    last = int(c["table"][0, (most - 1) // 16])
+    c["v"][last, 5, most % 16:, :] = math.nan  # behind the end (most is no multiple of 16)
+    c["v"][last, 7, (most - 1) % 16, 11] = math.inf
+    got = _run(c, window, sinks)
+    assert float(got[0, 7, 11]) == math.inf
+    got[0, 7, 11] = clean[0, 7, 11]
+    assert torch.equal(got, clean)
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("form", FORMS)
 def test_values_that_are_not_finite_in_every_kernel_form(form, bad):
