@@ -381,7 +381,9 @@ def test_every_kernel_form(form, window, sinks, dim, dtype):
 def test_every_block_and_split_is_done_once(kv_heads, seqs, new, n):
     """Workgroups are dealt out by head, sequence and split: every order of them, with sequences of unlike lengths."""
     lens = [n if i == 0 else (n * (3 * i + 1)) // (4 * i + 2) for i in range(seqs)]
-    _check(_case("f16", 2 * kv_heads, kv_heads, 64, page=32, lens=lens, new=[min(new, m) for m in lens]))
+    c = _case("f16", 2 * kv_heads, kv_heads, 64, page=32, lens=lens, new=[min(new, m) for m in lens])
+    _check(c)
+    _check(c, max_kv=max(lens) // 2)  # planned as a prompt
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
