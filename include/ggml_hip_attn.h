@@ -149,13 +149,13 @@ int hip_qmm_kv_copy_pages(const hip_qmm_kv_cache *cache, const int32_t *src, con
  * Moves the pages in use to the front of the pool.  In use are the pages (in
  * [0, n_pages)) of the first ceil(kv_lens[s] / page_size) entries of each of
  * the n_seqs rows of page_table; rows may share pages.  With n_live of them,
- * the k-th page in use at or above n_live, ascending, moves to the k-th unused page
- * below n_live; table_out (n_seqs rows, its own stride, at least as wide;
- * table_out may be page_table with the same stride) receives page_table's
- * table_width entries with the new numbers, -1 for those not in use, and
- * *n_live the count: the pages from there on are free.  A freed sequence has length 0.  All on
- * the device, with no host synchronization.  n_pages at most 2^20; the workspace is
- * scratch.
+ * the k-th page in use at or above n_live, ascending, moves to the k-th unused
+ * page below n_live; table_out (n_seqs rows, its own stride, at least as wide;
+ * page_table itself with the same stride, or apart from it) receives
+ * page_table's table_width entries with the new numbers, -1 for those not in
+ * use, and *n_live (apart from the others) the count: the pages from there on
+ * are free.  A freed sequence has length 0.  All on the device, with no host
+ * synchronization.  n_pages at most 2^20; the workspace is scratch.
  */
 size_t hip_qmm_kv_compact_workspace_size(const hip_qmm_kv_cache *cache);
 int hip_qmm_kv_compact(const hip_qmm_kv_cache *cache, const int32_t *page_table, int64_t table_stride,

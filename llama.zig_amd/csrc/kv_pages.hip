@@ -264,7 +264,8 @@ __global__ __launch_bounds__(COPY_THREADS) void small_kernel(Cache c, const int3
     const uint32_t low = below == 32 ? ~0u : (1u << below) - 1;
     const int high = scan(__popc(bits & ~low), 1, &moves);
     high_before[tid] = (uint16_t)high;
-    int h = min(page0, live) - (before - high), k = high;  // unused pages below n_live before this word; pages in use from it on
+    // The unused pages below n_live before this word, and the pages in use from n_live on.
+    int h = min(page0, live) - (before - high), k = high;
     for (uint32_t b = ~bits & low; b; b &= b - 1) hole[h++] = (uint16_t)(page0 + __ffs(b) - 1);
     for (uint32_t b = bits & ~low; b; b &= b - 1) from[k++] = (uint16_t)(page0 + __ffs(b) - 1);
     __syncthreads();
@@ -281,14 +282,15 @@ __global__ __launch_bounds__(COPY_THREADS) void small_kernel(Cache c, const int3
     move_pages(c, from, hole, moves, run, blockIdx.x, gridDim.x);
 }
 
-
+// Whole pages that are runs: workgroup (part of a page, copy, keys or values).
 __global__ __launch_bounds__(COPY_THREADS) void copy_run_kernel(Cache c, const int32_t *__restrict__ src,
                                                                 const int32_t *__restrict__ dst, int64_t n_copies,
                                                                 int run) {
     for (int64_t i = blockIdx.y; i < n_copies; i += gridDim.y) {
         const int from = src[i], to = dst[i];
         if (from < 0 || to < 0 || from >= c.n_pages || to >= c.n_pages) continue;
-        copy_run((blockIdx.z ? c.v : c.k) + from * c.page_stride, (blockIdx.z ? c.v : c.k) + to * c.page_stride, run, blockIdx.x);
+        uint16_t *pool = blockIdx.z ? c.v : c.k;
+        copy_run(pool + from * c.page_stride, pool + to * c.page_stride, run, blockIdx.x);
     }
 }
 
@@ -333,7 +335,8 @@ extern "C" int hip_qmm_kv_compact(const hip_qmm_kv_cache *cache, const int32_t *
     // In one launch, unless a workgroup would read rows of the table that another has rewritten, or every one a
     // large table.
     const uintptr_t in0 = (uintptr_t)page_table, out0 = (uintptr_t)table_out;
-    const uintptr_t in1 = in0 + (size_t)(n_seqs * table_stride) * 4, out1 = out0 + (size_t)(n_seqs * out_stride) * 4;
+    const uintptr_t in1 = in0 + (size_t)n_seqs * (size_t)table_stride * 4;
+    const uintptr_t out1 = out0 + (size_t)n_seqs * (size_t)out_stride * 4;
     if (c.n_pages <= SMALL_PAGES && n_seqs <= SMALL_ENTRIES && table_width <= SMALL_ENTRIES &&
         n_seqs * table_width <= SMALL_ENTRIES && (in1 <= out0 || out1 <= in0)) {
         const int64_t units = c.n_pages / 2 * c.n_kv_heads * 2 + 1;
