@@ -360,7 +360,7 @@ FORMS = [  # rows of a workgroup, whether the tokens are split, sequences, new t
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("dim", [64, 80, 128, 256])
+@pytest.mark.parametrize("dim", [64, 80, 128, 192, 256])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (0, 3), (900, 5)])
 @pytest.mark.parametrize("form", FORMS)
 def test_every_kernel_form(form, window, sinks, dim, dtype):
@@ -387,7 +387,7 @@ def test_every_block_and_split_is_done_once(kv_heads, seqs, new, n):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("dim", [64, 80, 128, 256])
+@pytest.mark.parametrize("dim", [64, 80, 128, 192, 256])
 @pytest.mark.parametrize("most,window,sinks", [(30, 0, 0), (380, 0, 0), (380, 100, 5)])
 def test_many_short_sequences(dtype, dim, most, window, sinks):
     """A wave for each: from empty ones to the longest, values that are hidden or seen and not finite among them."""
