@@ -164,10 +164,12 @@ __device__ __forceinline__ int swizzle(int t) { return DP == 64 ? (t >> 1) & 7 :
 // 16 bytes per lane from base + off to LDS at lds_base + 16 * lane (base and
 // lds_base wave-uniform).  Inline assembly, so that the compiler, which cannot
 // tell the stages of a ring apart, puts no vmcnt(0) of its own before the LDS
-// reads of another stage; every wait is wait_vm's.  M0 holds the LDS base, the s_nop
-// separates its write from the transfer.
+// reads of another stage; every wait is wait_vm's.  M0 holds the LDS base.  The
+// s_nop is what M0's write, and a base written by a vector instruction (lanes
+// read back, as the compiler keeps scalars that do not fit), need before they
+// are read, since it counts no wait states for an asm statement.
 __device__ __forceinline__ void dma16(const uint16_t *base, uint32_t off, uint32_t lds_base) {
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds_base) : "memory");
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds_base) : "memory");
 }
 
 template <int N>

@@ -61,7 +61,7 @@ def test_one_token_head_layouts(dtype, heads, kv_heads):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("dim", [8, 16, 40, 64, 72, 80, 96, 112, 128, 136, 192, 256])
+@pytest.mark.parametrize("dim", [8, 16, 40, 64, 72, 80, 96, 104, 112, 128, 136, 192, 200, 248, 256])
 def test_head_dims(dtype, dim):
     _check(_case(dtype, 8, 2, dim, lens=(1, 33, 300)))
     _check(_case(dtype, 8, 2, dim, lens=(40, 33, 300), new=[40, 5, 100]))
@@ -360,7 +360,7 @@ FORMS = [  # rows of a workgroup, whether the tokens are split, sequences, new t
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("dim", [64, 80, 128, 192, 256])
+@pytest.mark.parametrize("dim", [64, 80, 128, 192, 248, 256])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (0, 3), (900, 5)])
 @pytest.mark.parametrize("form", FORMS)
 def test_every_kernel_form(form, window, sinks, dim, dtype):
