@@ -836,13 +836,14 @@ __global__ __launch_bounds__(256, 2) void many_kernel(AttnArgs a) {
                 for (int i = 0; i < M::TN / 32; ++i) half(i);
             }
         }
-        if (care || !__syncthreads_or(w.any_nan())) break;
+        // A barrier after either pass: the join below writes over the stages, which other waves may still read.
+        if (!__syncthreads_or(!care && w.any_nan())) break;
         for (int i = threadIdx.x; i < odd.WORDS; i += 256) odd_bits[i] = 0;
         __syncthreads();  // (which also frees both stages)
         care = true;
         if (begin < end) start();
     }
-    if constexpr (WT == 2) {  // the stages are free: the check above was a barrier
+    if constexpr (WT == 2) {  // the stages are free: each pass ended in a barrier
         v4f *other = reinterpret_cast<v4f *>(stage[0]) + (wave & 1) * 64 * M::RT * (DU / 16 + 1) + lane;
         if (wave >= 2) {
 #pragma unroll
