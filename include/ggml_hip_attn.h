@@ -105,8 +105,10 @@ int hip_qmm_rope_kv_store(const float *q, int64_t n_heads, int64_t q_token_strid
  * key-value head h / (n_heads / n_kv_heads):
  *   dst[t][h] = sum_j w_j v_j / sum_j w_j,   w_j = exp(scale * q[t][h].k_j)
  * over the tokens it sees, a zero row where it sees none (as for a query at a
- * negative position, where m > n).  What hidden tokens hold, NaN and infinities
- * too, does not matter.  Results are f32 throughout: q and w enter the matrix
+ * negative position, where m > n) or only scores of -infinity.  What hidden
+ * tokens hold, NaN and infinities too, does not matter; what is seen counts as
+ * IEEE arithmetic has it (an infinite key gives a weight of 0 or a row of NaN),
+ * and a query that is not finite gives a row of NaN.  Results are f32 throughout: q and w enter the matrix
  * cores as sums of f16 or bf16 parts that hold 22 bits and more.
  * q_starts ascends from 0 or more to n_tokens or less; max_q is at least the
  * largest m; max_kv, the largest length in the host's knowledge, only plans the

@@ -21,6 +21,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_cache.h"
 
@@ -443,7 +444,12 @@ __device__ __forceinline__ bool is_edge(const AttnArgs &a, const Span<TN> &sp, i
     return t0 + TN - 1 > sp.p_first || (a.window && t0 <= sp.p_last - a.window && t0 + TN > a.sinks);
 }
 
-// Row r of a block (a valid one): where its result goes.
+// Row r of a sequence (a valid one): its query, and where its result goes.
+__device__ __forceinline__ const float *query_row(const AttnArgs &a, const Seq &q, int kvh, int r) {
+    const int t = r / a.group, g = r - t * a.group;
+    return a.q + (int64_t)(q.first + t) * a.q_token + (int64_t)(kvh * a.group + g) * a.q_head;
+}
+
 __device__ __forceinline__ float *result_row(const AttnArgs &a, const Seq &q, int kvh, int r) {
     const int t = r / a.group, g = r - t * a.group;
     return a.dst + (int64_t)(q.first + t) * a.dst_token + (int64_t)(kvh * a.group + g) * a.dst_head;
@@ -472,48 +478,92 @@ __device__ __forceinline__ void blank(const AttnArgs &a, const Span<TN> &sp, uin
     }
 }
 
-// ---------------------------------------------------------------- values that are not finite
+// ---------------------------------------------------------------- keys and values that are not finite
 
-// One that some rows of a block see and others do not must not reach the
+// A value that some rows of a block see and others do not must not reach the
 // others, where its weight is 0; and seen, it must not meet a weight's parts of
-// both signs.  No test for them is in the tiles' loops: a block whose results
-// hold a NaN is done again, and then each tile's values that are not finite
-// become zeros before it is contracted, and are noted by row and dimension: two
-// bits, inf and -inf, both for NaN and for a sum of the two.
-template <int DP, int ROWS>
+// both signs, nor an infinite key a query's parts.  No test for them is in the
+// tiles' loops: a block whose results hold a NaN is done again, and then each
+// tile's elements that are not finite become zeros before it is contracted, and
+// are noted, in two bits each: inf and -inf, both for NaN and for a sum of the
+// two.  Of values it is a row's and a dimension's, added to the results; of
+// keys a row's and a token's, the query's element times the key's, added to the
+// tile's scores.
+template <int DP, int ROWS, int TN>
 struct Odd {
-    static constexpr int WORDS = ROWS * DP / 16;
-    uint32_t *bits;
+    static constexpr int WORDS = ROWS * DP / 16, KEY_WORDS = ROWS * TN / 16;
+    uint32_t *bits, *key_bits;  // by row and dimension; by row and the tile's token
 
-    // The values of `tokens` tokens (t0 on) at lds, by threads first, first + step, ...
-    template <bool BF16>
-    __device__ __forceinline__ void sift(const AttnArgs &a, uint8_t *tile, int tokens, int t0, int ok, const int first_row,
-                                         const int rows, int first, int step, int p_first_row) const {
+    static __device__ __forceinline__ float number(uint32_t kind) {
+        return kind == 1 ? INFINITY : kind == 2 ? -INFINITY : NAN;
+    }
+
+    // What is not finite in the tile of t0 becomes 0; note(row, token, dimension, kind) for each row that sees it.  By
+    // threads first, first + step, ...; the block's rows begin at first_row of the sequence, whose first position is p0.
+    template <bool BF16, class Note>
+    static __device__ __forceinline__ void sift(const AttnArgs &a, uint8_t *tile, int t0, int ok, int first_row, int rows,
+                                                int first, int step, int p0, Note note) {
         constexpr uint32_t INF = El<BF16>::INF;
-        for (int i = first; i < tokens * (DP / 2); i += step) {
+        for (int i = first; i < TN * (DP / 2); i += step) {
             uint32_t *w = reinterpret_cast<uint32_t *>(tile) + i;
             const uint32_t pair = *w;
             const bool lo = (pair & INF) == INF, hi = (pair >> 16 & INF) == INF;
             if (!lo && !hi) continue;
             *w = pair & (lo ? 0xffff0000u : ~0u) & (hi ? 0x0000ffffu : ~0u);
             const int t = i / (DP / 2), d = (((i & (DP / 2 - 1)) >> 2) ^ swizzle<DP>(t)) * 8 + (i & 3) * 2;
-            if (!(ok >> (t >> 4) & 1)) continue;
+            if (!(ok >> (t >> 4) & 1) || d >= a.c.head_dim) continue;  // past the head: its last chunk again
             for (int r = 0; r < rows; ++r) {
-                const int p = p_first_row + (first_row + r) / a.group, j = t0 + t;
+                const int p = p0 + (first_row + r) / a.group, j = t0 + t;
                 if (!(j <= p && (!a.window || p - j < a.window || j < a.sinks))) continue;
                 for (int e = 0; e < 2; ++e) {
                     const uint32_t b = pair >> (16 * e) & 0xffffu;
-                    if ((b & INF) != INF) continue;
-                    const uint32_t kind = b == INF ? 1 : b == (INF | 0x8000u) ? 2 : 3;
-                    atomicOr(&bits[r * (DP / 16) + (d >> 4)], kind << (2 * ((d & 15) + e)));
+                    if ((b & INF) == INF) note(r, t, d + e, b == INF ? 1u : b == (INF | 0x8000u) ? 2u : 3u);
                 }
             }
         }
     }
+    __device__ __forceinline__ void clear_keys(int first, int step) const {
+        for (int i = first; i < KEY_WORDS; i += step) key_bits[i] = 0;
+    }
+    // The tile's keys; rows of q from the sequence's on.
+    template <bool BF16>
+    __device__ __forceinline__ void sift_keys(const AttnArgs &a, const Seq &q, int kvh, uint8_t *tile, int t0, int ok,
+                                              int first_row, int rows, int first, int step) const {
+        sift<BF16>(a, tile, t0, ok, first_row, rows, first, step, q.n - q.m, [&](int r, int t, int d, uint32_t kind) {
+            const float x = query_row(a, q, kvh, first_row + r)[d];
+            if (x == 0.0f || x != x || a.scale == 0.0f) kind = 3;
+            else if (kind != 3 && (x < 0.0f) != (a.scale < 0.0f)) kind ^= 3;
+            atomicOr(&key_bits[r * (TN / 16) + (t >> 4)], kind << (2 * (t & 15)));
+        });
+    }
+    // The tile's values, after its keys: times a weight of exactly 0 (a score of -inf) an infinity is NaN.
+    template <bool BF16>
+    __device__ __forceinline__ void sift_values(const AttnArgs &a, const Seq &q, uint8_t *tile, int t0, int ok,
+                                                int first_row, int rows, int first, int step) const {
+        sift<BF16>(a, tile, t0, ok, first_row, rows, first, step, q.n - q.m, [&](int r, int t, int d, uint32_t kind) {
+            if (key_bits[r * (TN / 16) + (t >> 4)] >> (2 * (t & 15)) & 3) kind = 3;
+            atomicOr(&bits[r * (DP / 16) + (d >> 4)], kind << (2 * (d & 15)));
+        });
+    }
+    // Scores of the tile's tokens [t, t + 32), as Rows::scores leaves them, for rows from r0 on.
+    template <int RT>
+    __device__ __forceinline__ void apply_keys(int r0, int t, v4f (&s)[RT][2]) const {
+        int lane = threadIdx.x & 63;
+        asm("" : "+v"(lane));  // nothing of this is computed ahead of the tiles' loop, whose registers are full
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t k = key_bits[(r0 + 16 * i + (lane & 15)) * (TN / 16) + (t >> 4) + j] >> (8 * (lane >> 4));
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (k >> (2 * e) & 3) s[i][j][e] += number(k >> (2 * e) & 3);
+            }
+    }
     // Row r's dimension d, given its result without them.
     __device__ __forceinline__ float apply(int r, int d, float x) const {
         const uint32_t k = bits[r * (DP / 16) + (d >> 4)] >> (2 * (d & 15)) & 3;
-        return k == 0 ? x : x + (k == 1 ? INFINITY : k == 2 ? -INFINITY : NAN);
+        return k == 0 ? x : x + number(k);
     }
 };
 
@@ -551,8 +601,8 @@ __global__ __launch_bounds__(64 * NW, RT * DP <= 128 ? 2 : 1) void few_kernel(At
     using F = Few<DP, RT, NW>;
     __shared__ __attribute__((aligned(1024))) uint8_t ring[NW][F::RING];
     __shared__ float tops[NW][16 * RT], sums[NW][16 * RT];
-    __shared__ uint32_t odd_bits[Odd<DP, 16 * RT>::WORDS];
-    const Odd<DP, 16 * RT> odd = {odd_bits};
+    using O = Odd<DP, 16 * RT, F::TN>;
+    __shared__ uint32_t odd_bits[O::WORDS], odd_keys[NW][O::KEY_WORDS];
     // Workgroups are dealt to the eight XCDs in turn, and the later splits of short sequences are empty: splits
     // slowest (first, four of them, XCDs 3 and 7 had only the longest sequences' last quarters), and where that would
     // leave all splits of a sequence to the same few XCDs each split begins with another sequence (48 of up to 8191
@@ -563,6 +613,7 @@ __global__ __launch_bounds__(64 * NW, RT * DP <= 128 ? 2 : 1) void few_kernel(At
     const int kvh = (pair - turn * per_seq) / a.blocks, block = pair - turn * per_seq - kvh * a.blocks;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int r0 = block * (16 * RT);
+    const O odd = {odd_bits, odd_keys[wave]};
     // Three loads that do not wait for one another: the rows, the length, and
     // the pages of the tile that is this wave's first where the length does
     // not change the split and there is no window.
@@ -628,8 +679,10 @@ __global__ __launch_bounds__(64 * NW, RT * DP <= 128 ? 2 : 1) void few_kernel(At
         const int in = 16 * i + (lane & 15);
         w.take_row(a, i, raw[i], in < sp.rows ? q.n - q.m + (r0 + in) / a.group : -1);
     }
-    bool care = false;
-    for (;;) {
+    // One pass over the tiles, and the join of the waves; whether some result is NaN.  Two copies of the code: the first
+    // pass keeps the registers of a loop that cares for nothing.
+    auto pass = [&](auto careful) {
+        constexpr bool care = decltype(careful)::value;
         w.clear();
         if (tiles > 0) start();
         for (int i = 0; i < tiles; ++i) {
@@ -640,7 +693,14 @@ __global__ __launch_bounds__(64 * NW, RT * DP <= 128 ? 2 : 1) void few_kernel(At
             wait_halves(min(after, 2 * F::ST - 1));
             v4f s[RT][2];
             v4u p[RT][El<BF16>::PARTS];
+            if (care) {
+                odd.clear_keys(lane, 64);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                odd.template sift_keys<BF16>(a, q, kvh, k, t0, ok0 | ok1 << 1, r0, sp.rows, lane, 64);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            }
             w.scores(a, k, 0, s);
+            if (care) odd.apply_keys(0, 0, s);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the keys have been read: their half may be refilled
             if (i + F::ST < tiles) issue_keys(i + F::ST);
             if (is_edge<F::TN>(a, sp, t0) || !(ok0 && ok1)) w.hide(a, s, t0, ok0, ok1);
@@ -648,7 +708,7 @@ __global__ __launch_bounds__(64 * NW, RT * DP <= 128 ? 2 : 1) void few_kernel(At
             wait_halves(min(after - 1, 2 * F::ST - 1));
             if (care || has_unseen<F::TN>(a, sp, t0) || !(ok0 && ok1)) {
                 blank<DP, F::TN>(a, sp, v, t0, ok0 | ok1 << 1, lane, 64);
-                if (care) odd.template sift<BF16>(a, v, F::TN, t0, ok0 | ok1 << 1, r0, sp.rows, lane, 64, q.n - q.m);
+                if (care) odd.template sift_values<BF16>(a, q, v, t0, ok0 | ok1 << 1, r0, sp.rows, lane, 64);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             }
             w.gather(v, 0, p);
@@ -704,11 +764,12 @@ __global__ __launch_bounds__(64 * NW, RT * DP <= 128 ? 2 : 1) void few_kernel(At
                 if (d == 0) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = make_float2(m, total);
             }
         }
-        if (care || !__syncthreads_or(nan)) return;
-        for (int i = threadIdx.x; i < odd.WORDS; i += NW * 64) odd_bits[i] = 0;
-        __syncthreads();
-        care = true;
-    }
+        return nan;
+    };
+    if (!__syncthreads_or(pass(std::false_type{}))) return;
+    for (int i = threadIdx.x; i < O::WORDS; i += NW * 64) odd_bits[i] = 0;
+    __syncthreads();
+    pass(std::true_type{});
 }
 
 // ---------------------------------------------------------------- many rows
@@ -740,8 +801,9 @@ __global__ __launch_bounds__(256, 2) void many_kernel(AttnArgs a) {
     using M = Many<DP, ROWS>;
     constexpr int WT = M::WT;
     __shared__ __attribute__((aligned(1024))) uint8_t stage[2][M::STAGE];
-    __shared__ uint32_t odd_bits[Odd<DP, ROWS>::WORDS];
-    const Odd<DP, ROWS> odd = {odd_bits};
+    using O = Odd<DP, ROWS, M::TN>;
+    __shared__ uint32_t odd_bits[O::WORDS], odd_keys[O::KEY_WORDS];
+    const O odd = {odd_bits, odd_keys};
     const int split = blockIdx.y;
     // Workgroups are dealt to the eight XCDs in turn.  Blocks of one key-value head share its keys and values, so a
     // head goes to one XCD, or to 8 / n of them in turn; and every sequence to all of them, as its length may be any
@@ -800,8 +862,9 @@ __global__ __launch_bounds__(256, 2) void many_kernel(AttnArgs a) {
             in < sp.rows);
         w.take_row(a, i, raw, in < sp.rows ? q.n - q.m + tok : -1);
     }
-    bool care = false;
-    for (;;) {
+    // One pass over the tiles.  Two copies of the code: the first pass keeps the registers of a loop that cares for nothing.
+    auto pass = [&](auto careful) {
+        constexpr bool care = decltype(careful)::value;
         w.clear();
         for (int u = begin; u < end; ++u) {
             wait_vm<0>();
@@ -811,9 +874,15 @@ __global__ __launch_bounds__(256, 2) void many_kernel(AttnArgs a) {
             const int ok = oks >> (M::GROUPS * (u & 1)) & M::ALL, t0 = sp.token(u);
             if (u + 1 < end) issue(u + 1);
             uint8_t *k = stage[u & 1], *v = k + M::HALF;
+            if (care) {
+                odd.clear_keys(threadIdx.x, 256);
+                __syncthreads();
+                odd.template sift_keys<BF16>(a, q, kvh, k, t0, ok, r0, sp.rows, threadIdx.x, 256);
+                __syncthreads();
+            }
             if (care || has_unseen<M::TN>(a, sp, t0) || ok != M::ALL) {
                 blank<DP, M::TN>(a, sp, v, t0, ok, threadIdx.x, 256);
-                if (care) odd.template sift<BF16>(a, v, M::TN, t0, ok, r0, sp.rows, threadIdx.x, 256, q.n - q.m);
+                if (care) odd.template sift_values<BF16>(a, q, v, t0, ok, r0, sp.rows, threadIdx.x, 256);
                 asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             }
             const bool edge = is_edge<M::TN>(a, sp, t0) || ok != M::ALL;
@@ -821,6 +890,7 @@ __global__ __launch_bounds__(256, 2) void many_kernel(AttnArgs a) {
                 v4f x[M::RT][2];
                 v4u p[M::RT][El<BF16>::PARTS];
                 w.scores(a, k, 32 * i, x);
+                if (care) odd.apply_keys(wave % (M::NW / WT) * (16 * M::RT), 32 * i, x);
                 if (edge) w.hide(a, x, t0 + 32 * i, ok >> (2 * i) & 1, ok >> (2 * i + 1) & 1);
                 // Matrix instructions first where the SIMD's other wave is at its softmax (274 -> 267 us for a
                 // prompt of 4096 tokens in f16, 353 -> 340 in bf16).
@@ -836,12 +906,15 @@ __global__ __launch_bounds__(256, 2) void many_kernel(AttnArgs a) {
                 for (int i = 0; i < M::TN / 32; ++i) half(i);
             }
         }
-        // A barrier after either pass: the join below writes over the stages, which other waves may still read.
-        if (!__syncthreads_or(!care && w.any_nan())) break;
-        for (int i = threadIdx.x; i < odd.WORDS; i += 256) odd_bits[i] = 0;
+    };
+    pass(std::false_type{});
+    const bool care = __syncthreads_or(w.any_nan());
+    if (care) {
+        for (int i = threadIdx.x; i < O::WORDS; i += 256) odd_bits[i] = 0;
         __syncthreads();  // (which also frees both stages)
-        care = true;
         if (begin < end) start();
+        pass(std::true_type{});
+        __syncthreads();  // as after the first pass: the join below writes over the stages
     }
     if constexpr (WT == 2) {  // the stages are free: each pass ended in a barrier
         v4f *other = reinterpret_cast<v4f *>(stage[0]) + (wave & 1) * 64 * M::RT * (DU / 16 + 1) + lane;
@@ -887,7 +960,7 @@ __global__ __launch_bounds__(256, 2) void many_kernel(AttnArgs a) {
         for (int d = 0; d < DU / 16; ++d) {
             const int e = d * 16 + 4 * (lane >> 4);
             v4f x = w.o[i][d] * f;
-            if (care) {
+            if (care && (sp.active > 1 || total != 0.0f)) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) x[c] = odd.apply(in, e + c, x[c]);
             }
