@@ -295,7 +295,8 @@ struct Rows {
             }
         big = quarter_max(big);
         const int ex = (int)(__float_as_uint(big) >> 23);  // biased; 255: not finite, left as it is
-        const int up = ex == 255 || ex == 0 ? 0 : min(E::QUERY - (ex - 127), 120);
+        // Not below -126, so that unit is finite: a largest query's parts then stay below 4.
+        const int up = ex == 255 || ex == 0 ? 0 : max(min(E::QUERY - (ex - 127), 120), -126);
         unit[i] = ldexpf(1.0f, -up);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
