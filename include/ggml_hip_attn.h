@@ -111,12 +111,16 @@ int hip_qmm_rope_kv_store(const float *q, int64_t n_heads, int64_t q_token_strid
  * and a query that is not finite gives a row of NaN.  Results are f32 throughout: q and w enter the matrix
  * cores as sums of f16 or bf16 parts that hold 22 bits and more.
  * q_starts ascends from 0 or more to n_tokens or less; max_q is at least the
- * largest m; max_kv, the largest length in the host's knowledge, only plans the
- * work.  n_heads a multiple of n_kv_heads; q and dst 16-byte aligned with strides
- * that are multiples of 4 floats; dst does not overlap q; window, sinks and
- * max_kv in [0, 2^30]; n_tokens at most 2^23, its product with
- * n_heads / n_kv_heads at most 2^30.  Deterministic.  The workspace is scratch:
- * its contents do not matter before the call, and it serves one call at a time.
+ * largest m and at most n_tokens; max_kv, the largest length in the host's
+ * knowledge, only plans the work.  n_heads a multiple of n_kv_heads; q and dst
+ * 16-byte aligned with strides that are multiples of 4 floats, dst's tokens
+ * apart (dst_token_stride at least (n_heads - 1) * dst_head_stride + head_dim);
+ * dst does not overlap q; window, sinks and max_kv in [0, 2^30]; n_heads and
+ * n_seqs at most 65535; n_tokens at most 2^23, its product with
+ * n_heads / n_kv_heads at most 2^30; n_seqs * n_kv_heads * ceil(max_q * n_heads
+ * / n_kv_heads / R) at most 2^23, R the 16 to 128 rows of a workgroup that the
+ * sizes give.  Deterministic.  The workspace is scratch: its contents do not
+ * matter before the call, and it serves one call at a time.
  */
 size_t hip_qmm_attn_paged_workspace_size(const hip_qmm_kv_cache *cache, int64_t n_heads, int64_t n_seqs,
                                          int64_t n_tokens, int64_t max_q, int64_t max_kv, int64_t window,

@@ -1094,7 +1094,10 @@ int64_t many_per(int64_t tiles, int64_t grid, double result_bytes, double *time)
     return per < tiles ? std::max((tiles * grid + 511) / 512, std::min(per, (int64_t)2)) : tiles;
 }
 
-// Which kernel, its rows per workgroup, and how the tokens are split.
+constexpr int64_t MAX_GROUPS = 1 << 23;  // workgroups of a launch
+
+// Which kernel, its rows per workgroup, and how the tokens are split; rows is 0 where even unsplit it is too many
+// workgroups.
 Plan plan_of(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t n_tokens, int64_t max_q, int64_t max_kv,
              int64_t window, int64_t sinks) {
     const int64_t rows = max_q * (n_heads / c.n_kv_heads), pairs = c.n_kv_heads * n_seqs;
@@ -1125,10 +1128,15 @@ Plan plan_of(const Cache &c, int64_t n_heads, int64_t n_seqs, int64_t n_tokens, 
             p.rows = 64, per = tiles(64);
     }
     p.blocks = (int)blocks(p.rows);
-    const int64_t n = tiles(p.few() || wide ? 32 : 64), grid = p.blocks * pairs;
+    const int64_t n = tiles(p.few() || wide ? 32 : 64), grid = blocks(p.rows) * pairs;
     if (p.few()) per = few_per(n, grid, n_seqs);
     else if (per == 0) per = many_per(n, grid, result_bytes, &time);  // at most 64 rows
-    per = std::max(per, (n + MAX_SPLITS - 1) / MAX_SPLITS);
+    if (grid > MAX_GROUPS) {
+        p.rows = 0;
+        return p;
+    }
+    const int64_t most = std::min((int64_t)MAX_SPLITS, MAX_GROUPS / grid);
+    per = std::max(per, (n + most - 1) / most);
     p.per = (int)per;
     p.splits = (int)((n + per - 1) / per);
     // Prompts: their last blocks see most, and go first in every head (4096 tokens of 32 key-value heads 274 us, head
@@ -1211,7 +1219,7 @@ extern "C" size_t hip_qmm_attn_paged_workspace_size(const hip_qmm_kv_cache *cach
         n_seqs == 0)
         return 0;
     const Plan p = plan_of(c, n_heads, n_seqs, n_tokens, max_q, max_kv, window, sinks);
-    return p.splits == 1 ? 0 : (size_t)p.splits * n_tokens * n_heads * (c.head_dim + 2) * sizeof(float);
+    return p.rows == 0 || p.splits == 1 ? 0 : (size_t)p.splits * n_tokens * n_heads * (c.head_dim + 2) * sizeof(float);
 }
 
 extern "C" int hip_qmm_attn_paged_rows(const hip_qmm_kv_cache *cache, int64_t n_heads, int64_t n_seqs,
@@ -1222,7 +1230,7 @@ extern "C" int hip_qmm_attn_paged_rows(const hip_qmm_kv_cache *cache, int64_t n_
         n_seqs == 0)
         return 0;
     const Plan p = plan_of(c, n_heads, n_seqs, n_tokens, max_q, max_kv, window, sinks);
-    if (splits) *splits = p.splits;
+    if (splits && p.rows) *splits = p.splits;
     return p.rows;
 }
 
@@ -1247,8 +1255,8 @@ extern "C" int hip_qmm_attn_paged(const hip_qmm_kv_cache *cache, const float *q,
         (n_tokens > 1 && dst_token_stride < (n_heads - 1) * dst_head_stride + D))
         return (int)hipErrorInvalidValue;
     const Plan p = plan_of(a.c, n_heads, n_seqs, n_tokens, max_q, max_kv, window, sinks);
+    if (p.rows == 0) return (int)hipErrorInvalidValue;
     const int64_t rows = (int64_t)p.splits * n_tokens * n_heads;
-    if ((int64_t)p.blocks * H * n_seqs * p.splits > (1 << 23)) return (int)hipErrorInvalidValue;
     if (p.splits > 1 && (!workspace || ((uintptr_t)workspace & 15) ||
                          workspace_size < (size_t)rows * (D + 2) * sizeof(float)))
         return (int)hipErrorInvalidValue;

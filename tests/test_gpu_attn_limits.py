@@ -2,7 +2,8 @@
 arguments may hold."""
 import pytest
 
-from test_gpu_attn import _case, _check
+import attn_ref as R
+from test_gpu_attn import _case, _check, _hold, _run
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -30,3 +31,19 @@ def test_the_largest_queries_on_keys_of_zero(new, dtype):
     c["q"].copy_(torch.copysign(torch.full_like(c["q"], 3.4e38), c["q"]))
     c["k"].zero_()
     _check(c)
+
+
+def test_planned_for_more_workgroups_than_a_launch_has():
+    """2048 sequences of 64 heads planned for 2^20 tokens: fewer splits than such a length would have alone."""
+    import ggml_hip as G
+    c = _case("f16", 64, 64, 64, lens=[40000] + [1 + i % 16 for i in range(2047)])
+    c["table"] = torch.nn.functional.pad(c["table"], (0, 65536 - c["table"].shape[1]), value=-1)
+    rows, splits = G.attn_paged_plan(G.PagedKV(c["k"], c["v"]), 64, 2048, 2048, 1, 1 << 20)
+    assert rows == 16 and splits > 2 and splits * 64 * 2048 <= 1 << 23
+    got = _run(c)
+    exact = _run(c, max_kv=40000)
+    for s in (slice(0, 1), slice(1, 40), slice(2000, 2048)):
+        want, top = R.attention(c["q"][s], c["k"], c["v"], c["table"][s], c["lens"][s], c["starts"][:s.stop - s.start + 1],
+                                64 ** -0.5)
+        _hold(got[s], want, top, 64)
+        _hold(exact[s], want, top, 64)
