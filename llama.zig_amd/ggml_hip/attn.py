@@ -57,13 +57,26 @@ def _need(ok, what):
         raise HipQmmError(what)
 
 
-def _raw_stream(t):
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
+def _raw_stream(device):
+    # A launch goes to the current device, whatever its stream's.
+    if device != torch._C._cuda_getDevice():
+        raise HipQmmError("tensors must live on the current GPU")
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
-def _int32(t, n, name):
-    if not (t.dtype is torch.int32 and t.is_cuda and t.numel() == n and t.is_contiguous()):
-        raise HipQmmError(f"{name} must be {n} contiguous int32 values on the GPU")
+def _int32(t, n, name, device):
+    if not (t.dtype is torch.int32 and t.get_device() == device and t.numel() == n and t.is_contiguous()):
+        raise HipQmmError(f"{name} must be {n} contiguous int32 values on the GPU of the others")
+
+
+def _scratch(workspace, need, device):
+    """A caller's scratch, checked: its address and bytes."""
+    have = workspace.numel() * workspace.element_size()
+    if have < need:
+        raise HipQmmError(f"workspace too small: {have} < {need}")
+    if need and not (workspace.get_device() == device and workspace.is_contiguous()):
+        raise HipQmmError("workspace must be contiguous, on the GPU of the others")
+    return workspace.data_ptr(), have
 
 
 class PagedKV:
@@ -76,7 +89,7 @@ class PagedKV:
               "k and v must be f16 or bf16 [n_pages, n_kv_heads, page_size, head_dim], alike")
         _need(k.is_cuda and v.device == k.device, "tensors must live on the GPU")
         _need(k.stride(3) == 1 and k.stride() == v.stride(), "k and v must have the same strides, head_dim contiguous")
-        self.k, self.v = k, v
+        self.k, self.v, self._device = k, v, k.get_device()
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
         self._c = _KVCache(k.data_ptr(), v.data_ptr(), _KV_TYPES[k.dtype], self.n_kv_heads, self.page_size,
                            self.head_dim, self.n_pages, k.stride(0), k.stride(1), k.stride(2))
@@ -99,10 +112,10 @@ def rope_steps(n_dims: int, freq_base=10000.0, freq_scale=1.0, ext_factor=0.0, a
     return steps.to(device), mscale.value
 
 
-def _heads(t, name):
+def _heads(t, name, device):
     """Token and head stride of f32 [n_tokens, n_heads, head_dim]."""
-    if not (t.is_cuda and t.dtype is torch.float32 and t.dim() == 3):
-        raise HipQmmError(f"{name} must be f32 [n_tokens, n_heads, head_dim] on the GPU")
+    if not (t.is_cuda and t.get_device() == device and t.dtype is torch.float32 and t.dim() == 3):
+        raise HipQmmError(f"{name} must be f32 [n_tokens, n_heads, head_dim] on the GPU (of the others)")
     st, sh, sd = t.stride()
     if sd != 1:
         raise HipQmmError(f"{name}'s head_dim must be contiguous")
@@ -114,15 +127,15 @@ def _result(out, x):
     if out is None:
         n, h, d = x.shape
         return x.new_empty((n, h, d)), h * d, d
-    st, sh = _heads(out, "out")
+    st, sh = _heads(out, "out", x.get_device())
     _need(out.shape == x.shape, "out must have the shape of its input")
     return out, st, sh
 
 
-def _rotation(pos, steps, n, layout):
-    _int32(pos, n, "pos")
-    if not (steps.dtype is torch.int64 and steps.is_cuda and steps.dim() == 1 and steps.is_contiguous()):
-        raise HipQmmError("steps must be what rope_steps returns")
+def _rotation(pos, steps, n, layout, device):
+    _int32(pos, n, "pos", device)
+    if not (steps.dtype is torch.int64 and steps.get_device() == device and steps.dim() == 1 and steps.is_contiguous()):
+        raise HipQmmError("steps must be what rope_steps returns, on the GPU of the others")
     mode = ROPE_LAYOUTS.get(layout)
     if mode is None:
         raise HipQmmError(f"layout must be one of {sorted(ROPE_LAYOUTS)}")
@@ -132,12 +145,13 @@ def _rotation(pos, steps, n, layout):
 def rope(x: torch.Tensor, pos: torch.Tensor, steps: torch.Tensor, layout="half", mscale=1.0, out=None):
     """x f32 [n_tokens, n_heads, head_dim] with the first 2 * len(steps)
     elements of each head rotated by pos int32 [n_tokens]; out may be x."""
-    xt, xh = _heads(x, "x")
+    device = x.get_device()
+    xt, xh = _heads(x, "x", device)
     n, h, d = x.shape
-    mode, n_dims = _rotation(pos, steps, n, layout)
+    mode, n_dims = _rotation(pos, steps, n, layout, device)
     out, ot, oh = _result(out, x)
     _check(_lib().hip_qmm_rope_f32(x.data_ptr(), n, h, d, xt, xh, pos.data_ptr(), steps.data_ptr(), n_dims, mode, mscale,
-                                   out.data_ptr(), ot, oh, _raw_stream(x)), "hip_qmm_rope_f32")
+                                   out.data_ptr(), ot, oh, _raw_stream(device)), "hip_qmm_rope_f32")
     return out
 
 
@@ -146,18 +160,19 @@ def rope_kv_store(q, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, steps:
     """Rotates q and k f32 [n_tokens, heads, head_dim], stores the rotated k and
     the plain v at cache slots int32 [n_tokens] (page * page_size + token;
     outside the cache: not stored) and returns the rotated q.  q may be None."""
-    kt, kh = _heads(k, "k")
+    device = kv._device
+    kt, kh = _heads(k, "k", device)
     n, h, d = k.shape
-    if _heads(v, "v") != (kt, kh) or v.shape != k.shape:
+    if _heads(v, "v", device) != (kt, kh) or v.shape != k.shape:
         raise HipQmmError("k and v must have the same shape and strides")
     if h != kv.n_kv_heads or d != kv.head_dim:
         raise HipQmmError("k and v must have the cache's heads and head_dim")
-    mode, n_dims = _rotation(pos, steps, n, layout)
-    _int32(slots, n, "slots")
+    mode, n_dims = _rotation(pos, steps, n, layout, device)
+    _int32(slots, n, "slots", device)
     qp = op = None
     heads = qt = qh = ot = oh = 0
     if q is not None:
-        qt, qh = _heads(q, "q")
+        qt, qh = _heads(q, "q", device)
         nq, heads, dq = q.shape
         if nq != n or dq != d:
             raise HipQmmError("q and k disagree on the tokens or head_dim")
@@ -167,7 +182,7 @@ def rope_kv_store(q, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, steps:
         out = None
     _check(_lib().hip_qmm_rope_kv_store(qp, heads, qt, qh, k.data_ptr(), v.data_ptr(), kt, kh, n, pos.data_ptr(),
                                         steps.data_ptr(), n_dims, mode, mscale, op, ot, oh, kv._p, slots.data_ptr(),
-                                        _raw_stream(k)), "hip_qmm_rope_kv_store")
+                                        _raw_stream(device)), "hip_qmm_rope_kv_store")
     return out
 
 
@@ -185,9 +200,10 @@ def attn_paged_plan(kv: PagedKV, n_heads: int, n_seqs: int, n_tokens: int, max_q
     return rows, splits.value
 
 
-def _table(t):
-    if not (t.dtype is torch.int32 and t.is_cuda and t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]):
-        raise HipQmmError("page_table must be int32 [n_seqs, width] on the GPU, its rows contiguous and apart")
+def _table(t, device):
+    if not (t.dtype is torch.int32 and t.get_device() == device and t.dim() == 2 and t.stride(1) == 1
+            and t.stride(0) >= t.shape[1]):
+        raise HipQmmError("page_table must be int32 [n_seqs, width] on the GPU of the others, its rows contiguous and apart")
     return t.shape
 
 
@@ -200,20 +216,22 @@ def attn_paged(q: torch.Tensor, kv: PagedKV, page_table: torch.Tensor, kv_lens: 
     new tokens of a sequence.  A query at position p sees token j <= p if
     window is 0, p - j < window or j < sinks; entries outside the pool hide
     their tokens; nothing seen gives zeros.  max_kv: the longest length that
-    the host knows of.  scale: head_dim ** -0.5 by default."""
-    qt, qh = _heads(q, "q")
+    the host knows of.  scale: head_dim ** -0.5 by default.  out does not
+    overlap q."""
+    device = kv._device
+    qt, qh = _heads(q, "q", device)
     n, h, d = q.shape
     if d != kv.head_dim:
         raise HipQmmError("q must have the cache's head_dim")
-    n_seqs, width = _table(page_table)
-    _int32(kv_lens, n_seqs, "kv_lens")
+    n_seqs, width = _table(page_table, device)
+    _int32(kv_lens, n_seqs, "kv_lens", device)
     starts = None
     if q_starts is None:
         if n != n_seqs:
             raise HipQmmError("one token per sequence without q_starts")
         max_q = 1 if n else 0
     else:
-        _int32(q_starts, n_seqs + 1, "q_starts")
+        _int32(q_starts, n_seqs + 1, "q_starts", device)
         starts = q_starts.data_ptr()
         max_q = n if max_q is None else max_q
     if not page_table.is_contiguous():  # the row stride is the width that lengths are cut to
@@ -229,12 +247,10 @@ def attn_paged(q: torch.Tensor, kv: PagedKV, page_table: torch.Tensor, kv_lens: 
             workspace = q.new_empty(need, dtype=torch.uint8)
             wp = workspace.data_ptr()
     else:
-        have, wp = workspace.numel(), workspace.data_ptr()
-        if have < need:
-            raise HipQmmError(f"workspace too small: {have} < {need}")
+        wp, have = _scratch(workspace, need, device)
     _check(L.hip_qmm_attn_paged(kv._p, q.data_ptr(), h, qt, qh, starts, n_seqs, n, max_q, page_table.data_ptr(), width,
                                 kv_lens.data_ptr(), max_kv, d ** -0.5 if scale is None else scale, window, sinks,
-                                out.data_ptr(), ot, oh, wp, have, _raw_stream(q)), "hip_qmm_attn_paged")
+                                out.data_ptr(), ot, oh, wp, have, _raw_stream(device)), "hip_qmm_attn_paged")
     return out
 
 
@@ -242,12 +258,13 @@ def copy_pages(kv: PagedKV, src: torch.Tensor, dst: torch.Tensor, n_tokens=None)
     """Copies the first n_tokens[i] tokens (None: all) of page src[i] into page
     dst[i], keys and values: what a fork does with the partly filled last page."""
     n = src.numel()
-    _int32(src, n, "src")
-    _int32(dst, n, "dst")
+    device = kv._device
+    _int32(src, n, "src", device)
+    _int32(dst, n, "dst", device)
     if n_tokens is not None:
-        _int32(n_tokens, n, "n_tokens")
+        _int32(n_tokens, n, "n_tokens", device)
     _check(_lib().hip_qmm_kv_copy_pages(kv._p, src.data_ptr(), dst.data_ptr(),
-                                        None if n_tokens is None else n_tokens.data_ptr(), n, _raw_stream(kv.k)),
+                                        None if n_tokens is None else n_tokens.data_ptr(), n, _raw_stream(device)),
            "hip_qmm_kv_copy_pages")
 
 
@@ -256,19 +273,19 @@ def compact_pages(kv: PagedKV, page_table: torch.Tensor, kv_lens: torch.Tensor, 
     the pool: (the table with their new numbers and -1 elsewhere, int32; the
     count of pages in use, int32 [1]), both on the device.  out may be
     page_table."""
-    n_seqs, width = _table(page_table)
-    _int32(kv_lens, n_seqs, "kv_lens")
+    device = kv._device
+    n_seqs, width = _table(page_table, device)
+    _int32(kv_lens, n_seqs, "kv_lens", device)
     if out is None:
         out = page_table.new_empty((n_seqs, width))
-    _need(_table(out) == page_table.shape, "out must have page_table's shape")
+    _need(_table(out, device) == page_table.shape, "out must have page_table's shape")
     n_live = page_table.new_empty(1)
     L = _lib()
     need = L.hip_qmm_kv_compact_workspace_size(kv._p)
     if workspace is None:
         workspace = page_table.new_empty(max(need, 1), dtype=torch.uint8)
-    elif workspace.numel() < need:
-        raise HipQmmError(f"workspace too small: {workspace.numel()} < {need}")
+    wp, have = _scratch(workspace, need, device)
     _check(L.hip_qmm_kv_compact(kv._p, page_table.data_ptr(), page_table.stride(0), width, kv_lens.data_ptr(), n_seqs,
-                                out.data_ptr(), out.stride(0), n_live.data_ptr(), workspace.data_ptr(),
-                                workspace.numel(), _raw_stream(out)), "hip_qmm_kv_compact")
+                                out.data_ptr(), out.stride(0), n_live.data_ptr(), wp, have, _raw_stream(device)),
+           "hip_qmm_kv_compact")
     return out, n_live
