@@ -767,7 +767,7 @@ __global__ __launch_bounds__(64 * NW, RT * DP <= 128 ? 2 : 1) void few_kernel(At
         }
         return nan;
     };
-    if (!__syncthreads_or(pass(std::false_type{}))) return;
+    if (!__syncthreads_or(pass(std::false_type{}))) [[likely]] return;
     for (int i = threadIdx.x; i < O::WORDS; i += NW * 64) odd_bits[i] = 0;
     __syncthreads();
     pass(std::true_type{});
@@ -910,7 +910,7 @@ __global__ __launch_bounds__(256, 2) void many_kernel(AttnArgs a) {
     };
     pass(std::false_type{});
     const bool care = __syncthreads_or(w.any_nan());
-    if (care) {
+    if (care) [[unlikely]] {
         for (int i = threadIdx.x; i < O::WORDS; i += 256) odd_bits[i] = 0;
         __syncthreads();  // (which also frees both stages)
         if (begin < end) start();
