@@ -150,6 +150,8 @@ def rope(x: torch.Tensor, pos: torch.Tensor, steps: torch.Tensor, layout="half",
     n, h, d = x.shape
     mode, n_dims = _rotation(pos, steps, n, layout, device)
     out, ot, oh = _result(out, x)
+    if n * h == 0:  # empty tensors have no address
+        return out
     _check(_lib().hip_qmm_rope_f32(x.data_ptr(), n, h, d, xt, xh, pos.data_ptr(), steps.data_ptr(), n_dims, mode, mscale,
                                    out.data_ptr(), ot, oh, _raw_stream(device)), "hip_qmm_rope_f32")
     return out
@@ -180,6 +182,8 @@ def rope_kv_store(q, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, steps:
         qp, op = q.data_ptr(), out.data_ptr()
     else:
         out = None
+    if n == 0:
+        return out
     _check(_lib().hip_qmm_rope_kv_store(qp, heads, qt, qh, k.data_ptr(), v.data_ptr(), kt, kh, n, pos.data_ptr(),
                                         steps.data_ptr(), n_dims, mode, mscale, op, ot, oh, kv._p, slots.data_ptr(),
                                         _raw_stream(device)), "hip_qmm_rope_kv_store")

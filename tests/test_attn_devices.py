@@ -103,3 +103,23 @@ def test_the_current_gpu(monkeypatch):
     assert A._raw_stream(1) == 71
     with pytest.raises(G.HipQmmError):
         A._raw_stream(0)
+
+
+def test_calls_without_tokens(monkeypatch):
+    """Empty tensors have no address: nothing to do, as for the C entries with no tokens."""
+    monkeypatch.setattr(A, "_raw_stream", lambda *_: 0)
+    t = lambda *shape, dtype=torch.float32: On(torch.zeros(shape, dtype=dtype))  # noqa: E731
+    pos, steps, kv = t(0, dtype=torch.int32), t(32, dtype=torch.int64), _kv()
+    assert G.rope(t(0, 4, 64), pos, steps).shape == (0, 4, 64)
+    assert G.rope(t(3, 0, 64), t(3, dtype=torch.int32), steps).shape == (3, 0, 64)
+    out = t(0, 4, 64)
+    assert G.rope(t(0, 4, 64), pos, steps, out=out) is out
+    none = t(0, 2, 64)
+    assert G.rope_kv_store(t(0, 4, 64), none, none, pos, steps, kv, pos).shape == (0, 4, 64)
+    assert G.rope_kv_store(None, none, none, pos, steps, kv, pos) is None
+    G.copy_pages(kv, pos, pos)
+    assert G.attn_paged(t(0, 4, 64), kv, t(0, 2, dtype=torch.int32), pos).shape == (0, 4, 64)
+    with pytest.raises(G.HipQmmError):
+        G.rope(t(0, 4, 64), t(1, dtype=torch.int32), steps)
+    with pytest.raises(G.HipQmmError):
+        G.rope_kv_store(t(0, 4, 64), none, none, pos, steps, kv, pos, layout="other")
