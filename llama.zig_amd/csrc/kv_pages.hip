@@ -331,6 +331,7 @@ extern "C" int hip_qmm_kv_compact(const hip_qmm_kv_cache *cache, const int32_t *
     if (table_width > INT32_MAX || n_seqs > INT32_MAX || out_stride > ((int64_t)1 << 40) ||
         table_stride > ((int64_t)1 << 40) || (page_table == table_out && table_stride != out_stride))
         return (int)hipErrorInvalidValue;
+    if (table_width == 0) n_seqs = 0;  // nothing in use; the lengths, which may be absent then, are not read
     hipStream_t s = (hipStream_t)stream;
     // In one launch, unless a workgroup would read rows of the table that another has rewritten, or every one a
     // large table.

@@ -47,3 +47,26 @@ def test_planned_for_more_workgroups_than_a_launch_has():
                                 64 ** -0.5)
         _hold(got[s], want, top, 64)
         _hold(exact[s], want, top, 64)
+
+
+@pytest.mark.parametrize("pages", [40, 9000])
+def test_compaction_of_tables_without_entries(pages):
+    """No table, no lengths: no page is in use, in one launch and in two."""
+    import ctypes as C
+
+    import ggml_hip as G
+    from ggml_hip import attn as A
+    k = torch.randn((pages, 1, 16, 8), device="cuda").half()
+    kv, want = G.PagedKV(k, k.clone()), k.clone()
+    size = A._lib().hip_qmm_kv_compact_workspace_size(kv._p)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    live = torch.full((1,), 7, dtype=torch.int32, device="cuda")
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert A._lib().hip_qmm_kv_compact(kv._p, None, 0, 0, None, 5, None, 0, live.data_ptr(), ws.data_ptr(), size, stream) == 0
+    assert live.tolist() == [0]
+    table, n = G.compact_pages(kv, torch.zeros((5, 0), dtype=torch.int32, device="cuda"),
+                               torch.full((5,), 100, dtype=torch.int32, device="cuda"))
+    assert table.shape == (5, 0) and n.tolist() == [0]
+    table, n = G.compact_pages(kv, torch.zeros((0, 4), dtype=torch.int32, device="cuda"),
+                               torch.zeros(0, dtype=torch.int32, device="cuda"))
+    assert table.shape == (0, 4) and n.tolist() == [0] and torch.equal(kv.k, want)
