@@ -489,21 +489,22 @@ __device__ __forceinline__ void blank(const AttnArgs &a, const Span<TN> &sp, uin
 // are noted, in two bits each: inf and -inf, both for NaN and for a sum of the
 // two.  Of values it is a row's and a dimension's, added to the results; of
 // keys a row's and a token's, the query's element times the key's, added to the
-// tile's scores.
+// tile's scores; a NaN among a key's elements is the token's, whatever the row.
 template <int DP, int ROWS, int TN>
 struct Odd {
-    static constexpr int WORDS = ROWS * DP / 16, KEY_WORDS = ROWS * TN / 16;
-    uint32_t *bits, *key_bits;  // by row and dimension; by row and the tile's token
+    static constexpr int WORDS = ROWS * DP / 16, NAN_KEYS = ROWS * TN / 16, KEY_WORDS = NAN_KEYS + TN / 32;
+    uint32_t *bits, *key_bits;  // by row and dimension; by row and the tile's token, then a bit per token
 
     static __device__ __forceinline__ float number(uint32_t kind) {
         return kind == 1 ? INFINITY : kind == 2 ? -INFINITY : NAN;
     }
 
-    // What is not finite in the tile of t0 becomes 0; note(row, token, dimension, kind) for each row that sees it.  By
-    // threads first, first + step, ...; the block's rows begin at first_row of the sequence, whose first position is p0.
-    template <bool BF16, class Note>
+    // What is not finite in the tile of t0 becomes 0; note(row, token, dimension, kind) for each row that sees it, unless
+    // done(token, whether it is NaN).  By threads first, first + step, ...; the block's rows begin at first_row of the
+    // sequence, whose first position is p0.
+    template <bool BF16, class Done, class Note>
     static __device__ __forceinline__ void sift(const AttnArgs &a, uint8_t *tile, int t0, int ok, int first_row, int rows,
-                                                int first, int step, int p0, Note note) {
+                                                int first, int step, int p0, Done done, Note note) {
         constexpr uint32_t INF = El<BF16>::INF;
         for (int i = first; i < TN * (DP / 2); i += step) {
             uint32_t *w = reinterpret_cast<uint32_t *>(tile) + i;
@@ -513,6 +514,7 @@ struct Odd {
             *w = pair & (lo ? 0xffff0000u : ~0u) & (hi ? 0x0000ffffu : ~0u);
             const int t = i / (DP / 2), d = (((i & (DP / 2 - 1)) >> 2) ^ swizzle<DP>(t)) * 8 + (i & 3) * 2;
             if (!(ok >> (t >> 4) & 1) || d >= a.c.head_dim) continue;  // past the head: its last chunk again
+            if (done(t, (pair & 0x7fffu) > INF || (pair >> 16 & 0x7fffu) > INF)) continue;
             for (int r = 0; r < rows; ++r) {
                 const int p = p0 + (first_row + r) / a.group, j = t0 + t;
                 if (!(j <= p && (!a.window || p - j < a.window || j < a.sinks))) continue;
@@ -530,10 +532,15 @@ struct Odd {
     template <bool BF16>
     __device__ __forceinline__ void sift_keys(const AttnArgs &a, const Seq &q, int kvh, uint8_t *tile, int t0, int ok,
                                               int first_row, int rows, int first, int step) const {
-        sift<BF16>(a, tile, t0, ok, first_row, rows, first, step, q.n - q.m, [&](int r, int t, int d, uint32_t kind) {
+        auto done = [&](int t, bool nan) {
+            uint32_t *w = &key_bits[NAN_KEYS + (t >> 5)];
+            if (nan) atomicOr(w, 1u << (t & 31));
+            return nan || (*w >> (t & 31) & 1);
+        };
+        sift<BF16>(a, tile, t0, ok, first_row, rows, first, step, q.n - q.m, done, [&](int r, int t, int d, uint32_t kind) {
             const float x = query_row(a, q, kvh, first_row + r)[d];
             if (x == 0.0f || x != x || a.scale == 0.0f) kind = 3;
-            else if (kind != 3 && (x < 0.0f) != (a.scale < 0.0f)) kind ^= 3;
+            else if ((x < 0.0f) != (a.scale < 0.0f)) kind ^= 3;
             atomicOr(&key_bits[r * (TN / 16) + (t >> 4)], kind << (2 * (t & 15)));
         });
     }
@@ -541,7 +548,8 @@ struct Odd {
     template <bool BF16>
     __device__ __forceinline__ void sift_values(const AttnArgs &a, const Seq &q, uint8_t *tile, int t0, int ok,
                                                 int first_row, int rows, int first, int step) const {
-        sift<BF16>(a, tile, t0, ok, first_row, rows, first, step, q.n - q.m, [&](int r, int t, int d, uint32_t kind) {
+        auto done = [](int, bool) { return false; };
+        sift<BF16>(a, tile, t0, ok, first_row, rows, first, step, q.n - q.m, done, [&](int r, int t, int d, uint32_t kind) {
             if (key_bits[r * (TN / 16) + (t >> 4)] >> (2 * (t & 15)) & 3) kind = 3;
             atomicOr(&bits[r * (DP / 16) + (d >> 4)], kind << (2 * (d & 15)));
         });
@@ -556,9 +564,12 @@ struct Odd {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const uint32_t k = key_bits[(r0 + 16 * i + (lane & 15)) * (TN / 16) + (t >> 4) + j] >> (8 * (lane >> 4));
+                const uint32_t nan = key_bits[NAN_KEYS + (t >> 5)] >> (16 * j + 4 * (lane >> 4));
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
+                for (int e = 0; e < 4; ++e) {
                     if (k >> (2 * e) & 3) s[i][j][e] += number(k >> (2 * e) & 3);
+                    if (nan >> e & 1) s[i][j][e] = NAN;
+                }
             }
     }
     // Row r's dimension d, given its result without them.
