@@ -114,7 +114,7 @@ def rope_steps(n_dims: int, freq_base=10000.0, freq_scale=1.0, ext_factor=0.0, a
 
 def _heads(t, name, device):
     """Token and head stride of f32 [n_tokens, n_heads, head_dim]."""
-    if not (t.is_cuda and t.get_device() == device and t.dtype is torch.float32 and t.dim() == 3):
+    if not (t.get_device() == device >= 0 and t.dtype is torch.float32 and t.dim() == 3):
         raise HipQmmError(f"{name} must be f32 [n_tokens, n_heads, head_dim] on the GPU (of the others)")
     st, sh, sd = t.stride()
     if sd != 1:
