@@ -594,9 +594,9 @@ __device__ __forceinline__ float weight_of(float top, float m) {
 // with no barrier.  At the end the waves' results are joined in LDS.
 //
 // 32 query heads on 8 of 128 dimensions, f16: 131072 tokens (537 MB) 98 us, 5.5
-// TB/s (a large copy: 5.3); 16384 18.4; 4096 11.7; 333 8.7, where a launch is
-// 2.5.  100 sequences of a 1024-token window with 32 heads of 64 (819 MB): 151
-// us, 5.4 TB/s.  48 of up to 8191 in bf16 (447 MB): 98 us, 4.6 TB/s, with the
+// TB/s (a large copy: 5.3); 16384 18.6; 4096 11.8; 333 8.7, where a launch is
+// 2.5.  100 sequences of a 1024-token window with 32 heads of 64 (819 MB): 148
+// us, 5.5 TB/s.  48 of up to 8191 in bf16 (447 MB): 97 us, 4.6 TB/s, with the
 // join's 5 us.  Four waves with one stage leave room for two workgroups a CU:
 // two stages took 9.4, 11.8 and 108 us for 333 tokens, 4096 and the 48, eight
 // waves 8.0, 12.0 and 105.  With many short sequences NW is 1 (`plan_of`).
@@ -788,9 +788,9 @@ __global__ __launch_bounds__(64 * NW, RT * DP <= 128 ? 2 : 1) void few_kernel(At
 
 // 128 rows, 32 per wave, against tiles of 64 tokens that the four waves share:
 // bound by the matrix cores and the softmax beside them, whose times add up on
-// this part (a prompt of 4096 tokens, 32 heads on 8 of 128 in f16: 262 us, 525
-// TFLOP/s of the one product that counts, 1050 of the two that run; matrix
-// instructions are 44 % of the cycles, vector ones 31).  A row takes 5 to 6
+// this part (a prompt of 4096 tokens, 32 heads on 8 of 128 in f16: 258 us, 533
+// TFLOP/s of the one product that counts, 1066 of the two that run; matrix
+// instructions are 45 % of the cycles, vector ones 31).  A row takes 5 to 6
 // vector operations per score, of which the exponential counts for four, so
 // that 16 rows a wave, which would double the reads of LDS, or parts of P
 // passed through LDS gain nothing.
