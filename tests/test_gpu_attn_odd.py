@@ -58,6 +58,8 @@ def _definition(c, window=0, sinks=0, scale=None):
     scale = q.shape[2] ** -0.5 if scale is None else scale
     for s, n in enumerate(c["lens"].tolist()):
         lo, m = int(c["starts"][s]), c["new"][s]
+        if n == 0:
+            continue
         ks, ok = R.rows_of(c["k"], c["table"][s], n)
         vs, _ = R.rows_of(c["v"], c["table"][s], n)
         see = R.seen(m, n, ok, window, sinks)
@@ -155,3 +157,36 @@ def test_a_stored_key_over_the_types_range():
     c["v"][page, :, slot, 11] = 0.0
     c["q"][:, :, 11].abs_().neg_()
     assert bool(torch.isfinite(_check(c)).all())
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("form", FORMS)
+def test_infinite_values(form, dim, dtype):
+    """In the first, a middle and the last tile, alone and where an infinity of the other sign follows."""
+    _, _, seqs, new, n = form
+    c = _case(dtype, 8, 4, dim, page=32, lens=[n] * seqs, new=[new] * seqs)
+    clean, v, inf = _run(c, decode=False), c["v"], math.inf
+    for token, h, d, x in ((0, 0, 3, inf), (n // 2, 0, 5, -inf), (n - 1, 0, 7, inf), (1, 1, 3, inf), (n - 1, 1, 3, -inf),
+                           (n - 1 - new // 2, 2, dim - 1, math.nan), (n - 1 - new // 3, 2, dim - 2, inf)):
+        page, slot = _at(c, 0, token)
+        v[page, h, slot, d] = x
+    got = _check(c)
+    assert torch.equal(got[:, 6:], clean[:, 6:]) and torch.equal(got[new:], clean[new:])
+    _check(c, window=max(1, n // 3), sinks=2)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("most", [30, 380])
+def test_many_short_sequences(most, dim, dtype):
+    """A wave for each: keys and values that are not finite in some of them."""
+    lens = [most, 0, 1, most - 1] + [(37 * i) % most for i in range(13)]
+    c = _case(dtype, 64, 64, dim, page=16, lens=lens)
+    clean = _run(c)
+    for s, h, token, where, x in ((0, 1, most - 1, "k", math.inf), (0, 2, 0, "k", -math.inf), (0, 3, 0, "v", math.inf),
+                                  (2, 4, 0, "k", -math.inf), (2, 4, 0, "v", math.nan), (3, 5, most - 2, "k", math.nan)):
+        page, slot = _at(c, s, token)
+        c[where][page, h, slot, 6] = x
+    got = _check(c)
+    assert torch.equal(got[4:], clean[4:]) and torch.equal(got[:, 6:], clean[:, 6:])
