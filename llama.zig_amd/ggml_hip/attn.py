@@ -51,7 +51,10 @@ def _lib():
     return _bound
 
 
-# The checks build their messages only when they refuse: a step's call lasts a few microseconds.
+# The checks build their messages only when they refuse, and look up little: a step's call lasts a few microseconds.
+_C, _I32, _I64, _F32 = torch._C, torch.int32, torch.int64, torch.float32
+
+
 def _need(ok, what):
     if not ok:
         raise HipQmmError(what)
@@ -59,13 +62,13 @@ def _need(ok, what):
 
 def _raw_stream(device):
     # A launch goes to the current device, whatever its stream's.
-    if device != torch._C._cuda_getDevice():
+    if device != _C._cuda_getDevice():
         raise HipQmmError("tensors must live on the current GPU")
-    return torch._C._cuda_getCurrentRawStream(device)
+    return _C._cuda_getCurrentRawStream(device)
 
 
 def _int32(t, n, name, device):
-    if not (t.dtype is torch.int32 and t.get_device() == device and t.numel() == n and t.is_contiguous()):
+    if not (t.dtype is _I32 and t.get_device() == device and t.numel() == n and t.is_contiguous()):
         raise HipQmmError(f"{name} must be {n} contiguous int32 values on the GPU of the others")
 
 
@@ -114,7 +117,7 @@ def rope_steps(n_dims: int, freq_base=10000.0, freq_scale=1.0, ext_factor=0.0, a
 
 def _heads(t, name, device):
     """Token and head stride of f32 [n_tokens, n_heads, head_dim]."""
-    if not (t.get_device() == device >= 0 and t.dtype is torch.float32 and t.dim() == 3):
+    if not (t.get_device() == device >= 0 and t.dtype is _F32 and t.dim() == 3):
         raise HipQmmError(f"{name} must be f32 [n_tokens, n_heads, head_dim] on the GPU (of the others)")
     st, sh, sd = t.stride()
     if sd != 1:
@@ -134,7 +137,7 @@ def _result(out, x):
 
 def _rotation(pos, steps, n, layout, device):
     _int32(pos, n, "pos", device)
-    if not (steps.dtype is torch.int64 and steps.get_device() == device and steps.dim() == 1 and steps.is_contiguous()):
+    if not (steps.dtype is _I64 and steps.get_device() == device and steps.dim() == 1 and steps.is_contiguous()):
         raise HipQmmError("steps must be what rope_steps returns, on the GPU of the others")
     mode = ROPE_LAYOUTS.get(layout)
     if mode is None:
@@ -205,7 +208,7 @@ def attn_paged_plan(kv: PagedKV, n_heads: int, n_seqs: int, n_tokens: int, max_q
 
 
 def _table(t, device):
-    if not (t.dtype is torch.int32 and t.get_device() == device and t.dim() == 2 and t.stride(1) == 1
+    if not (t.dtype is _I32 and t.get_device() == device and t.dim() == 2 and t.stride(1) == 1
             and t.stride(0) >= t.shape[1]):
         raise HipQmmError("page_table must be int32 [n_seqs, width] on the GPU of the others, its rows contiguous and apart")
     return t.shape
