@@ -553,3 +553,4 @@ def mul_mat_id_glu(qtype, w: torch.Tensor, w_gate: torch.Tensor, x: torch.Tensor
 
 from .attn import (PagedKV, attn_paged, attn_paged_plan, attn_paged_workspace_size, compact_pages,  # noqa: E402,F401
                    copy_pages, rope, rope_kv_store, rope_steps)
+from .moe import combine, mul_mat_i8, mul_mat_id_i8, quantize_i8, route  # noqa: E402,F401
