@@ -55,8 +55,9 @@ int hip_qmm_moe_route(const float *logits, int64_t n_tokens, int64_t n_experts, 
                       int64_t weights_stride, void *stream);
 
 /*
- * Rows to 8-bit integers: scale[r] = max|x[r]| / 127 and q[r] = x[r] / scale[r]
- * to the nearest, half to even, cut to +-127; divisions are IEEE f32 ones.  A row
+ * Rows to 8-bit integers: scale[r] = max|x[r]| * (1/127) and q[r] = x[r] / scale[r]
+ * to the nearest, half to even, cut to +-127: one f32 product with the f32 next
+ * to 1/127, and IEEE f32 divisions.  A row
  * whose scale rounds to 0 has zeros, and one with a value that is not finite
  * zeros and a scale of NaN.  Only the K values of a row are written.  K at most
  * 131071, n_rows at most 2^24.
@@ -66,13 +67,14 @@ int hip_qmm_quantize_i8(const float *x, int64_t K, int64_t n_rows, int64_t x_str
 
 /*
  * dst[n][m] = (sum_k w[m][k] * x[n][k]) * x_scale[n] * w_scale[m], the sum in
- * 32-bit integers (exact), the result rounded to f32 once.  With x_scale
+ * 32-bit integers (exact), then three f32 roundings (the sum's and the two
+ * products'; only the result's range matters, not a product's).  With x_scale
  * NULL x is f32 and quantized in the call as hip_qmm_quantize_i8 does.
  *
  * w is int8, 16-byte aligned with a row stride that is a multiple of 16, and so
  * is an int8 x; the bytes from K to the next multiple of 16 of each of their
  * rows must be readable but do not matter.  K at most 131071, nrows and ncols at
- * most 2^22.  The workspace is scratch, 256-byte aligned: its contents do
+ * most 2^22, their product at most 2^38.  The workspace is scratch, 256-byte aligned: its contents do
  * not matter before the call, and it serves one call at a time.
  */
 size_t hip_qmm_mul_mat_i8_workspace_size(int64_t K, int64_t nrows, int64_t ncols, int quantized);
@@ -86,7 +88,7 @@ int hip_qmm_mul_mat_i8(const int8_t *w, const float *w_scale, int64_t K, int64_t
  * w + e*expert_stride, scales at w_scale + e*nrows) with row t*ne11 + s % ne11 of x
  * (ne11 1 or n_ids; x_stride between rows, x_scale one a row or NULL as above).
  * An id outside [0, n_as) leaves a zero row.  n_as at most 1024, n_tokens*n_ids
- * at most 2^22, expert_stride a multiple of 16; otherwise the limits of
+ * at most 2^22, times nrows at most 2^38; expert_stride a multiple of 16; otherwise the limits of
  * hip_qmm_mul_mat_i8.
  */
 size_t hip_qmm_mul_mat_id_i8_workspace_size(int64_t K, int64_t nrows, int64_t n_as, int64_t ne11, int64_t n_tokens,

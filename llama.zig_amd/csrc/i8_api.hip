@@ -1,5 +1,7 @@
 // i8_api.hip -- the entry points of the 8-bit products: their checks, their
 // workspaces, and which kernel runs.
+#include <algorithm>
+
 #include "i8.h"
 
 using namespace i8;
@@ -25,26 +27,28 @@ Tokens tokens_at(size_t at, int64_t K, int64_t n) {
     return t;
 }
 
-// A tile's columns.
-int columns(int64_t n) { return n <= 16 ? 16 : n <= 32 ? 32 : 64; }
-
 struct Grouped {
-    size_t src, dst, tiles, n_tiles, end;
-    int bn;
+    size_t src, dst, tiles, n_tiles, counts, places, end;
+    TileForm form;
     int64_t max_tiles;
 };
 
 Grouped grouped_at(size_t at, int64_t n_as, int64_t pairs) {
     Grouped g;
-    g.bn = columns((pairs + n_as - 1) / n_as);
-    g.max_tiles = pairs / g.bn + (pairs < n_as ? pairs : n_as);
+    g.form = tile_form_grouped(n_as, pairs);
+    g.max_tiles = pairs / tile_columns(g.form) + std::min(pairs, n_as);
     g.src = at;
     g.dst = a256(g.src + (size_t)pairs * 4);
     g.tiles = a256(g.dst + (size_t)pairs * 4);
     g.n_tiles = a256(g.tiles + (size_t)g.max_tiles * 16);
-    g.end = a256(g.n_tiles + 4);
+    g.counts = a256(g.n_tiles + 4);
+    g.places = a256(g.counts + (size_t)((pairs + PAIR_CHUNK - 1) / PAIR_CHUNK * n_as) * 4);
+    g.end = a256(g.places + (size_t)pairs * 2);
     return g;
 }
+
+// Whole aligned float4, as the kernels for few columns read f32 columns.
+bool float4s(const void *x, int64_t K, int64_t stride) { return !(K % 4 || stride % 4 || (uintptr_t)x % 16); }
 
 bool operand_ok(const void *p, int64_t stride, int64_t K, bool bytes) {
     if (!p || stride < K || stride > MAX_STRIDE) return false;
@@ -53,6 +57,16 @@ bool operand_ok(const void *p, int64_t stride, int64_t K, bool bytes) {
 
 bool workspace_ok(const void *ws, size_t have, size_t need) {
     return need == 0 || (ws && !((uintptr_t)ws % 256) && have >= need);
+}
+
+// p's f32 columns to 8-bit ones in the workspace.
+int quantize_tokens(Product &p, const Tokens &t, int64_t n, void *workspace, hipStream_t s) {
+    uint8_t *ws = (uint8_t *)workspace;
+    int8_t *q = (int8_t *)(ws + t.q);
+    float *scale = (float *)(ws + t.scale);
+    const int e = quantize((const float *)p.x, p.K, n, p.x_stride, q, token_stride(p.K), scale, s);
+    p.x = q, p.x_scale = scale, p.x_stride = token_stride(p.K);
+    return e;
 }
 
 }  // namespace
@@ -67,6 +81,7 @@ extern "C" int hip_qmm_mul_mat_i8(const int8_t *w, const float *w_scale, int64_t
                                   int64_t dst_stride, void *workspace, size_t workspace_size, void *stream) {
     if (!sizes_ok(K, nrows) || ncols < 0 || ncols > MAX_ROWS) return (int)hipErrorInvalidValue;
     if (ncols == 0) return 0;
+    if (nrows > MAX_RESULTS / ncols) return (int)hipErrorInvalidValue;
     if (!w_scale || !dst || dst_stride < nrows || dst_stride > MAX_STRIDE || !operand_ok(w, w_stride, K, true) ||
         !operand_ok(x, x_stride, K, x_scale != nullptr) ||
         !workspace_ok(workspace, workspace_size, hip_qmm_mul_mat_i8_workspace_size(K, nrows, ncols, x_scale != nullptr)))
@@ -78,15 +93,18 @@ extern "C" int hip_qmm_mul_mat_i8(const int8_t *w, const float *w_scale, int64_t
     p.K = (int)K, p.nrows = (int)nrows, p.ncols = (int)ncols;
     p.x = (const int8_t *)x, p.x_scale = x_scale, p.x_stride = x_stride;
     if (!x_scale) {
-        uint8_t *ws = (uint8_t *)workspace;
-        const Tokens t = tokens_at(0, K, ncols);
-        const int64_t stride = token_stride(K);
-        if (int e = quantize((const float *)x, K, ncols, x_stride, (int8_t *)(ws + t.q), stride, (float *)(ws + t.scale), s))
-            return e;
-        p.x = (const int8_t *)(ws + t.q), p.x_scale = (const float *)(ws + t.scale), p.x_stride = stride;
+        if (float4s(x, K, x_stride)) {
+            const FewPlan plan = few_plan(true, K, nrows, ncols);
+            if (plan.bytes) return few_product(p, plan, s);
+        }
+        if (int e = quantize_tokens(p, tokens_at(0, K, ncols), ncols, workspace, s)) return e;
     }
-    const int bn = columns(ncols);
-    return stream_product(p, (ncols + bn - 1) / bn, bn, s);
+    const FewPlan plan = few_plan(false, K, nrows, ncols);
+    // Many rows and over 16 columns: tiles, whose workgroups share the columns (14336 x 4096 by 32: 15 us, 19 us).
+    if (plan.bytes && (ncols <= 16 || plan.mode == RESIDENT || nrows < 8192)) return few_product(p, plan, s);
+    const TileForm form = tile_form(nrows, ncols);
+    const int bn = tile_columns(form);
+    return tile_product(p, form, (ncols + bn - 1) / bn, s);
 }
 
 extern "C" size_t hip_qmm_mul_mat_id_i8_workspace_size(int64_t K, int64_t nrows, int64_t n_as, int64_t ne11,
@@ -106,6 +124,7 @@ extern "C" int hip_qmm_mul_mat_id_i8(const int8_t *w, const float *w_scale, int6
         n_tokens > MAX_ROWS || (n_ids > 0 && n_tokens > MAX_ROWS / n_ids) || (ne11 != 1 && ne11 != n_ids))
         return (int)hipErrorInvalidValue;
     if (n_tokens == 0 || n_ids == 0) return 0;
+    if (nrows > MAX_RESULTS / (n_tokens * n_ids)) return (int)hipErrorInvalidValue;
     const bool quantized = x_scale != nullptr;
     if (!w_scale || !dst || !ids || ids_stride < n_ids || ids_stride > MAX_STRIDE || dst_stride < nrows ||
         dst_stride > MAX_STRIDE || !operand_ok(w, w_stride, K, true) || expert_stride % 16 ||
@@ -123,17 +142,21 @@ extern "C" int hip_qmm_mul_mat_id_i8(const int8_t *w, const float *w_scale, int6
     p.dst = dst, p.dst_stride = dst_stride;
     p.K = (int)K, p.nrows = (int)nrows;
     p.x = (const int8_t *)x, p.x_scale = x_scale, p.x_stride = x_stride;
+    const int pairs = (int)(n_tokens * n_ids);
     if (!quantized) {
-        const int64_t stride = token_stride(K);
-        if (int e = quantize((const float *)x, K, n_tokens * ne11, x_stride, (int8_t *)(ws + t.q), stride,
-                             (float *)(ws + t.scale), s))
-            return e;
-        p.x = (const int8_t *)(ws + t.q), p.x_scale = (const float *)(ws + t.scale), p.x_stride = stride;
+        if (float4s(x, K, x_stride)) {
+            const FewPlan plan = few_pairs_plan(true, K, nrows, n_as, n_tokens, n_ids);
+            if (plan.bytes) return few_pairs(p, plan, ids, ids_stride, pairs, (int)n_ids, (int)n_as, ne11 > 1, s);
+        }
+        if (int e = quantize_tokens(p, t, n_tokens * ne11, workspace, s)) return e;
     }
-    int32_t *src = (int32_t *)(ws + g.src), *to = (int32_t *)(ws + g.dst);
-    int32_t *tiles = (int32_t *)(ws + g.tiles), *n_tiles = (int32_t *)(ws + g.n_tiles);
-    if (int e = group(ids, ids_stride, n_tokens, n_ids, n_as, ne11, g.bn, src, to, tiles, n_tiles, dst, dst_stride, nrows, s))
+    const FewPlan plan = few_pairs_plan(false, K, nrows, n_as, n_tokens, n_ids);
+    if (plan.bytes) return few_pairs(p, plan, ids, ids_stride, pairs, (int)n_ids, (int)n_as, ne11 > 1, s);
+    const Groups to = {(int32_t *)(ws + g.src), (int32_t *)(ws + g.dst), (int32_t *)(ws + g.tiles),
+                       (int32_t *)(ws + g.n_tiles), (int32_t *)(ws + g.counts), (uint16_t *)(ws + g.places)};
+    if (int e = group(ids, ids_stride, pairs, (int)n_ids, (int)n_as, ne11 > 1, tile_columns(g.form), to, dst, dst_stride,
+                      nrows, s))
         return e;
-    p.tiles = tiles, p.n_tiles = n_tiles, p.col_src = src, p.col_dst = to;
-    return stream_product(p, g.max_tiles, g.bn, s);
+    p.tiles = to.tiles, p.n_tiles = to.n_tiles, p.col_src = to.col_src, p.col_dst = to.col_dst;
+    return tile_product(p, g.form, g.max_tiles, s);
 }

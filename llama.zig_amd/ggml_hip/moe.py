@@ -121,7 +121,7 @@ def route(logits: torch.Tensor, k: int, gating="softmax", bias=None, groups=1, k
 
 def quantize_i8(x: torch.Tensor, out=None, scale=None):
     """f32 [.., K] to 8-bit rows: (int8 [.., K], scale f32 [..]) with x near
-    q * scale, scale = max|x| / 127 of each row; of tokens, or of weights with a
+    q * scale, scale = max|x| * (1/127) of each row; of tokens, or of weights with a
     row per channel.  The result's rows are 16-byte aligned."""
     device, K = x.get_device(), x.shape[-1] if x.dim() else 0
     if device < 0 or x.dtype is not _F32 or x.dim() < 2:

@@ -55,11 +55,11 @@ def route(logits, k, gating="softmax", bias=None, groups=1, keep=1, top=2, renor
 
 
 def quantize(x):
-    """(q int8, scale f32) of f32 rows, by the f32 divisions of the definition."""
+    """(q int8, scale f32) of f32 rows, by the f32 product and divisions of the definition."""
     x = np.asarray(x, np.float32)
     with np.errstate(all="ignore"):
         most = np.abs(x).max(-1) if x.shape[-1] else np.zeros(x.shape[:-1], np.float32)
-        d = (most / np.float32(127)).astype(np.float32)
+        d = (most * (np.float32(1) / np.float32(127))).astype(np.float32)
         fine = np.isfinite(most)
         q = np.where((fine & (d > 0))[..., None], np.clip(np.rint(x / d[..., None]), -127, 127), 0)
     return np.nan_to_num(q).astype(np.int8), np.where(fine, d, np.float32(np.nan)).astype(np.float32)
