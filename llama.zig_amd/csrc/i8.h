@@ -128,7 +128,7 @@ int few_pairs(const Product &p, const FewPlan &plan, const int32_t *ids, int64_t
               int per_slot, hipStream_t s);
 
 // i8_tile.hip: tiles of TM weight rows and TN columns.
-enum TileForm { TILE_64x64, TILE_128x64, TILE_128x128, TILE_256x128, TILE_256x256 };
+enum TileForm { TILE_64x64, TILE_128x64, TILE_128x128, TILE_128x128_DEEP, TILE_256x256 };
 TileForm tile_form(int64_t nrows, int64_t ncols);                   // dense
 TileForm tile_form_grouped(int64_t n_as, int64_t n_pairs);         // by experts
 int tile_columns(TileForm form);

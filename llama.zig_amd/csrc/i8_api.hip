@@ -47,9 +47,6 @@ Grouped grouped_at(size_t at, int64_t n_as, int64_t pairs) {
     return g;
 }
 
-// Whole aligned float4, as the kernels for few columns read f32 columns.
-bool float4s(const void *x, int64_t K, int64_t stride) { return !(K % 4 || stride % 4 || (uintptr_t)x % 16); }
-
 bool operand_ok(const void *p, int64_t stride, int64_t K, bool bytes) {
     if (!p || stride < K || stride > MAX_STRIDE) return false;
     return bytes ? !((uintptr_t)p % 16 || stride % 16) : !((uintptr_t)p % 4);
@@ -72,7 +69,7 @@ int quantize_tokens(Product &p, const Tokens &t, int64_t n, void *workspace, hip
 }  // namespace
 
 extern "C" size_t hip_qmm_mul_mat_i8_workspace_size(int64_t K, int64_t nrows, int64_t ncols, int quantized) {
-    if (!sizes_ok(K, nrows) || ncols < 1 || ncols > MAX_ROWS || quantized) return 0;
+    if (!sizes_ok(K, nrows) || ncols < 1 || ncols > MAX_ROWS || quantized || few_plan(true, K, nrows, ncols).bytes) return 0;
     return tokens_at(0, K, ncols).end;
 }
 
@@ -93,10 +90,8 @@ extern "C" int hip_qmm_mul_mat_i8(const int8_t *w, const float *w_scale, int64_t
     p.K = (int)K, p.nrows = (int)nrows, p.ncols = (int)ncols;
     p.x = (const int8_t *)x, p.x_scale = x_scale, p.x_stride = x_stride;
     if (!x_scale) {
-        if (float4s(x, K, x_stride)) {
-            const FewPlan plan = few_plan(true, K, nrows, ncols);
-            if (plan.bytes) return few_product(p, plan, s);
-        }
+        const FewPlan plan = few_plan(true, K, nrows, ncols);
+        if (plan.bytes) return few_product(p, plan, s);
         if (int e = quantize_tokens(p, tokens_at(0, K, ncols), ncols, workspace, s)) return e;
     }
     const FewPlan plan = few_plan(false, K, nrows, ncols);
@@ -112,6 +107,9 @@ extern "C" size_t hip_qmm_mul_mat_id_i8_workspace_size(int64_t K, int64_t nrows,
     if (!sizes_ok(K, nrows) || n_as < 1 || n_as > MAX_EXPERTS || n_tokens < 1 || n_ids < 1 || n_ids > MAX_ROWS ||
         n_tokens > MAX_ROWS / n_ids || (ne11 != 1 && ne11 != n_ids))
         return 0;
+    const bool few = few_pairs_plan(false, K, nrows, n_as, n_tokens, n_ids).bytes != 0;  // no tables
+    if (!quantized && few_pairs_plan(true, K, nrows, n_as, n_tokens, n_ids).bytes) return 0;
+    if (few) return quantized ? 0 : tokens_at(0, K, n_tokens * ne11).end;
     return grouped_at(quantized ? 0 : tokens_at(0, K, n_tokens * ne11).end, n_as, n_tokens * n_ids).end;
 }
 
@@ -144,10 +142,8 @@ extern "C" int hip_qmm_mul_mat_id_i8(const int8_t *w, const float *w_scale, int6
     p.x = (const int8_t *)x, p.x_scale = x_scale, p.x_stride = x_stride;
     const int pairs = (int)(n_tokens * n_ids);
     if (!quantized) {
-        if (float4s(x, K, x_stride)) {
-            const FewPlan plan = few_pairs_plan(true, K, nrows, n_as, n_tokens, n_ids);
-            if (plan.bytes) return few_pairs(p, plan, ids, ids_stride, pairs, (int)n_ids, (int)n_as, ne11 > 1, s);
-        }
+        const FewPlan plan = few_pairs_plan(true, K, nrows, n_as, n_tokens, n_ids);
+        if (plan.bytes) return few_pairs(p, plan, ids, ids_stride, pairs, (int)n_ids, (int)n_as, ne11 > 1, s);
         if (int e = quantize_tokens(p, t, n_tokens * ne11, workspace, s)) return e;
     }
     const FewPlan plan = few_pairs_plan(false, K, nrows, n_as, n_tokens, n_ids);

@@ -59,6 +59,7 @@ struct Few {
     int x_bytes;            // of a column in LDS
     int columns;            // in LDS at once, at most 16 NT
     int staged;             // QUANTIZE: columns whose f32 values fit in LDS at once
+    bool float4s;           // QUANTIZE: rows of whole aligned float4
 };
 
 // Chunk c of row r of 128 bytes sits at c ^ swizzle(r): the 16 rows that read one chunk column meet all banks.
@@ -206,10 +207,19 @@ __global__ __launch_bounds__(THREADS) void few_kernel(Few f) {
         if constexpr (MODE == QUANTIZE) {
             uint8_t *stage = x_lds + f.columns * f.x_bytes;
             // Waves that share a column.
+            const int units = (a.K + 3) / 4;  // float4
             const int share = n == 1 ? 8 : n == 2 ? 4 : n <= 4 ? 2 : 1, team = wave / share;
             for (int c0 = 0; c0 < n; c0 += f.staged) {
                 const int count = min(f.staged, n - c0);
-                bring_columns((const uint8_t *)a.x, a.x_stride * 4, c0, count, a.K * 4, stage, a.K * 4);
+                if (f.float4s) {
+                    bring_columns((const uint8_t *)a.x, a.x_stride * 4, c0, count, a.K * 4, stage, units * 16);
+                } else {
+                    for (int i = wave; i < count; i += WAVES) {
+                        const float *row = (const float *)a.x + src[c0 + i] * a.x_stride;
+                        for (int k = lane; k < units * 4; k += 64)
+                            reinterpret_cast<float *>(stage)[i * units * 4 + k] = k < a.K ? row[k] : 0.0f;
+                    }
+                }
                 if (c0 == 0) {
                     bring_first();
                     wait_for<2 * PER * DEPTH>();
@@ -219,10 +229,10 @@ __global__ __launch_bounds__(THREADS) void few_kernel(Few f) {
                 __syncthreads();
                 for (int base = 0; base < count; base += WAVES / share) {
                     const int c = base + team;
-                    const float4 *row = reinterpret_cast<const float4 *>(stage + (int64_t)min(c, count - 1) * a.K * 4);
+                    const float4 *row = reinterpret_cast<const float4 *>(stage + min(c, count - 1) * units * 16);
                     const int begin = tid - team * share * 64, hop = share * 64;
                     uint32_t m = 0;
-                    for (int k = begin; k < a.K / 4; k += hop) {
+                    for (int k = begin; k < units; k += hop) {
                         const float4 v = row[k];
                         m = max(m, max(max(magnitude(v.x), magnitude(v.y)), max(magnitude(v.z), magnitude(v.w))));
                     }
@@ -236,7 +246,7 @@ __global__ __launch_bounds__(THREADS) void few_kernel(Few f) {
                     }
                     const Scale scale(m);
                     if (c < count) {
-                        for (int k = begin; k < a.K / 4; k += hop)
+                        for (int k = begin; k < units; k += hop)
                             *reinterpret_cast<uint32_t *>(x_lds + (c0 + c) * f.x_bytes + k * 4) = scale.four(row[k]);
                         if (begin == 0) x_scale[c0 + c] = scale.value;
                     }
@@ -330,9 +340,9 @@ bool fits(FewPlan &p, int64_t K, int most) {
     int64_t bytes = fixed_bytes(p.nt, p.depth, p.mode == THROUGH, p.rows);
     if (p.mode != THROUGH) bytes += (int64_t)p.columns * column_bytes(K);
     if (p.mode == QUANTIZE) {
-        p.staged = (int)std::min((int64_t)p.columns, std::max((int64_t)0, most - bytes) / (K * 4));
+        p.staged = (int)std::min((int64_t)p.columns, std::max((int64_t)0, most - bytes) / ((K + 3) / 4 * 16));
         if (p.staged < 1) return false;
-        bytes += p.staged * K * 4;
+        bytes += p.staged * ((K + 3) / 4 * 16);
     }
     if (bytes > most) return false;
     p.bytes = (int)bytes;
@@ -341,6 +351,7 @@ bool fits(FewPlan &p, int64_t K, int most) {
 
 Few arguments(const Product &p, const FewPlan &plan) {
     Few f = {};
+    f.float4s = !(p.K % 4 || p.x_stride % 4 || (uintptr_t)p.x % 16);
     f.p = p, f.rows = plan.rows, f.x_bytes = column_bytes(p.K), f.columns = plan.columns, f.staged = plan.staged;
     return f;
 }

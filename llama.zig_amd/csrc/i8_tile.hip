@@ -104,7 +104,7 @@ __device__ __forceinline__ void tile(const Product &a, uint8_t *ring, const int8
 #pragma unroll
             for (int i = 0; i < L; ++i)
                 if (i >= lo && i < hi) {
-                    const int chunk = (lane & 7) ^ swizzle(8 * ((i < LM ? i : i - LM) & 1) + (lane >> 3));
+                    const int chunk = (lane & 7) ^ swizzle(8 * (i < LM ? wave * LM + i : wave * LN + i - LM) + (lane >> 3));
                     from[i] -= max(chunk - last, 0) * 16;
                 }
         }
@@ -239,8 +239,8 @@ __device__ __forceinline__ void tile(const Product &a, uint8_t *ring, const int8
     v4i *turn = reinterpret_cast<v4i *>(ring) + wave * 32 * CHUNKS;
     const int mine = lane % CHUNKS * 4, m = m0 + wm * (TM / 2) + mine, left = a.nrows - m;
     const float4 ws = *reinterpret_cast<const float4 *>(scales + wm * (TM / 2) + mine);
-    const bool whole_tile = first + TN <= end && m0 + TM <= a.nrows &&
-                            !(((uintptr_t)a.dst | (uintptr_t)(a.dst_stride * 4)) & 15);
+    const bool whole_tile = first + TN <= end && m0 + TM <= a.nrows;
+    typedef float v4f __attribute__((ext_vector_type(4), aligned(4)));  // a store of 16 bytes need not be aligned
     float *const out = a.dst + m;
 #pragma clang loop unroll(disable)
     for (int j = 0; j < RN; ++j) {
@@ -270,19 +270,24 @@ __device__ __forceinline__ void tile(const Product &a, uint8_t *ring, const int8
             if (plain && whole_tile) {
 #pragma unroll
                 for (int u = 0; u < AT_ONCE; ++u)
-                    *reinterpret_cast<float4 *>(out + (int64_t)row[u] * a.dst_stride) =
-                        make_float4((float)s[u][0] * xs[u] * ws.x, (float)s[u][1] * xs[u] * ws.y,
-                                    (float)s[u][2] * xs[u] * ws.z, (float)s[u][3] * xs[u] * ws.w);
+                    *reinterpret_cast<v4f *>(out + (int64_t)row[u] * a.dst_stride) =
+                        (v4f){(float)s[u][0] * xs[u] * ws.x, (float)s[u][1] * xs[u] * ws.y, (float)s[u][2] * xs[u] * ws.z,
+                              (float)s[u][3] * xs[u] * ws.w};
             } else {
 #pragma unroll
-                for (int u = 0; u < AT_ONCE; ++u)
-                    if (first + c0 + k + u * COLS + lane / CHUNKS < end) {
-                        float *o = out + (int64_t)row[u] * a.dst_stride;
-                        if (left > 0) o[0] = scaled(s[u][0], xs[u], ws.x);
-                        if (left > 1) o[1] = scaled(s[u][1], xs[u], ws.y);
-                        if (left > 2) o[2] = scaled(s[u][2], xs[u], ws.z);
-                        if (left > 3) o[3] = scaled(s[u][3], xs[u], ws.w);
+                for (int u = 0; u < AT_ONCE; ++u) {
+                    if (first + c0 + k + u * COLS + lane / CHUNKS >= end) continue;
+                    float *o = out + (int64_t)row[u] * a.dst_stride;
+                    const v4f v = {scaled(s[u][0], xs[u], ws.x), scaled(s[u][1], xs[u], ws.y), scaled(s[u][2], xs[u], ws.z),
+                                   scaled(s[u][3], xs[u], ws.w)};
+                    if (left >= 4) {
+                        *reinterpret_cast<v4f *>(o) = v;
+                    } else {
+                        if (left > 0) o[0] = v[0];
+                        if (left > 1) o[1] = v[1];
+                        if (left > 2) o[2] = v[2];
                     }
+                }
             }
         }
     }
@@ -365,25 +370,30 @@ int launch(const Product &p, int64_t max_tiles, hipStream_t s) {
 }  // namespace
 
 // The largest tile of which there are enough: by the time of a stage and of a tile's start and end, a large one on some
-// CUs beats small ones on all of them early (14336 x 4096 by 512 columns: 112 of 256 x 256 39.2 us, 448 of 128 x 128 43.6;
-// 2048 x 2048 by 2000: 64 of 256 x 256 24.2, 256 of 128 x 128 18.9, 512 of 128 x 64 17.1; 5003 x 2720 by 333: 240 of 128 x 64
-// 16.5, 474 of 64 x 64 18.6).
+// CUs beats small ones on all of them early.  Measured, us:
+//   14336 x 4096 by 512: 112 of 256 x 256 39, 448 of 128 x 128 42, two a CU; by 128: 224 of 128 x 64 22.9, 448 of 64 x 64 23.5
+//   4096 x 4096 by 1536: 96 of 256 x 256 36.9, 384 of 128 x 128 35.3; by 1024: 64 of 256 x 256 34.8, 256 of 128 x 128 23.9
+//     with four stages, one a CU, 29.1 with two; by 512: 128 of 128 x 128 19.6, 256 of 128 x 64 19.1; by 256: 128 of
+//     128 x 64 17.0, 256 of 64 x 64 12.6
+//   5003 x 2720 by 333: 120 of 128 x 128 16.8, 240 of 128 x 64 14.8, 474 of 64 x 64 16.5
 TileForm i8::tile_form(int64_t nrows, int64_t ncols) {
     auto tiles = [&](int64_t m, int64_t n) { return ((nrows + m - 1) / m) * ((ncols + n - 1) / n); };
     if (tiles(256, 256) >= 100) return TILE_256x256;
-    if (tiles(128, 128) >= 320) return TILE_128x128;
+    if (tiles(128, 128) > 256) return TILE_128x128;
+    if (tiles(128, 128) >= 140) return TILE_128x128_DEEP;
     if (tiles(128, 64) >= 200) return TILE_128x64;
     return TILE_64x64;
 }
 
-// By the mean number of an expert's columns (1536 x 2048, 128 experts: 32 columns 94.5 us in 128 x 64, 100 in 128 x 128;
-// 256 columns 214 in 256 x 128, 228 in 128 x 128, 218 in 256 x 256).
+// By the mean number of an expert's columns.  Measured with 128 experts of 1536 x 2048, us: 16 columns 81 in 128 x 64, 87 in
+// 64 x 64; 64 108 in 128 x 64, 118 in 128 x 128; 128 140 in 256 x 256 (its half tiles), 144 in 128 x 64; 256 212 in
+// 256 x 256, 228 in 128 x 128.
 TileForm i8::tile_form_grouped(int64_t n_as, int64_t n_pairs) {
-    return n_pairs <= 64 * n_as ? TILE_128x64 : TILE_256x128;
+    return n_pairs <= 64 * n_as ? TILE_128x64 : TILE_256x256;
 }
 
 int i8::tile_columns(TileForm form) {
-    return form == TILE_256x256 ? 256 : form == TILE_256x128 || form == TILE_128x128 ? 128 : 64;
+    return form == TILE_256x256 ? 256 : form == TILE_128x128 || form == TILE_128x128_DEEP ? 128 : 64;
 }
 
 int i8::tile_product(const Product &p, TileForm form, int64_t max_tiles, hipStream_t s) {
@@ -391,7 +401,7 @@ int i8::tile_product(const Product &p, TileForm form, int64_t max_tiles, hipStre
     case TILE_64x64: return launch<64, 64, 4, 4, 4>(p, max_tiles, s);
     case TILE_128x64: return launch<128, 64, 3, 3, 2>(p, max_tiles, s);
     case TILE_128x128: return launch<128, 128, 2, 2, 1>(p, max_tiles, s);
-    case TILE_256x128: return launch<256, 128, 3, 3, 1>(p, max_tiles, s);
+    case TILE_128x128_DEEP: return launch<128, 128, 4, 4, 2>(p, max_tiles, s);
     default: return launch<256, 256, 3, 2, 1, true>(p, max_tiles, s);
     }
 }

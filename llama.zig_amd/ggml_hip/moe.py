@@ -45,6 +45,8 @@ def _lib():
 # The checks build their messages only when they refuse.
 def _rows(t, shape, dtype, name, device):
     """The stride between rows of a [.., n] tensor of the shape, its last dimension contiguous."""
+    if t.is_contiguous() and t.shape == shape and t.dtype is dtype and t.get_device() == device >= 0:
+        return shape[-1]
     if not (t.dtype is dtype and t.get_device() == device >= 0 and t.shape == shape):
         raise HipQmmError(f"{name} must be {dtype} {list(shape)} on the GPU (of the others), not {t.dtype} {list(t.shape)}")
     n, stride = shape[-1], t.stride(-2)
@@ -73,15 +75,18 @@ def _rows3(t, name):
 
 
 def _i8_rows(t, stride, name):
-    """8-bit rows as the products take them; the last one's chunk of 16 bytes may end behind the row, but not behind
-    the tensor's memory."""
+    """The stride of 8-bit rows as the products take them; the last one's chunk of 16 bytes may end behind the row, but
+    not behind the tensor's memory."""
+    n = t.shape[-1]
+    if n % 16:
+        if t.numel() == n:  # one row
+            stride = (n + 15) // 16 * 16
+        last = t.storage_offset() + sum((s - 1) * d for s, d in zip(t.shape[:-1], t.stride()[:-1]))
+        if t.numel() and last + (n + 15) // 16 * 16 > t.untyped_storage().nbytes():
+            raise HipQmmError(f"{name}'s last row must end in memory of the tensor's up to 16 bytes")
     if stride % 16 or t.data_ptr() % 16:
         raise HipQmmError(f"{name}'s rows must be 16-byte aligned (quantize_i8 lays them so)")
-    n = t.shape[-1]
-    if n % 16 and t.numel():
-        last = t.storage_offset() + sum((s - 1) * d for s, d in zip(t.shape[:-1], t.stride()[:-1]))
-        if last + (n + 15) // 16 * 16 > t.untyped_storage().nbytes():
-            raise HipQmmError(f"{name}'s last row must end in memory of the tensor's up to 16 bytes")
+    return stride
 
 
 def route(logits: torch.Tensor, k: int, gating="softmax", bias=None, groups=1, keep=1, top=2, renormalize=False,
@@ -164,14 +169,12 @@ def mul_mat_i8(w: torch.Tensor, w_scale: torch.Tensor, x: torch.Tensor, x_scale=
         raise HipQmmError("w and x must be 2-D")
     rows, K = w.shape
     n = x.shape[0]
-    ws = _rows(w, w.shape, _I8, "w", device)
-    _i8_rows(w, ws, "w")
+    ws = _i8_rows(w, _rows(w, w.shape, _I8, "w", device), "w")
     sp = _flat(w_scale, rows, _F32, "w_scale", device)
     if x_scale is None:
         xs, xp = _rows(x, (n, K), _F32, "x", device), None
     else:
-        xs = _rows(x, (n, K), _I8, "x", device)
-        _i8_rows(x, xs, "x")
+        xs = _i8_rows(x, _rows(x, (n, K), _I8, "x", device), "x")
         xp = _flat(x_scale, n, _F32, "x_scale", device)
     if out is None:
         out, os_ = w_scale.new_empty((n, rows)), rows
@@ -206,9 +209,8 @@ def mul_mat_id_i8(w: torch.Tensor, w_scale: torch.Tensor, x: torch.Tensor, ids: 
     e, rows, K = w.shape
     n, ne11, _ = x.shape
     n_ids = ids.shape[1]
-    ws = _rows(w, w.shape, _I8, "w", device)
+    ws = _i8_rows(w, _rows(w, w.shape, _I8, "w", device), "w")
     es = w.stride(0) if e > 1 else rows * ws
-    _i8_rows(w, ws, "w")
     sp = _flat(w_scale, e * rows, _F32, "w_scale", device)
     xs = _rows3(x, "x")
     if x_scale is None:
@@ -216,7 +218,7 @@ def mul_mat_id_i8(w: torch.Tensor, w_scale: torch.Tensor, x: torch.Tensor, ids: 
         xp = None
     else:
         _rows(x, (n, ne11, K), _I8, "x", device)
-        _i8_rows(x, xs, "x")
+        xs = _i8_rows(x, xs, "x")
         xp = _flat(x_scale, n * ne11, _F32, "x_scale", device)
     si = _rows(ids, (n, n_ids), _I32, "ids", device)
     if out is None:

@@ -298,3 +298,48 @@ def test_two_streams_and_dirty_workspaces(n):
                     outs.append(call())
         torch.cuda.synchronize()
         assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.parametrize("K", [1, 2, 3, 5, 127, 1001, 2048, 4096])
+@pytest.mark.parametrize("shift", [0, 1, 2])
+def test_tokens_of_any_alignment(K, shift):
+    """f32 rows of one and a few tokens that start at any float."""
+    r = np.random.RandomState(K)
+    w, wn, ws, wsn = _experts(r, 5, 40, K)
+    for n in (1, 2, 3):
+        x = torch.randn(n, K + 5, device="cuda")[:, shift:shift + K]
+        q, s = R.quantize(x.cpu().numpy())
+        _near(G.mul_mat_i8(w[1], ws[1], x), R.product(wn[1], wsn[1], q, s))
+        ids = torch.from_numpy(r.randint(-1, 6, (n, 3)).astype(np.int32)).cuda()
+        _near(G.mul_mat_id_i8(w, ws, x[:, None], ids), R.product_id(wn, wsn, q[:, None], s[:, None], ids.cpu().numpy()))
+
+
+def test_one_row_of_any_length():
+    q = torch.randint(-127, 128, (32,), dtype=torch.int8, device="cuda")
+    one = torch.ones(1, device="cuda")
+    got = G.mul_mat_i8(q[None, :21], one, q[None, :21], one)
+    assert got.item() == float((q[:21].double() ** 2).sum())
+
+
+@pytest.mark.parametrize("rows,K,n", [(300, 256, 17), (9000, 640, 20), (9000, 160, 40), (260, 300, 520), (4100, 200, 600),
+                                      (2050, 130, 2100), (30000, 100, 300), (30000, 96, 1)])
+def test_every_form(rows, K, n):
+    """Sizes at which each kernel and tile is chosen, with ragged ends."""
+    r = np.random.RandomState(K)
+    w, wn = _rows(r, rows, K)
+    (ws, wsn), x = _scales(r, rows), r.randn(n, K).astype(np.float32)
+    q, s = R.quantize(x)
+    _near(G.mul_mat_i8(w, ws, torch.from_numpy(x).cuda()), R.product(wn, wsn, q, s))
+
+
+@pytest.mark.parametrize("n,e,k", [(4200, 3, 1), (9000, 2, 1), (2500, 70, 2), (1100, 300, 8)])
+def test_pairs_in_several_chunks(n, e, k):
+    """More pairs than one grouping workgroup takes, some without an expert."""
+    r = np.random.RandomState(n)
+    w, wn, ws, wsn = _experts(r, e, 33, 48)
+    ids = r.randint(-1, e + 1, (n, k)).astype(np.int32)
+    x = r.randn(n, 1, 48).astype(np.float32)
+    q, s = R.quantize(x)
+    out = torch.full((n, k, 33), np.nan, device="cuda")
+    G.mul_mat_id_i8(w, ws, torch.from_numpy(x).cuda(), torch.from_numpy(ids).cuda(), out=out)
+    _near(out, R.product_id(wn, wsn, q, s, ids))
