@@ -100,7 +100,7 @@ int hip_qmm_mul_mat_id_i8(const int8_t *w, const float *w_scale, int64_t K, int6
 
 /*
  * dst[t] = add[t] + sum_s weights[t][s] * y[t][s], over rows of nrows values,
- * summed in f32 with s ascending (add NULL: from 0).  With ids, slots whose id
+ * summed in f64 and rounded to f32 once (add NULL: from 0).  With ids, slots whose id
  * is negative are left out, whatever their rows hold.  Row (t, s) of y is at
  * y + t*y_token_stride + s*y_row_stride.  dst may be add with its stride.
  * n_ids 0..65535, n_tokens and nrows at most 2^31 - 1.

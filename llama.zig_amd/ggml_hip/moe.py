@@ -42,14 +42,16 @@ def _lib():
     return _bound
 
 
-# The checks build their messages only when they refuse.
+# The checks build their messages only when they refuse, and ask little of a contiguous tensor: a step's call lasts a few
+# microseconds.
 def _rows(t, shape, dtype, name, device):
     """The stride between rows of a [.., n] tensor of the shape, its last dimension contiguous."""
-    if t.is_contiguous() and t.shape == shape and t.dtype is dtype and t.get_device() == device >= 0:
-        return shape[-1]
-    if not (t.dtype is dtype and t.get_device() == device >= 0 and t.shape == shape):
+    if t.dtype is not dtype or t.get_device() != device or t.shape != shape or device < 0:
         raise HipQmmError(f"{name} must be {dtype} {list(shape)} on the GPU (of the others), not {t.dtype} {list(t.shape)}")
-    n, stride = shape[-1], t.stride(-2)
+    n = shape[-1]
+    if t.is_contiguous():
+        return n
+    stride = t.stride(-2)
     if n > 1 and t.stride(-1) != 1:
         raise HipQmmError(f"{name}'s last dimension must be contiguous")
     if shape[-2] <= 1:
@@ -60,18 +62,21 @@ def _rows(t, shape, dtype, name, device):
 
 
 def _flat(t, n, dtype, name, device):
-    if not (t.dtype is dtype and t.get_device() == device and t.numel() == n and t.is_contiguous()):
+    if t.dtype is not dtype or t.get_device() != device or t.numel() != n or not t.is_contiguous():
         raise HipQmmError(f"{name} must be {n} contiguous {dtype} values on the GPU of the others")
     return t.data_ptr()
 
 
-def _rows3(t, name):
+def _rows3(t, shape, dtype, name, device):
     """The stride between rows of a 3-D tensor whose first two dimensions run on as one."""
-    a, b, _ = t.shape
+    stride = _rows(t, shape, dtype, name, device)
+    if t.is_contiguous():
+        return stride
+    a, b, n = shape
     sa, sb, _ = t.stride()
     if a > 1 and b > 1 and sa != b * sb:
         raise HipQmmError(f"{name}'s first two dimensions must be evenly spaced")
-    return sb if b > 1 else sa if a > 1 else max(sb, t.shape[2])
+    return sb if b > 1 else sa if a > 1 else max(sb, n)
 
 
 def _i8_rows(t, stride, name):
@@ -100,11 +105,11 @@ def route(logits: torch.Tensor, k: int, gating="softmax", bias=None, groups=1, k
     weights by their sum, at least min_sum; scale multiplies them.  An expert
     whose logit or bias is -inf is never chosen; where none is left the id is
     -1 and the weight 0."""
-    device = logits.get_device()
-    if logits.dim() != 2:
+    device, size = logits.get_device(), logits.shape
+    if len(size) != 2:
         raise HipQmmError("logits must be f32 [n_tokens, n_experts]")
-    n, e = logits.shape
-    ls = _rows(logits, logits.shape, _F32, "logits", device)
+    n, e = size
+    ls = _rows(logits, size, _F32, "logits", device)
     bp = None if bias is None else _flat(bias, e, _F32, "bias", device)
     mode = GATINGS.get(gating)
     if mode is None:
@@ -148,7 +153,7 @@ def quantize_i8(x: torch.Tensor, out=None, scale=None):
             raise HipQmmError("out must be int8 of x's shape on its GPU, its last dimension contiguous")
         if out.dim() > 3:
             raise HipQmmError("out of more than three dimensions")
-        qs = _rows3(out, "out") if out.dim() == 3 else _rows(out, out.shape, _I8, "out", device)
+        qs = (_rows3 if out.dim() == 3 else _rows)(out, out.shape, _I8, "out", device)
         if n > 1 and qs < K:
             raise HipQmmError("out's rows must not overlap")
     if scale is None:
@@ -164,12 +169,12 @@ def mul_mat_i8(w: torch.Tensor, w_scale: torch.Tensor, x: torch.Tensor, x_scale=
     """f32 [n, rows]: (x . w) * x_scale[n] * w_scale[row], summed in integers.
     w int8 [rows, K], w_scale f32 [rows]; x int8 [n, K] with x_scale f32 [n], or
     f32 [n, K], quantized in the call."""
-    device = w.get_device()
-    if w.dim() != 2 or x.dim() != 2:
+    device, size, xsize = w.get_device(), w.shape, x.shape
+    if len(size) != 2 or len(xsize) != 2:
         raise HipQmmError("w and x must be 2-D")
-    rows, K = w.shape
-    n = x.shape[0]
-    ws = _i8_rows(w, _rows(w, w.shape, _I8, "w", device), "w")
+    rows, K = size
+    n = xsize[0]
+    ws = _i8_rows(w, _rows(w, size, _I8, "w", device), "w")
     sp = _flat(w_scale, rows, _F32, "w_scale", device)
     if x_scale is None:
         xs, xp = _rows(x, (n, K), _F32, "x", device), None
@@ -203,29 +208,25 @@ def mul_mat_id_i8(w: torch.Tensor, w_scale: torch.Tensor, x: torch.Tensor, ids: 
     w int8 [n_experts, rows, K], w_scale f32 [n_experts, rows]; x int8 [n_tokens,
     1 or n_ids, K] with x_scale f32 of its first two dimensions, or f32,
     quantized in the call; ids int32 [n_tokens, n_ids]."""
-    device = w.get_device()
-    if w.dim() != 3 or x.dim() != 3 or ids.dim() != 2:
+    device, size, xsize, isize = w.get_device(), w.shape, x.shape, ids.shape
+    if len(size) != 3 or len(xsize) != 3 or len(isize) != 2:
         raise HipQmmError("w and x must be 3-D, ids 2-D")
-    e, rows, K = w.shape
-    n, ne11, _ = x.shape
-    n_ids = ids.shape[1]
-    ws = _i8_rows(w, _rows(w, w.shape, _I8, "w", device), "w")
+    e, rows, K = size
+    n, ne11, _ = xsize
+    n_ids = isize[1]
+    ws = _i8_rows(w, _rows(w, size, _I8, "w", device), "w")
     es = w.stride(0) if e > 1 else rows * ws
     sp = _flat(w_scale, e * rows, _F32, "w_scale", device)
-    xs = _rows3(x, "x")
     if x_scale is None:
-        _rows(x, (n, ne11, K), _F32, "x", device)
-        xp = None
+        xs, xp = _rows3(x, (n, ne11, K), _F32, "x", device), None
     else:
-        _rows(x, (n, ne11, K), _I8, "x", device)
-        xs = _i8_rows(x, xs, "x")
+        xs = _i8_rows(x, _rows3(x, (n, ne11, K), _I8, "x", device), "x")
         xp = _flat(x_scale, n * ne11, _F32, "x_scale", device)
     si = _rows(ids, (n, n_ids), _I32, "ids", device)
     if out is None:
         out, os_ = w_scale.new_empty((n, n_ids, rows)), rows
     else:
-        _rows(out, (n, n_ids, rows), _F32, "out", device)
-        os_ = _rows3(out, "out")
+        os_ = _rows3(out, (n, n_ids, rows), _F32, "out", device)
     L = _lib()
     if n * n_ids == 0:
         return out
@@ -247,12 +248,12 @@ def combine(y: torch.Tensor, weights: torch.Tensor, ids=None, add=None, out=None
     and add[t].  y f32 [n_tokens, n_ids, rows], weights f32 [n_tokens, n_ids];
     with ids int32 [n_tokens, n_ids], slots of negative ids are left out.  out
     may be add."""
-    device = y.get_device()
-    if y.dim() != 3 or y.dtype is not _F32 or device < 0:
+    device, size = y.get_device(), y.shape
+    if len(size) != 3 or y.dtype is not _F32 or device < 0:
         raise HipQmmError("y must be f32 [n_tokens, n_ids, rows] on the GPU")
-    n, n_ids, rows = y.shape
+    n, n_ids, rows = size
     yt, ys, yc = y.stride()
-    if rows > 1 and yc != 1:
+    if yc != 1 and rows > 1:
         raise HipQmmError("y's rows must be contiguous")
     sw = _rows(weights, (n, n_ids), _F32, "weights", device)
     ip, si = (None, 0) if ids is None else (ids.data_ptr(), _rows(ids, (n, n_ids), _I32, "ids", device))
