@@ -59,7 +59,7 @@ int hip_qmm_moe_route(const float *logits, int64_t n_tokens, int64_t n_experts, 
  * to the nearest, half to even, cut to +-127: one f32 product with the f32 next
  * to 1/127, and IEEE f32 divisions.  A row
  * whose scale rounds to 0 has zeros, and one with a value that is not finite
- * zeros and a scale of NaN.  Only the K values of a row are written.  K at most
+ * zeros and a scale of NaN.  Only the K values of a row are written.  K 1 to
  * 131071, n_rows at most 2^24.
  */
 int hip_qmm_quantize_i8(const float *x, int64_t K, int64_t n_rows, int64_t x_stride, int8_t *q, int64_t q_stride,
@@ -73,7 +73,7 @@ int hip_qmm_quantize_i8(const float *x, int64_t K, int64_t n_rows, int64_t x_str
  *
  * w is int8, 16-byte aligned with a row stride that is a multiple of 16, and so
  * is an int8 x; the bytes from K to the next multiple of 16 of each of their
- * rows must be readable but do not matter.  K at most 131071, nrows and ncols at
+ * rows must be readable but do not matter.  K 1 to 131071, nrows and ncols at
  * most 2^22, their product at most 2^38.  The workspace is scratch, 256-byte aligned: its contents do
  * not matter before the call, and it serves one call at a time.
  */

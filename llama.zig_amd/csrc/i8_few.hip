@@ -358,9 +358,6 @@ Few arguments(const Product &p, const FewPlan &plan) {
 
 template <int NT, int DEPTH, FewMode MODE, bool IDS>
 int launch(const Few &f, dim3 grid, int bytes, hipStream_t s) {
-    static const hipError_t grown = hipFuncSetAttribute((const void *)few_kernel<NT, DEPTH, MODE, IDS>,
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-    if (grown != hipSuccess) return (int)grown;
     hipLaunchKernelGGL((few_kernel<NT, DEPTH, MODE, IDS>), grid, dim3(THREADS), bytes, s, f);
     return (int)hipGetLastError();
 }
@@ -402,12 +399,13 @@ FewPlan i8::few_pairs_plan(bool f32, int64_t K, int64_t nrows, int64_t n_as, int
     p.nt = 1;
     p.depth = 2;
     p.columns = (int)std::min(n_tokens, (int64_t)16);  // of an expert, unless a token asks for it twice
-    const int64_t rows = std::min((experts * nrows + 511) / 512, std::min(nrows, (int64_t)512));
-    p.rows = (int)std::max((rows + 15) / 16 * 16, (int64_t)16);
-    for (; p.rows > 64; p.rows -= 16)
-        if (fits(p, K, HALF)) return p;
-    if (fits(p, K, HALF)) return p;
-    for (; p.columns > 4; --p.columns)
+    const int64_t want = std::min((experts * nrows + 511) / 512, std::min(nrows, (int64_t)512));
+    const int rows = (int)std::max((want + 15) / 16 * 16, (int64_t)16), least = std::min(rows, 64);
+    for (const int most : {HALF, LDS})
+        for (p.rows = rows; p.rows >= least; p.rows -= 16)
+            if (fits(p, K, most)) return p;
+    // Long rows: fewer columns at a time, and the weights read again for the others.
+    for (p.rows = least; p.columns > 4; --p.columns)
         if (fits(p, K, LDS)) return p;
     fits(p, K, LDS);
     return p;

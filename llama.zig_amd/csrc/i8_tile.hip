@@ -355,9 +355,6 @@ int launch(const Product &p, int64_t max_tiles, hipStream_t s) {
     total = (total + 7) / 8;
     if (HALVES) total += std::min(total, (int64_t)NEIGHBOURS / 2);
     constexpr int bytes = std::max((TM * SW + TN * SX) * STAGE, TM / 8 * 2048 + (TM + 2 * TN + 4) * 4);
-    static const hipError_t grown = hipFuncSetAttribute((const void *)tile_kernel<TM, TN, SW, SX, G, HALVES>,
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (grown != hipSuccess) return (int)grown;
     constexpr int64_t MOST = 1 << 18;  // of an XCD in one launch
     for (int64_t base = 0; base < total; base += MOST) {
         hipLaunchKernelGGL((tile_kernel<TM, TN, SW, SX, G, HALVES>), dim3((unsigned)std::min(total - base, MOST) * 8),

@@ -83,11 +83,13 @@ def _i8_rows(t, stride, name):
     """The stride of 8-bit rows as the products take them; the last one's chunk of 16 bytes may end behind the row, but
     not behind the tensor's memory."""
     n = t.shape[-1]
+    if not t.numel():
+        return stride
     if n % 16:
         if t.numel() == n:  # one row
             stride = (n + 15) // 16 * 16
         last = t.storage_offset() + sum((s - 1) * d for s, d in zip(t.shape[:-1], t.stride()[:-1]))
-        if t.numel() and last + (n + 15) // 16 * 16 > t.untyped_storage().nbytes():
+        if last + (n + 15) // 16 * 16 > t.untyped_storage().nbytes():
             raise HipQmmError(f"{name}'s last row must end in memory of the tensor's up to 16 bytes")
     if stride % 16 or t.data_ptr() % 16:
         raise HipQmmError(f"{name}'s rows must be 16-byte aligned (quantize_i8 lays them so)")
@@ -114,6 +116,8 @@ def route(logits: torch.Tensor, k: int, gating="softmax", bias=None, groups=1, k
     mode = GATINGS.get(gating)
     if mode is None:
         raise HipQmmError(f"gating must be one of {sorted(GATINGS)}")
+    if k < 1:
+        raise HipQmmError("k must be at least 1")
     shape = (n, k)
     if ids is None:
         ids, si = logits.new_empty(shape, dtype=_I32), k

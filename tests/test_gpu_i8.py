@@ -64,7 +64,7 @@ def test_numbers_of_columns(n, rows, K):
 
 
 @pytest.mark.parametrize("rows,K,n", [(4096, 14336, 1), (14336, 4096, 24), (5003, 2720, 333), (1024, 131071, 2),
-                                      (300, 131071, 300), (2048, 768, 1), (1000, 4096, 700), (2304, 4096, 2100)])
+                                      (300, 131071, 300), (40, 131071, 1), (2048, 768, 1), (1000, 4096, 700), (2304, 4096, 2100)])
 def test_large_products(rows, K, n):
     r = np.random.RandomState(1)
     w, wn = _rows(r, rows, K)
@@ -330,6 +330,18 @@ def test_every_form(rows, K, n):
     (ws, wsn), x = _scales(r, rows), r.randn(n, K).astype(np.float32)
     q, s = R.quantize(x)
     _near(G.mul_mat_i8(w, ws, torch.from_numpy(x).cuda()), R.product(wn, wsn, q, s))
+
+
+@pytest.mark.parametrize("K,n,k,e", [(4096, 40, 8, 64), (9000, 30, 4, 40), (20000, 30, 4, 40), (40000, 3, 2, 6), (100000, 1, 2, 3),
+                                     (100000, 4, 2, 3)])
+def test_experts_of_long_rows(K, n, k, e):
+    """Columns that do not fit in LDS together, or not at all."""
+    r = np.random.RandomState(K)
+    w, wn, ws, wsn = _experts(r, e, 20, K)
+    ids = r.randint(0, e, (n, k)).astype(np.int32)
+    x = r.randn(n, 1, K).astype(np.float32)
+    q, s = R.quantize(x)
+    _near(G.mul_mat_id_i8(w, ws, torch.from_numpy(x).cuda(), torch.from_numpy(ids).cuda()), R.product_id(wn, wsn, q, s, ids))
 
 
 @pytest.mark.parametrize("n,e,k", [(4200, 3, 1), (9000, 2, 1), (2500, 70, 2), (1100, 300, 8)])

@@ -175,6 +175,7 @@ def test_calls_without_tokens(library):
     w = On(_rows(5, 32))
     assert G.mul_mat_i8(w, t(5), t(0, 32)).shape == (0, 5)
     assert G.mul_mat_id_i8(On(_rows(2, 5, 32)), t(2, 5), t(0, 1, 32), t(0, 3, dtype=I32)).shape == (0, 3, 5)
+    assert G.mul_mat_i8(On(_rows(5, 32)[:, :20]), t(5), t(0, 20, dtype=I8), t(0)).shape == (0, 5)
     assert G.combine(t(0, 2, 8), t(0, 2)).shape == (0, 8)
     assert G.quantize_i8(t(0, 32))[0].shape == (0, 32)
     assert not library.calls
@@ -183,3 +184,6 @@ def test_calls_without_tokens(library):
 def test_unknown_gating(library):
     with pytest.raises(G.HipQmmError):
         G.route(On(_t(2, 8)), 2, gating="relu")
+    with pytest.raises(G.HipQmmError):
+        G.route(On(_t(2, 8)), 0)
+    assert not library.calls
