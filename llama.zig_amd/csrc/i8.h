@@ -109,8 +109,10 @@ struct Groups {
 // i8_quantize.hip
 int quantize(const float *x, int64_t K, int64_t n_rows, int64_t x_stride, int8_t *q, int64_t q_stride, float *scale,
              hipStream_t s);
+// The tables; and, in the same launch, n_rows f32 rows of K at x as 8-bit ones (x NULL: none).
 int group(const int32_t *ids, int64_t ids_stride, int n_pairs, int n_ids, int n_as, int per_slot, int bn, const Groups &to,
-          float *dst, int64_t dst_stride, int64_t nrows, hipStream_t s);
+          float *dst, int64_t dst_stride, int64_t nrows, const float *x, int64_t K, int64_t n_rows, int64_t x_stride,
+          int8_t *q, int64_t q_stride, float *scale, hipStream_t s);
 
 // i8_few.hip: how few columns are taken, from the sizes alone.
 enum FewMode { QUANTIZE, RESIDENT, THROUGH };  // f32 columns quantized in LDS; 8-bit ones in LDS; through the ring

@@ -56,14 +56,11 @@ bool workspace_ok(const void *ws, size_t have, size_t need) {
     return need == 0 || (ws && !((uintptr_t)ws % 256) && have >= need);
 }
 
-// p's f32 columns to 8-bit ones in the workspace.
-int quantize_tokens(Product &p, const Tokens &t, int64_t n, void *workspace, hipStream_t s) {
-    uint8_t *ws = (uint8_t *)workspace;
-    int8_t *q = (int8_t *)(ws + t.q);
-    float *scale = (float *)(ws + t.scale);
-    const int e = quantize((const float *)p.x, p.K, n, p.x_stride, q, token_stride(p.K), scale, s);
-    p.x = q, p.x_scale = scale, p.x_stride = token_stride(p.K);
-    return e;
+// p with its columns as they will be in the workspace.
+Product quantized_tokens(Product p, const Tokens &t, void *workspace) {
+    p.x = (const int8_t *)workspace + t.q, p.x_scale = (const float *)((uint8_t *)workspace + t.scale);
+    p.x_stride = token_stride(p.K);
+    return p;
 }
 
 }  // namespace
@@ -92,7 +89,8 @@ extern "C" int hip_qmm_mul_mat_i8(const int8_t *w, const float *w_scale, int64_t
     if (!x_scale) {
         const FewPlan plan = few_plan(true, K, nrows, ncols);
         if (plan.bytes) return few_product(p, plan, s);
-        if (int e = quantize_tokens(p, tokens_at(0, K, ncols), ncols, workspace, s)) return e;
+        p = quantized_tokens(p, tokens_at(0, K, ncols), workspace);
+        if (int e = quantize((const float *)x, K, ncols, x_stride, (int8_t *)p.x, p.x_stride, (float *)p.x_scale, s)) return e;
     }
     const FewPlan plan = few_plan(false, K, nrows, ncols);
     // Many rows and over 16 columns: tiles, whose workgroups share the columns (14336 x 4096 by 32: 15 us, 19 us).
@@ -144,14 +142,21 @@ extern "C" int hip_qmm_mul_mat_id_i8(const int8_t *w, const float *w_scale, int6
     if (!quantized) {
         const FewPlan plan = few_pairs_plan(true, K, nrows, n_as, n_tokens, n_ids);
         if (plan.bytes) return few_pairs(p, plan, ids, ids_stride, pairs, (int)n_ids, (int)n_as, ne11 > 1, s);
-        if (int e = quantize_tokens(p, t, n_tokens * ne11, workspace, s)) return e;
+        p = quantized_tokens(p, t, workspace);
     }
+    const float *xf = quantized ? nullptr : (const float *)x;
+    int8_t *q = (int8_t *)p.x;
+    float *scale = (float *)p.x_scale;
     const FewPlan plan = few_pairs_plan(false, K, nrows, n_as, n_tokens, n_ids);
-    if (plan.bytes) return few_pairs(p, plan, ids, ids_stride, pairs, (int)n_ids, (int)n_as, ne11 > 1, s);
+    if (plan.bytes) {
+        if (xf)
+            if (int e = quantize(xf, K, n_tokens * ne11, x_stride, q, p.x_stride, scale, s)) return e;
+        return few_pairs(p, plan, ids, ids_stride, pairs, (int)n_ids, (int)n_as, ne11 > 1, s);
+    }
     const Groups to = {(int32_t *)(ws + g.src), (int32_t *)(ws + g.dst), (int32_t *)(ws + g.tiles),
                        (int32_t *)(ws + g.n_tiles), (int32_t *)(ws + g.counts), (uint16_t *)(ws + g.places)};
     if (int e = group(ids, ids_stride, pairs, (int)n_ids, (int)n_as, ne11 > 1, tile_columns(g.form), to, dst, dst_stride,
-                      nrows, s))
+                      nrows, xf, K, n_tokens * ne11, x_stride, q, p.x_stride, scale, s))
         return e;
     p.tiles = to.tiles, p.n_tiles = to.n_tiles, p.col_src = to.col_src, p.col_dst = to.col_dst;
     return tile_product(p, g.form, g.max_tiles, s);

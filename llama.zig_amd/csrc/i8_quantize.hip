@@ -11,27 +11,37 @@ using namespace i8;
 
 namespace {
 
-// A workgroup a row, its values in registers between the maximum and the rounding: one read of memory.  HBM bound on
-// many rows, latency on few.  V float4 a thread; WIDE: rows of whole aligned float4.
-template <int THREADS, int V, bool WIDE>
-__global__ __launch_bounds__(THREADS) void quantize_kernel(const float *__restrict__ x0, int K, int64_t n_rows,
-                                                           int64_t x_stride, int8_t *__restrict__ q0, int64_t q_stride,
-                                                           float *__restrict__ scale) {
-    __shared__ uint32_t most[2][THREADS / 64];
-    const int tid = threadIdx.x;
+struct Rows {
+    const float *x;
+    int K;
+    int64_t n_rows, x_stride;
+    int8_t *q;
+    int64_t q_stride;
+    float *scale;
+};
+
+// TEAM threads a row, its values in registers between the maximum and the rounding: one read of memory, for rows of up to
+// TEAM * V float4.  HBM bound on many rows, latency on few.  WIDE: rows of whole aligned float4.  Workgroup `block` of
+// `blocks` of BLOCK threads; `most` is for 2 * BLOCK / 64 values in LDS.
+template <int BLOCK, int TEAM, int V, bool WIDE>
+__device__ __forceinline__ void quantize_rows(const Rows &a, int block, int blocks, uint32_t *most) {
+    constexpr int TEAMS = BLOCK / TEAM, WAVES = BLOCK / 64;
+    const int team = threadIdx.x / TEAM, tid = threadIdx.x % TEAM, units = (a.K + 3) / 4;
     int turn = 0;
-    for (int64_t r = blockIdx.x; r < n_rows; r += gridDim.x, turn ^= 1) {
-        const float *x = x0 + r * x_stride;
-        int8_t *q = q0 + r * q_stride;
+    for (int64_t base = (int64_t)block * TEAMS; base < a.n_rows; base += (int64_t)blocks * TEAMS, turn ^= 1) {
+        const int64_t r = base + team;
+        const bool real = r < a.n_rows;
+        const float *x = a.x + r * a.x_stride;
+        int8_t *q = a.q + r * a.q_stride;
         uint32_t m = 0;
         float4 v[V];
         auto load = [&](int k) {  // values 4 k .. 4 k + 3
             if (WIDE) return reinterpret_cast<const float4 *>(x)[k];
             float4 u = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             u.x = x[4 * k];
-            if (4 * k + 1 < K) u.y = x[4 * k + 1];
-            if (4 * k + 2 < K) u.z = x[4 * k + 2];
-            if (4 * k + 3 < K) u.w = x[4 * k + 3];
+            if (4 * k + 1 < a.K) u.y = x[4 * k + 1];
+            if (4 * k + 2 < a.K) u.z = x[4 * k + 2];
+            if (4 * k + 3 < a.K) u.w = x[4 * k + 3];
             return u;
         };
         auto store = [&](int k, uint32_t b) {
@@ -39,51 +49,62 @@ __global__ __launch_bounds__(THREADS) void quantize_kernel(const float *__restri
                 reinterpret_cast<uint32_t *>(q)[k] = b;
                 return;
             }
-            for (int i = 0; i < min(4, K - 4 * k); ++i) q[4 * k + i] = (int8_t)(b >> (8 * i));
+            for (int i = 0; i < min(4, a.K - 4 * k); ++i) q[4 * k + i] = (int8_t)(b >> (8 * i));
         };
         auto larger = [&](float4 u) {
             m = max(m, max(max(magnitude(u.x), magnitude(u.y)), max(magnitude(u.z), magnitude(u.w))));
         };
-        const int units = (K + 3) / 4;
+        const int end = real ? units : 0;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (i * THREADS + tid < units) v[i] = load(i * THREADS + tid);
+            if (i * TEAM + tid < end) v[i] = load(i * TEAM + tid);
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) larger(v[i]);
-        for (int k = V * THREADS + tid; k < units; k += THREADS) larger(load(k));  // rows longer than the registers: read twice
+        for (int k = V * TEAM + tid; k < end; k += TEAM) larger(load(k));  // rows longer than the registers: read twice
 #pragma unroll
         for (int d = 32; d; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
-        if ((tid & 63) == 0) most[turn][tid >> 6] = m;
-        __syncthreads();
+        if constexpr (TEAM > 64) {
+            if ((threadIdx.x & 63) == 0) most[turn * WAVES + (threadIdx.x >> 6)] = m;
+            __syncthreads();
 #pragma unroll
-        for (int w = 0; w < THREADS / 64; ++w) m = max(m, most[turn][w]);
+            for (int w = 0; w < TEAM / 64; ++w) m = max(m, most[turn * WAVES + team * (TEAM / 64) + w]);
+        }
         const Scale s(m);
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (i * THREADS + tid < units) store(i * THREADS + tid, s.four(v[i]));
-        for (int k = V * THREADS + tid; k < units; k += THREADS) store(k, s.four(load(k)));
-        if (tid == 0) scale[r] = s.value;
+            if (i * TEAM + tid < end) store(i * TEAM + tid, s.four(v[i]));
+        for (int k = V * TEAM + tid; k < end; k += TEAM) store(k, s.four(load(k)));
+        if (real && tid == 0) a.scale[r] = s.value;
     }
 }
 
-template <int THREADS, int V>
-int launch(bool wide, const float *x, int K, int64_t n_rows, int64_t x_stride, int8_t *q, int64_t q_stride, float *scale,
-           hipStream_t s) {
-    const dim3 grid((unsigned)std::min(n_rows, (int64_t)1 << 20)), block(THREADS);
+template <int TEAM, int V, bool WIDE>
+__global__ __launch_bounds__(TEAM) void quantize_kernel(Rows a) {
+    __shared__ uint32_t most[2 * (TEAM / 64)];
+    quantize_rows<TEAM, TEAM, V, WIDE>(a, blockIdx.x, gridDim.x, most);
+}
+
+template <int TEAM, int V>
+int launch(bool wide, const Rows &a, hipStream_t s) {
+    const dim3 grid((unsigned)std::min(a.n_rows, (int64_t)1 << 20)), block(TEAM);
     if (wide)
-        hipLaunchKernelGGL((quantize_kernel<THREADS, V, true>), grid, block, 0, s, x, K, n_rows, x_stride, q, q_stride, scale);
+        hipLaunchKernelGGL((quantize_kernel<TEAM, V, true>), grid, block, 0, s, a);
     else
-        hipLaunchKernelGGL((quantize_kernel<THREADS, V, false>), grid, block, 0, s, x, K, n_rows, x_stride, q, q_stride, scale);
+        hipLaunchKernelGGL((quantize_kernel<TEAM, V, false>), grid, block, 0, s, a);
     return (int)hipGetLastError();
+}
+
+bool wide_rows(const Rows &a) {
+    return !(a.K % 4 || a.x_stride % 4 || a.q_stride % 4 || (uintptr_t)a.x % 16 || (uintptr_t)a.q % 4);
 }
 
 constexpr int GROUP_THREADS = 1024, PER = PAIR_CHUNK / GROUP_THREADS;
 
 // The pairs of (token, slot) by experts: where a pair's column stands among its expert's does not matter to any result,
 // so it is the order in which LDS counters are met.  A workgroup counts the experts of a chunk of pairs and notes each
-// pair's place in its chunk.  With more than one chunk `place_kernel` goes on from the counts; with one, it is done here.
+// pair's place in its chunk.  With more than one chunk `place_kernel` goes on from the counts; with one, it is done at once.
 struct Pairs {
     const int32_t *ids;
     int64_t ids_stride;
@@ -160,12 +181,10 @@ __device__ __forceinline__ void load(const Pairs &a, int chunk, int (&id)[PER]) 
 }
 
 template <bool ONE>
-__global__ __launch_bounds__(GROUP_THREADS) void count_kernel(Pairs a) {
-    __shared__ int count[GROUP_THREADS];
-    __shared__ int2 sums[GROUP_THREADS / 64];
+__device__ __forceinline__ void count_pairs(const Pairs &a, int chunk, int *count, int2 *sums) {
     int id[PER], at[PER];
     count[threadIdx.x] = 0;
-    load(a, blockIdx.x, id);
+    load(a, chunk, id);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < PER; ++i) at[i] = id[i] >= 0 ? atomicAdd(&count[id[i]], 1) : 0;
@@ -175,13 +194,34 @@ __global__ __launch_bounds__(GROUP_THREADS) void count_kernel(Pairs a) {
         __syncthreads();
         place(a, id, at, 0, 0, total, true, count, sums);
     } else {
-        if ((int)threadIdx.x < a.n_as) a.counts[(int64_t)blockIdx.x * a.n_as + threadIdx.x] = count[threadIdx.x];
+        if ((int)threadIdx.x < a.n_as) a.counts[(int64_t)chunk * a.n_as + threadIdx.x] = count[threadIdx.x];
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int p = blockIdx.x * PAIR_CHUNK + i * GROUP_THREADS + threadIdx.x;
+            const int p = chunk * PAIR_CHUNK + i * GROUP_THREADS + threadIdx.x;
             if (p < a.n_pairs) a.places[p] = (uint16_t)at[i];
         }
     }
+}
+
+// The first workgroups count pairs, the others quantize tokens meanwhile.
+template <int TEAM, int V, bool ONE>
+__global__ __launch_bounds__(GROUP_THREADS) void prepare_kernel(Pairs a, int chunks, Rows tokens) {
+    __shared__ int count[GROUP_THREADS];
+    __shared__ int2 sums[GROUP_THREADS / 64];
+    if ((int)blockIdx.x < chunks)
+        count_pairs<ONE>(a, blockIdx.x, count, sums);
+    else
+        quantize_rows<GROUP_THREADS, TEAM, V, true>(tokens, blockIdx.x - chunks, gridDim.x - chunks, (uint32_t *)count);
+}
+
+template <int TEAM, int V>
+void launch_prepare(const Pairs &a, int chunks, const Rows &tokens, hipStream_t s) {
+    const int64_t blocks = tokens.n_rows ? (tokens.n_rows * TEAM + GROUP_THREADS - 1) / GROUP_THREADS : 0;
+    const dim3 grid((unsigned)(chunks + std::min(blocks, (int64_t)1 << 18))), block(GROUP_THREADS);
+    if (chunks == 1)
+        hipLaunchKernelGGL((prepare_kernel<TEAM, V, true>), grid, block, 0, s, a, chunks, tokens);
+    else
+        hipLaunchKernelGGL((prepare_kernel<TEAM, V, false>), grid, block, 0, s, a, chunks, tokens);
 }
 
 __global__ __launch_bounds__(GROUP_THREADS) void place_kernel(Pairs a) {
@@ -207,27 +247,38 @@ __global__ __launch_bounds__(GROUP_THREADS) void place_kernel(Pairs a) {
 
 }  // namespace
 
+static int quantize_rows_of(const Rows &a, hipStream_t s) {
+    const bool wide = wide_rows(a);
+    if (a.K <= 1024) return launch<64, 4>(wide, a, s);
+    if (a.K <= 8192) return launch<256, 8>(wide, a, s);
+    return launch<1024, 4>(wide, a, s);
+}
+
 int i8::quantize(const float *x, int64_t K, int64_t n_rows, int64_t x_stride, int8_t *q, int64_t q_stride, float *scale,
                  hipStream_t s) {
-    const bool wide = !(K % 4 || x_stride % 4 || q_stride % 4 || (uintptr_t)x % 16 || (uintptr_t)q % 4);
-    if (K <= 1024) return launch<64, 4>(wide, x, (int)K, n_rows, x_stride, q, q_stride, scale, s);
-    if (K <= 8192) return launch<256, 8>(wide, x, (int)K, n_rows, x_stride, q, q_stride, scale, s);
-    return launch<1024, 4>(wide, x, (int)K, n_rows, x_stride, q, q_stride, scale, s);
+    return quantize_rows_of({x, (int)K, n_rows, x_stride, q, q_stride, scale}, s);
 }
 
 int i8::group(const int32_t *ids, int64_t ids_stride, int n_pairs, int n_ids, int n_as, int per_slot, int bn,
-              const Groups &to, float *dst, int64_t dst_stride, int64_t nrows, hipStream_t s) {
+              const Groups &to, float *dst, int64_t dst_stride, int64_t nrows, const float *x, int64_t K, int64_t n_rows,
+              int64_t x_stride, int8_t *q, int64_t q_stride, float *scale, hipStream_t s) {
     const Pairs a = {ids, ids_stride, n_pairs, n_ids, n_as, per_slot, bn, to.col_src, to.col_dst, to.tiles, to.n_tiles,
                      to.counts, to.places, dst, dst_stride, nrows};
-    const dim3 block(GROUP_THREADS);
-    if (n_pairs <= PAIR_CHUNK) {
-        hipLaunchKernelGGL(count_kernel<true>, dim3(1), block, 0, s, a);
-        return (int)hipGetLastError();
+    Rows tokens = {x, (int)K, x ? n_rows : 0, x_stride, q, q_stride, scale};
+    if (x && !wide_rows(tokens)) {
+        if (int e = quantize_rows_of(tokens, s)) return e;
+        tokens.n_rows = 0;
     }
-    const dim3 grid((unsigned)((n_pairs + PAIR_CHUNK - 1) / PAIR_CHUNK));
-    hipLaunchKernelGGL(count_kernel<false>, grid, block, 0, s, a);
-    if (int e = (int)hipGetLastError()) return e;
-    hipLaunchKernelGGL(place_kernel, grid, block, 0, s, a);
+    const int chunks = (n_pairs + PAIR_CHUNK - 1) / PAIR_CHUNK;
+    if (K <= 1024)
+        launch_prepare<64, 4>(a, chunks, tokens, s);
+    else if (K <= 8192)
+        launch_prepare<256, 8>(a, chunks, tokens, s);
+    else
+        launch_prepare<1024, 4>(a, chunks, tokens, s);
+    const int e = (int)hipGetLastError();
+    if (e || chunks == 1) return e;
+    hipLaunchKernelGGL(place_kernel, dim3((unsigned)chunks), dim3(GROUP_THREADS), 0, s, a);
     return (int)hipGetLastError();
 }
 
