@@ -124,7 +124,7 @@ def route(logits: torch.Tensor, k: int, gating="softmax", bias=None, groups=1, k
     else:
         si = _rows(ids, shape, _I32, "ids", device)
     if weights is None:
-        weights, sw = logits.new_empty(shape), k
+        weights, sw = logits.new_empty(n, k), k
     else:
         sw = _rows(weights, shape, _F32, "weights", device)
     _check(_lib().hip_qmm_moe_route(logits.data_ptr(), n, e, ls, bp, mode, groups, keep, top, k, bool(renormalize),
@@ -186,20 +186,21 @@ def mul_mat_i8(w: torch.Tensor, w_scale: torch.Tensor, x: torch.Tensor, x_scale=
         xs = _i8_rows(x, _rows(x, (n, K), _I8, "x", device), "x")
         xp = _flat(x_scale, n, _F32, "x_scale", device)
     if out is None:
-        out, os_ = w_scale.new_empty((n, rows)), rows
+        out, os_ = w_scale.new_empty(n, rows), rows
     else:
         os_ = _rows(out, (n, rows), _F32, "out", device)
     L = _lib()
     if n == 0:
         return out
-    need = L.hip_qmm_mul_mat_i8_workspace_size(K, rows, n, xp is not None)
     if workspace is None:
-        wp, have = None, need
-        if need:
-            workspace = w_scale.new_empty(need, dtype=torch.uint8)
+        # Of many tokens the header's bound: cheaper than to ask.
+        have = n * (K + 131) + 512 if xp is None and n > 32 else L.hip_qmm_mul_mat_i8_workspace_size(K, rows, n, xp is not None)
+        wp = None
+        if have:
+            workspace = w_scale.new_empty(have, dtype=torch.uint8)
             wp = workspace.data_ptr()
     else:
-        wp, have = _scratch(workspace, need, device)
+        wp, have = _scratch(workspace, L.hip_qmm_mul_mat_i8_workspace_size(K, rows, n, xp is not None), device)
     _check(L.hip_qmm_mul_mat_i8(w.data_ptr(), sp, K, rows, ws, x.data_ptr(), xp, n, xs, out.data_ptr(), os_, wp, have,
                                 _raw_stream(device)), "hip_qmm_mul_mat_i8")
     return out
@@ -228,7 +229,7 @@ def mul_mat_id_i8(w: torch.Tensor, w_scale: torch.Tensor, x: torch.Tensor, ids: 
         xp = _flat(x_scale, n * ne11, _F32, "x_scale", device)
     si = _rows(ids, (n, n_ids), _I32, "ids", device)
     if out is None:
-        out, os_ = w_scale.new_empty((n, n_ids, rows)), rows
+        out, os_ = w_scale.new_empty(n, n_ids, rows), rows
     else:
         os_ = _rows3(out, (n, n_ids, rows), _F32, "out", device)
     L = _lib()
@@ -263,7 +264,7 @@ def combine(y: torch.Tensor, weights: torch.Tensor, ids=None, add=None, out=None
     ip, si = (None, 0) if ids is None else (ids.data_ptr(), _rows(ids, (n, n_ids), _I32, "ids", device))
     ap, sa = (None, 0) if add is None else (add.data_ptr(), _rows(add, (n, rows), _F32, "add", device))
     if out is None:
-        out, so = y.new_empty((n, rows)), rows
+        out, so = y.new_empty(n, rows), rows
     else:
         so = _rows(out, (n, rows), _F32, "out", device)
     if n * rows == 0:

@@ -70,6 +70,9 @@ def test_product_refusals():
     for kw in (dict(size=need - 1), dict(workspace=None), dict(workspace=P + 128)):
         assert _product(**kw, xs=None, n=400) == BAD, kw
     f = M._lib().hip_qmm_mul_mat_i8_workspace_size
+    for K in (1, 127, 128, 129, 4096, 131071):
+        for n in (1, 2, 16, 17, 33, 1000, 1 << 22):
+            assert f(K, 500, n, 0) <= n * (K + 131) + 512 and f(K, 500, n, 1) == 0
     assert f(0, 32, 4, 0) == f(64, 0, 4, 0) == f(64, 32, 0, 0) == f(64, 32, -1, 1) == 0
 
 
