@@ -205,7 +205,7 @@ __device__ __forceinline__ void count_pairs(const Pairs &a, int chunk, int *coun
 
 // The first workgroups count pairs, the others quantize tokens meanwhile.
 template <int TEAM, int V, bool ONE>
-__global__ __launch_bounds__(GROUP_THREADS) void prepare_kernel(Pairs a, int chunks, Rows tokens) {
+__global__ __launch_bounds__(GROUP_THREADS, 8) void prepare_kernel(Pairs a, int chunks, Rows tokens) {
     __shared__ int count[GROUP_THREADS];
     __shared__ int2 sums[GROUP_THREADS / 64];
     if ((int)blockIdx.x < chunks)
@@ -236,12 +236,19 @@ __global__ __launch_bounds__(GROUP_THREADS) void place_kernel(Pairs a) {
         at[i] = p < a.n_pairs ? a.places[p] : 0;
     }
     int before = 0, total = 0;
-    if (e < a.n_as)
-        for (int c = 0; c < (int)gridDim.x; ++c) {
-            const int n = a.counts[(int64_t)c * a.n_as + e];
-            before += c < chunk ? n : 0;
-            total += n;
+    if (e < a.n_as) {
+        const int chunks = gridDim.x;
+        for (int c0 = 0; c0 < chunks; c0 += 8) {  // eight loads under way together
+            int n[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) n[i] = a.counts[(int64_t)min(c0 + i, chunks - 1) * a.n_as + e];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                before += c0 + i < chunk ? n[i] : 0;
+                total += c0 + i < chunks ? n[i] : 0;
+            }
         }
+    }
     place(a, id, at, chunk, before, total, chunk == 0, base, sums);
 }
 
@@ -270,10 +277,11 @@ int i8::group(const int32_t *ids, int64_t ids_stride, int n_pairs, int n_ids, in
         tokens.n_rows = 0;
     }
     const int chunks = (n_pairs + PAIR_CHUNK - 1) / PAIR_CHUNK;
+    // Four float4 a thread: two workgroups a CU.
     if (K <= 1024)
         launch_prepare<64, 4>(a, chunks, tokens, s);
-    else if (K <= 8192)
-        launch_prepare<256, 8>(a, chunks, tokens, s);
+    else if (K <= 4096)
+        launch_prepare<256, 4>(a, chunks, tokens, s);
     else
         launch_prepare<1024, 4>(a, chunks, tokens, s);
     const int e = (int)hipGetLastError();
