@@ -77,3 +77,17 @@ def test_what_is_not_finite():
     got = G.combine(y, w).cpu()
     assert torch.isnan(got[0, 2]) and (got[0, [0, 1, 3, 4, 5, 6, 7]] == 2).all()
     assert got[1, 3] == float("inf") and (got[1, :3] == 1).all() and torch.isinf(got[2]).all()
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 6, 7, 514, 1031])
+@pytest.mark.parametrize("off", [0, 1, 2, 3])
+def test_ends_of_rows(rows, off):
+    """Rows of any length from any multiple of four bytes; nothing before or behind them is written."""
+    torch.manual_seed(rows)
+    y = torch.randn(9, 4, rows + 5, device="cuda")[..., off:off + rows]
+    w = torch.randn(9, 4, device="cuda")
+    add = torch.randn(9, rows + 6, device="cuda")[:, 1:1 + rows]
+    out = torch.full((9, rows + 5), 7.0, device="cuda")
+    got = G.combine(y, w, add=add, out=out[:, off:off + rows])
+    _check(y, w, add=add, got=got)
+    assert (out[:, :off] == 7).all() and (out[:, off + rows:] == 7).all()
