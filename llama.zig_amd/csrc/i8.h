@@ -1,5 +1,5 @@
 // i8.h -- what the sources of the 8-bit integer products share (i8_quantize.hip,
-// i8_stream.hip, i8_api.hip).
+// i8_few.hip, i8_tile.hip, i8_api.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -46,6 +46,13 @@ __device__ __forceinline__ v4i cut(v4i v, int keep) {
 
 // A row's largest magnitude, as the bits of an f32: integers compare as magnitudes do, and a NaN is above infinity.
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// Four values that need not be aligned to more than one: nor need a load of 16 bytes.
+__device__ __forceinline__ float4 four_at(const float *x) {
+    typedef float v4f __attribute__((ext_vector_type(4), aligned(4)));
+    const v4f v = *reinterpret_cast<const v4f *>(x);
+    return make_float4(v[0], v[1], v[2], v[3]);
+}
 
 // What a row's values are divided by.
 struct Scale {
@@ -132,7 +139,7 @@ int few_pairs(const Product &p, const FewPlan &plan, const int32_t *ids, int64_t
 // i8_tile.hip: tiles of TM weight rows and TN columns.
 enum TileForm { TILE_64x64, TILE_128x64, TILE_128x128, TILE_128x128_DEEP, TILE_256x256 };
 TileForm tile_form(int64_t nrows, int64_t ncols);                   // dense
-TileForm tile_form_grouped(int64_t n_as, int64_t n_pairs);         // by experts
+TileForm tile_form_grouped(int64_t K, int64_t nrows, int64_t n_as, int64_t n_pairs);  // by experts
 int tile_columns(TileForm form);
 int tile_product(const Product &p, TileForm form, int64_t max_tiles, hipStream_t s);
 

@@ -33,9 +33,9 @@ struct Grouped {
     int64_t max_tiles;
 };
 
-Grouped grouped_at(size_t at, int64_t n_as, int64_t pairs) {
+Grouped grouped_at(size_t at, int64_t K, int64_t nrows, int64_t n_as, int64_t pairs) {
     Grouped g;
-    g.form = tile_form_grouped(n_as, pairs);
+    g.form = tile_form_grouped(K, nrows, n_as, pairs);
     g.max_tiles = pairs / tile_columns(g.form) + std::min(pairs, n_as);
     g.src = at;
     g.dst = a256(g.src + (size_t)pairs * 4);
@@ -108,7 +108,7 @@ extern "C" size_t hip_qmm_mul_mat_id_i8_workspace_size(int64_t K, int64_t nrows,
     const bool few = few_pairs_plan(false, K, nrows, n_as, n_tokens, n_ids).bytes != 0;  // no tables
     if (!quantized && few_pairs_plan(true, K, nrows, n_as, n_tokens, n_ids).bytes) return 0;
     if (few) return quantized ? 0 : tokens_at(0, K, n_tokens * ne11).end;
-    return grouped_at(quantized ? 0 : tokens_at(0, K, n_tokens * ne11).end, n_as, n_tokens * n_ids).end;
+    return grouped_at(quantized ? 0 : tokens_at(0, K, n_tokens * ne11).end, K, nrows, n_as, n_tokens * n_ids).end;
 }
 
 extern "C" int hip_qmm_mul_mat_id_i8(const int8_t *w, const float *w_scale, int64_t K, int64_t nrows, int64_t w_stride,
@@ -132,7 +132,7 @@ extern "C" int hip_qmm_mul_mat_id_i8(const int8_t *w, const float *w_scale, int6
     hipStream_t s = (hipStream_t)stream;
     uint8_t *ws = (uint8_t *)workspace;
     const Tokens t = tokens_at(0, K, n_tokens * ne11);
-    const Grouped g = grouped_at(quantized ? 0 : t.end, n_as, n_tokens * n_ids);
+    const Grouped g = grouped_at(quantized ? 0 : t.end, K, nrows, n_as, n_tokens * n_ids);
     Product p = {};
     p.w = w, p.w_scale = w_scale, p.w_stride = w_stride, p.expert_stride = expert_stride;
     p.dst = dst, p.dst_stride = dst_stride;

@@ -216,8 +216,10 @@ __global__ __launch_bounds__(THREADS) void few_kernel(Few f) {
                 } else {
                     for (int i = wave; i < count; i += WAVES) {
                         const float *row = (const float *)a.x + src[c0 + i] * a.x_stride;
-                        for (int k = lane; k < units * 4; k += 64)
-                            reinterpret_cast<float *>(stage)[i * units * 4 + k] = k < a.K ? row[k] : 0.0f;
+                        float *to = reinterpret_cast<float *>(stage) + i * units * 4;
+#pragma unroll 4
+                        for (int k = lane * 4; k + 4 <= a.K; k += 256) *reinterpret_cast<float4 *>(to + k) = four_at(row + k);
+                        if (const int k = a.K / 4 * 4 + lane; k < units * 4) to[k] = k < a.K ? row[k] : 0.0f;
                     }
                 }
                 if (c0 == 0) {

@@ -21,12 +21,13 @@ struct Rows {
 };
 
 // TEAM threads a row, its values in registers between the maximum and the rounding: one read of memory, for rows of up to
-// TEAM * V float4.  HBM bound on many rows, latency on few.  WIDE: rows of whole aligned float4.  Workgroup `block` of
-// `blocks` of BLOCK threads; `most` is for 2 * BLOCK / 64 values in LDS.
-template <int BLOCK, int TEAM, int V, bool WIDE>
+// TEAM * V float4.  HBM bound on many rows, latency on few.  Workgroup `block` of `blocks` of BLOCK threads; `most` is for
+// 2 * BLOCK / 64 values in LDS.
+template <int BLOCK, int TEAM, int V>
 __device__ __forceinline__ void quantize_rows(const Rows &a, int block, int blocks, uint32_t *most) {
     constexpr int TEAMS = BLOCK / TEAM, WAVES = BLOCK / 64;
-    const int team = threadIdx.x / TEAM, tid = threadIdx.x % TEAM, units = (a.K + 3) / 4;
+    typedef uint32_t word __attribute__((aligned(1)));  // a store of 4 bytes need not be aligned
+    const int team = threadIdx.x / TEAM, tid = threadIdx.x % TEAM, units = a.K / 4;
     int turn = 0;
     for (int64_t base = (int64_t)block * TEAMS; base < a.n_rows; base += (int64_t)blocks * TEAMS, turn ^= 1) {
         const int64_t r = base + team;
@@ -35,22 +36,6 @@ __device__ __forceinline__ void quantize_rows(const Rows &a, int block, int bloc
         int8_t *q = a.q + r * a.q_stride;
         uint32_t m = 0;
         float4 v[V];
-        auto load = [&](int k) {  // values 4 k .. 4 k + 3
-            if (WIDE) return reinterpret_cast<const float4 *>(x)[k];
-            float4 u = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            u.x = x[4 * k];
-            if (4 * k + 1 < a.K) u.y = x[4 * k + 1];
-            if (4 * k + 2 < a.K) u.z = x[4 * k + 2];
-            if (4 * k + 3 < a.K) u.w = x[4 * k + 3];
-            return u;
-        };
-        auto store = [&](int k, uint32_t b) {
-            if (WIDE) {
-                reinterpret_cast<uint32_t *>(q)[k] = b;
-                return;
-            }
-            for (int i = 0; i < min(4, a.K - 4 * k); ++i) q[4 * k + i] = (int8_t)(b >> (8 * i));
-        };
         auto larger = [&](float4 u) {
             m = max(m, max(max(magnitude(u.x), magnitude(u.y)), max(magnitude(u.z), magnitude(u.w))));
         };
@@ -58,11 +43,15 @@ __device__ __forceinline__ void quantize_rows(const Rows &a, int block, int bloc
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (i * TEAM + tid < end) v[i] = load(i * TEAM + tid);
+            if (i * TEAM + tid < end) v[i] = four_at(x + 4 * (i * TEAM + tid));
         }
+        // The up to three values behind the last four, a thread each.
+        const int rest = 4 * units + tid;
+        const float last = real && rest < a.K && tid < 3 ? x[rest] : 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) larger(v[i]);
-        for (int k = V * TEAM + tid; k < end; k += TEAM) larger(load(k));  // rows longer than the registers: read twice
+        m = max(m, magnitude(last));
+        for (int k = V * TEAM + tid; k < end; k += TEAM) larger(four_at(x + 4 * k));  // rows longer than the registers: read twice
 #pragma unroll
         for (int d = 32; d; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
         if constexpr (TEAM > 64) {
@@ -74,30 +63,23 @@ __device__ __forceinline__ void quantize_rows(const Rows &a, int block, int bloc
         const Scale s(m);
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (i * TEAM + tid < end) store(i * TEAM + tid, s.four(v[i]));
-        for (int k = V * TEAM + tid; k < end; k += TEAM) store(k, s.four(load(k)));
+            if (i * TEAM + tid < end) reinterpret_cast<word *>(q)[i * TEAM + tid] = s.four(v[i]);
+        for (int k = V * TEAM + tid; k < end; k += TEAM) reinterpret_cast<word *>(q)[k] = s.four(four_at(x + 4 * k));
+        if (real && rest < a.K && tid < 3) q[rest] = (int8_t)s.divided(last);
         if (real && tid == 0) a.scale[r] = s.value;
     }
 }
 
-template <int TEAM, int V, bool WIDE>
+template <int TEAM, int V>
 __global__ __launch_bounds__(TEAM) void quantize_kernel(Rows a) {
     __shared__ uint32_t most[2 * (TEAM / 64)];
-    quantize_rows<TEAM, TEAM, V, WIDE>(a, blockIdx.x, gridDim.x, most);
+    quantize_rows<TEAM, TEAM, V>(a, blockIdx.x, gridDim.x, most);
 }
 
 template <int TEAM, int V>
-int launch(bool wide, const Rows &a, hipStream_t s) {
-    const dim3 grid((unsigned)std::min(a.n_rows, (int64_t)1 << 20)), block(TEAM);
-    if (wide)
-        hipLaunchKernelGGL((quantize_kernel<TEAM, V, true>), grid, block, 0, s, a);
-    else
-        hipLaunchKernelGGL((quantize_kernel<TEAM, V, false>), grid, block, 0, s, a);
+int launch(const Rows &a, hipStream_t s) {
+    hipLaunchKernelGGL((quantize_kernel<TEAM, V>), dim3((unsigned)std::min(a.n_rows, (int64_t)1 << 20)), dim3(TEAM), 0, s, a);
     return (int)hipGetLastError();
-}
-
-bool wide_rows(const Rows &a) {
-    return !(a.K % 4 || a.x_stride % 4 || a.q_stride % 4 || (uintptr_t)a.x % 16 || (uintptr_t)a.q % 4);
 }
 
 constexpr int GROUP_THREADS = 1024, PER = PAIR_CHUNK / GROUP_THREADS;
@@ -211,7 +193,7 @@ __global__ __launch_bounds__(GROUP_THREADS, 8) void prepare_kernel(Pairs a, int 
     if ((int)blockIdx.x < chunks)
         count_pairs<ONE>(a, blockIdx.x, count, sums);
     else
-        quantize_rows<GROUP_THREADS, TEAM, V, true>(tokens, blockIdx.x - chunks, gridDim.x - chunks, (uint32_t *)count);
+        quantize_rows<GROUP_THREADS, TEAM, V>(tokens, blockIdx.x - chunks, gridDim.x - chunks, (uint32_t *)count);
 }
 
 template <int TEAM, int V>
@@ -254,16 +236,12 @@ __global__ __launch_bounds__(GROUP_THREADS) void place_kernel(Pairs a) {
 
 }  // namespace
 
-static int quantize_rows_of(const Rows &a, hipStream_t s) {
-    const bool wide = wide_rows(a);
-    if (a.K <= 1024) return launch<64, 4>(wide, a, s);
-    if (a.K <= 8192) return launch<256, 8>(wide, a, s);
-    return launch<1024, 4>(wide, a, s);
-}
-
 int i8::quantize(const float *x, int64_t K, int64_t n_rows, int64_t x_stride, int8_t *q, int64_t q_stride, float *scale,
                  hipStream_t s) {
-    return quantize_rows_of({x, (int)K, n_rows, x_stride, q, q_stride, scale}, s);
+    const Rows a = {x, (int)K, n_rows, x_stride, q, q_stride, scale};
+    if (K <= 1024) return launch<64, 4>(a, s);
+    if (K <= 8192) return launch<256, 8>(a, s);
+    return launch<1024, 4>(a, s);
 }
 
 int i8::group(const int32_t *ids, int64_t ids_stride, int n_pairs, int n_ids, int n_as, int per_slot, int bn,
@@ -271,19 +249,15 @@ int i8::group(const int32_t *ids, int64_t ids_stride, int n_pairs, int n_ids, in
               int64_t x_stride, int8_t *q, int64_t q_stride, float *scale, hipStream_t s) {
     const Pairs a = {ids, ids_stride, n_pairs, n_ids, n_as, per_slot, bn, to.col_src, to.col_dst, to.tiles, to.n_tiles,
                      to.counts, to.places, dst, dst_stride, nrows};
-    Rows tokens = {x, (int)K, x ? n_rows : 0, x_stride, q, q_stride, scale};
-    if (x && !wide_rows(tokens)) {
-        if (int e = quantize_rows_of(tokens, s)) return e;
-        tokens.n_rows = 0;
-    }
+    const Rows tokens = {x, (int)K, x ? n_rows : 0, x_stride, q, q_stride, scale};
     const int chunks = (n_pairs + PAIR_CHUNK - 1) / PAIR_CHUNK;
-    // Four float4 a thread: two workgroups a CU.
+    // Registers for two workgroups a CU: four float4 a thread, or two with what longer rows need beside them.
     if (K <= 1024)
         launch_prepare<64, 4>(a, chunks, tokens, s);
     else if (K <= 4096)
         launch_prepare<256, 4>(a, chunks, tokens, s);
     else
-        launch_prepare<1024, 4>(a, chunks, tokens, s);
+        launch_prepare<1024, 2>(a, chunks, tokens, s);
     const int e = (int)hipGetLastError();
     if (e || chunks == 1) return e;
     hipLaunchKernelGGL(place_kernel, dim3((unsigned)chunks), dim3(GROUP_THREADS), 0, s, a);

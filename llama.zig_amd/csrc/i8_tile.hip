@@ -382,11 +382,19 @@ TileForm i8::tile_form(int64_t nrows, int64_t ncols) {
     return TILE_64x64;
 }
 
-// By the mean number of an expert's columns.  Measured with 128 experts of 1536 x 2048, us: 16 columns 81 in 128 x 64, 87 in
-// 64 x 64; 64 108 in 128 x 64, 118 in 128 x 128; 128 140 in 256 x 256 (its half tiles), 144 in 128 x 64; 256 212 in
-// 256 x 256, 228 in 128 x 128.
-TileForm i8::tile_form_grouped(int64_t n_as, int64_t n_pairs) {
-    return n_pairs <= 64 * n_as ? TILE_128x64 : TILE_256x256;
+// By experts, whose last tiles are half full on the average.  The smallest where there are few tiles, as above; tall narrow
+// ones for experts with few columns; else 256 x 256 if rounds of them and their start and end, 15 us a tile, are few beside
+// the work.  Measured (weight rows x inner, pairs by experts), us:
+//   282 x 842, 1360 by 8: 6.0 in 64 x 64, 7.9 in 128 x 64, 9.6 in 128 x 128, 15.8 in 256 x 256
+//   2048 x 2048, 1024 by 8: 17.5, 15.7, 17.8, 21.2
+//   1536 x 2048, 8192 by 128: 116, 108, 117, 111; 16384: 174, 145, 141, 131; 32768: -, -, 209, 194
+//   2027 x 1209, 3921 by 23 (184 of 256 x 256): 34.1, 32.3, 29.9, 34.1;  1039 x 723, 33880 by 44: 98, 79, 64, 75
+TileForm i8::tile_form_grouped(int64_t K, int64_t nrows, int64_t n_as, int64_t n_pairs) {
+    const int64_t experts = std::min(n_pairs, n_as);
+    auto tiles = [&](int64_t m, int64_t n) { return (nrows + m - 1) / m * (n_pairs / n + experts / 2); };
+    if (tiles(128, 64) < 200) return TILE_64x64;
+    if (n_pairs <= 64 * experts || tiles(128, 128) < 400) return TILE_128x64;
+    return K >= 1024 && tiles(256, 256) >= 600 ? TILE_256x256 : TILE_128x128;
 }
 
 int i8::tile_columns(TileForm form) {

@@ -355,3 +355,35 @@ def test_pairs_in_several_chunks(n, e, k):
     out = torch.full((n, k, 33), np.nan, device="cuda")
     G.mul_mat_id_i8(w, ws, torch.from_numpy(x).cuda(), torch.from_numpy(ids).cuda(), out=out)
     _near(out, R.product_id(wn, wsn, q, s, ids))
+
+
+@pytest.mark.parametrize("rows,K,n,k,e", [(282, 842, 272, 5, 8), (2100, 130, 500, 2, 8), (300, 200, 3750, 4, 32), (4100, 1030, 1250, 4, 32),
+                                          (1540, 2061, 900, 8, 56)])
+def test_tiles_of_each_size_by_experts(rows, K, n, k, e):
+    """Some experts with few columns, some with many, and some pairs without one."""
+    r = np.random.RandomState(rows)
+    w, wn, ws, wsn = _experts(r, e, rows, K)
+    liked = r.rand(e) ** 2 + 0.01
+    ids = r.choice(e, (n, k), p=liked / liked.sum()).astype(np.int32)
+    ids[r.rand(n, k) < 0.02] = -1
+    x = r.randn(n, 1, K).astype(np.float32)
+    q, s = R.quantize(x)
+    out = torch.full((n, k, rows), np.nan, device="cuda")
+    G.mul_mat_id_i8(w, ws, torch.from_numpy(x).cuda(), torch.from_numpy(ids).cuda(), out=out)
+    _near(out, R.product_id(wn, wsn, q, s, ids))
+
+
+@pytest.mark.parametrize("K", [1, 2, 3, 4, 5, 7, 1021, 4099, 8193, 20002])
+@pytest.mark.parametrize("off", [0, 1, 2, 3])
+def test_quantized_rows_at_any_byte(K, off):
+    """Values from any multiple of four bytes, results to any byte, and nothing behind a row is written."""
+    r = np.random.RandomState(K)
+    n = 7
+    x = np.zeros((n, K + 9), np.float32)
+    x[:, off:off + K] = r.randn(n, K)
+    q, s = R.quantize(x[:, off:off + K])
+    xd = torch.from_numpy(x).cuda()
+    out = torch.full((n, K + 6), 99, dtype=torch.int8, device="cuda")
+    got, scale = G.quantize_i8(xd[:, off:off + K], out=out[:, off:off + K])
+    assert np.array_equal(got.cpu().numpy(), q) and np.array_equal(scale.cpu().numpy(), s)
+    assert (out[:, :off] == 99).all() and (out[:, off + K:] == 99).all()
