@@ -1,7 +1,7 @@
 // i8_few.hip -- the 8-bit product for few columns: what counts is that the
 // weights stream from memory without a pause.
 //
-// A workgroup of eight waves takes some weight rows, in blocks of 16, and 16 * NT
+// A workgroup of eight waves takes some weight rows, in blocks of 16, and up to 16 * NT
 // columns.  (Row block, step of 128 inner bytes) are its items; wave w takes
 // items w, w + 8, ..., each through a ring of its own in LDS that direct
 // global->LDS transfers fill DEPTH items ahead: no barrier, and the next row
@@ -83,7 +83,8 @@ __global__ __launch_bounds__(THREADS) void few_kernel(Few f) {
     const int m0 = blockIdx.x * f.rows, m1 = min(m0 + f.rows, a.nrows), nb = (m1 - m0 + 15) / 16;
     const int8_t *w = a.w;
     const float *w_scale = a.w_scale;
-    int first = 0, end = a.ncols;  // columns of this workgroup, or places among the expert's pairs
+    // Columns of this workgroup, or places among the expert's pairs.
+    int first = IDS ? 0 : blockIdx.y * f.columns, end = IDS ? 0 : min(first + f.columns, a.ncols);
     int mine = 0;                  // IDS: the places of this thread's pair ...
     bool is = false;
     if constexpr (IDS) {
@@ -154,7 +155,7 @@ __global__ __launch_bounds__(THREADS) void few_kernel(Few f) {
                 dst[mine - first] = tid;
             }
         } else {
-            if (tid < n) src[tid] = dst[tid] = tid;
+            if (tid < n) src[tid] = dst[tid] = first + tid;
         }
         for (int i = tid; i < nb * NT * 256; i += THREADS) sums[i] = 0;
         __syncthreads();
@@ -366,12 +367,22 @@ int launch(const Few &f, dim3 grid, int bytes, hipStream_t s) {
 
 }  // namespace
 
-// Up to 32 columns.  Two workgroups a CU, two items ahead, where both fit and there are 16 rows for each: one's start
+// Up to 32 columns: two workgroups a CU, two items ahead, where both fit and there are 16 rows for each: one's start
 // overlaps the other's work (14336 x 4096 by one column 13.6 us, 14.2 with one a CU and four ahead); else one with as many
 // items ahead as fit.  At least 8 rows, of the 16 that an instruction takes: fewer do not make a small product faster.
+//
+// More columns, 32 to a workgroup, where one round of workgroups takes them all: eight shares of K in each instead of a
+// tile's long way along it on few CUs (1024 x 4096 by 64 columns 5.8 us, 10.2 in tiles; 269 x 16070 by 469 17.9, 30.5;
+// 4096 x 4096 by 64, 32 rows a workgroup, 9.6, 10.8; with two rounds 524 x 4915 by 450 takes 13.7, 12.1 in tiles).
 FewPlan i8::few_plan(bool f32, int64_t K, int64_t nrows, int64_t ncols) {
     FewPlan p = {};
-    if (ncols < 1 || ncols > 32) return p;
+    if (ncols < 1 || (f32 && ncols > 32)) return p;
+    if (ncols > 32) {
+        p.mode = THROUGH, p.nt = 2, p.depth = 3, p.columns = 32;
+        for (p.rows = 16; p.rows <= 32; p.rows += 16)
+            if ((nrows + p.rows - 1) / p.rows * ((ncols + 31) / 32) <= 256 && fits(p, K, LDS)) break;
+        return p;
+    }
     p.nt = ncols <= 16 ? 1 : 2;
     p.columns = (int)ncols;
     p.mode = f32 ? QUANTIZE : RESIDENT;
@@ -417,7 +428,7 @@ FewPlan i8::few_pairs_plan(bool f32, int64_t K, int64_t nrows, int64_t n_as, int
 }
 
 int i8::few_product(const Product &p, const FewPlan &plan, hipStream_t s) {
-    const dim3 grid((unsigned)((p.nrows + plan.rows - 1) / plan.rows), 1);
+    const dim3 grid((unsigned)((p.nrows + plan.rows - 1) / plan.rows), (unsigned)((p.ncols + plan.columns - 1) / plan.columns));
     const Few f = arguments(p, plan);
 #define FEW(NT, DEPTH, MODE) \
     if (plan.nt == NT && plan.depth == DEPTH && plan.mode == MODE) return launch<NT, DEPTH, MODE, false>(f, grid, plan.bytes, s)

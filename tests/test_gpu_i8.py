@@ -387,3 +387,21 @@ def test_quantized_rows_at_any_byte(K, off):
     got, scale = G.quantize_i8(xd[:, off:off + K], out=out[:, off:off + K])
     assert np.array_equal(got.cpu().numpy(), q) and np.array_equal(scale.cpu().numpy(), s)
     assert (out[:, :off] == 99).all() and (out[:, off + K:] == 99).all()
+
+
+@pytest.mark.parametrize("rows,K,n", [(269, 16070, 469), (16, 131071, 33), (4096, 129, 64), (4090, 2061, 37), (1, 300, 5000), (33, 4097, 2700),
+                                      (1000, 20001, 128)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_more_columns_than_one_workgroup_takes(rows, K, n, f32):
+    """Few weight rows or few columns, so that the inner axis is shared by waves."""
+    r = np.random.RandomState(n)
+    w, wn = _rows(r, rows, K)
+    ws, wsn = _scales(r, rows)
+    x = r.randn(n, K).astype(np.float32)
+    q, s = R.quantize(x)
+    xd = torch.from_numpy(x).cuda()
+    out = torch.full((n, rows + 3), np.nan, device="cuda")
+    x8, scale = (xd, None) if f32 else G.quantize_i8(xd)
+    got = G.mul_mat_i8(w, ws, x8, scale, out=out[:, 1:1 + rows])
+    _near(got, R.product(wn, wsn, q, s))
+    assert out[:, 0].isnan().all() and out[:, 1 + rows:].isnan().all()
