@@ -76,7 +76,7 @@ int hip_qmm_quantize_i8(const float *x, int64_t K, int64_t n_rows, int64_t x_str
  * rows must be readable but do not matter.  K 1 to 131071, nrows and ncols at
  * most 2^22, their product at most 2^38.  The workspace is scratch, 256-byte aligned: its contents do
  * not matter before the call, and it serves one call at a time.  Its size is at
- * most ncols * (K + 131) + 512.
+ * most ncols * (K + 131) + 512, and 0 for an int8 x.
  */
 size_t hip_qmm_mul_mat_i8_workspace_size(int64_t K, int64_t nrows, int64_t ncols, int quantized);
 int hip_qmm_mul_mat_i8(const int8_t *w, const float *w_scale, int64_t K, int64_t nrows, int64_t w_stride,

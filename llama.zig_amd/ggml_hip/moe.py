@@ -193,8 +193,8 @@ def mul_mat_i8(w: torch.Tensor, w_scale: torch.Tensor, x: torch.Tensor, x_scale=
     if n == 0:
         return out
     if workspace is None:
-        # Of many tokens the header's bound: cheaper than to ask.
-        have = n * (K + 131) + 512 if xp is None and n > 32 else L.hip_qmm_mul_mat_i8_workspace_size(K, rows, n, xp is not None)
+        # What the header promises of int8 tokens and of many: cheaper than to ask.
+        have = 0 if xp is not None else n * (K + 131) + 512 if n > 32 else L.hip_qmm_mul_mat_i8_workspace_size(K, rows, n, 0)
         wp = None
         if have:
             workspace = w_scale.new_empty(have, dtype=torch.uint8)
