@@ -12,6 +12,12 @@
 // The columns are in LDS whole (quantized there, if they come as f32), or come
 // with the weights through the ring where they do not fit.  Their transfers are
 // issued before the weights', and so are waited for without them.
+//
+// HBM bound: 14336 x 4096 by 24 columns take 14.2 us (4.2 TB/s of weights; a copy
+// reaches 5.1), 4096 x 14336 by one 13.2 to 15; 48 tokens by 8 of 128 experts of
+// 2048 x 768, f32, 36 to 45 (4.4 to 5.4 TB/s of the weights asked for).  What is
+// short of the copy's rate is the start of a launch, with no transfer under way
+// until the columns' rows are known, and its end.
 #include <math.h>
 
 #include <algorithm>

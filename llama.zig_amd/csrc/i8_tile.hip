@@ -9,6 +9,12 @@
 // is contracted, whose operands are in registers by then, so that the stage's
 // places are free.  The transfers into them are issued among the matrix
 // instructions from there on: all at once they would wait for each other.
+//
+// 14336 x 4096 by 4096 columns, 256 x 256 tiles: 228 us, 2.11 POP/s (a library's
+// product of these sizes 226, of 8192^3 2.44 POP/s).  A tile's stages run at 78 % of
+// the matrix cycles of a clock that falls to 1.63 to 1.7 GHz under them; its first
+// transfers take 2.5 us and its results 9 to 11 of 62.  Small tiles (5003 x 2720 by 333, 128 x 64:
+// 14.5 us) are bound by reading operands from L2, 11 to 14 TB/s in all.
 #include <algorithm>
 
 #include "i8.h"

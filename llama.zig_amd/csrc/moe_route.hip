@@ -9,6 +9,11 @@
 // it.  Else f32 scores are tried: their errors are below SURE, so two that are
 // further apart have the right order, and only a token of which some that matter
 // are not is done again in f64 (a few in a thousand).
+//
+// Bound by the issue of instructions, 670 vector and 450 scalar ones a token of
+// 256 experts in groups: 8192 such tokens take 16.5 us, where their logits could
+// be read in 1.8, 61 tokens 6.2; one of 128 experts 3.4.  Several tokens a wave,
+// one after the other, took longer.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
