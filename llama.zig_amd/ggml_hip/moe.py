@@ -80,18 +80,22 @@ def _rows3(t, shape, dtype, name, device):
 
 
 def _i8_rows(t, stride, name):
-    """The stride of 8-bit rows as the products take them; the last one's chunk of 16 bytes may end behind the row, but
-    not behind the tensor's memory."""
-    n = t.shape[-1]
-    if not t.numel():
-        return stride
+    """The stride of 8-bit rows, 2-D or 3-D, as the products take them; the last one's chunk of 16 bytes may end behind the
+    row, but not behind the tensor's memory."""
+    size = t.shape
+    n = size[-1]
     if n % 16:
-        if t.numel() == n:  # one row
-            stride = (n + 15) // 16 * 16
-        last = t.storage_offset() + sum((s - 1) * d for s, d in zip(t.shape[:-1], t.stride()[:-1]))
-        if last + (n + 15) // 16 * 16 > t.untyped_storage().nbytes():
+        if not t.numel():
+            return stride
+        whole = (n + 15) // 16 * 16
+        last = t.storage_offset() + (size[-2] - 1) * stride
+        if len(size) == 3:
+            last += (size[0] - 1) * t.stride(0)
+        if last + whole > t.untyped_storage().nbytes():
             raise HipQmmError(f"{name}'s last row must end in memory of the tensor's up to 16 bytes")
-    if stride % 16 or t.data_ptr() % 16:
+        if t.numel() == n:  # one row
+            stride = whole
+    if (stride % 16 or t.data_ptr() % 16) and t.numel():
         raise HipQmmError(f"{name}'s rows must be 16-byte aligned (quantize_i8 lays them so)")
     return stride
 
