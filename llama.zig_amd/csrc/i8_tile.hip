@@ -388,6 +388,9 @@ TileForm i8::tile_form(int64_t nrows, int64_t ncols) {
     return TILE_64x64;
 }
 
+// (256 x 128, two a CU: 8192 x 768 by 8192 89 for 97 in 256 x 256, 8192 x 1200 153 for 133, 33880 pairs by 44 experts of
+// 1039 x 723 13 us more than 128 x 128: not taken.)
+//
 // By experts, whose last tiles are half full on the average.  The smallest where there are few tiles, as above; tall narrow
 // ones for experts with few columns; else 256 x 256 if rounds of them and their start and end, 15 us a tile, are few beside
 // the work.  Measured (weight rows x inner, pairs by experts), us:

@@ -358,6 +358,7 @@ def test_pairs_in_several_chunks(n, e, k):
 
 
 @pytest.mark.parametrize("rows,K,n,k,e", [(282, 842, 272, 5, 8), (2100, 130, 500, 2, 8), (300, 200, 3750, 4, 32), (4100, 1030, 1250, 4, 32),
+                                          (4100, 1030, 1400, 4, 32), (4100, 65, 1400, 4, 32), (4100, 1600, 1400, 4, 32), (4100, 2061, 1400, 4, 32),
                                           (1540, 2061, 900, 8, 56)])
 def test_tiles_of_each_size_by_experts(rows, K, n, k, e):
     """Some experts with few columns, some with many, and some pairs without one."""
@@ -405,3 +406,20 @@ def test_more_columns_than_one_workgroup_takes(rows, K, n, f32):
     got = G.mul_mat_i8(w, ws, x8, scale, out=out[:, 1:1 + rows])
     _near(got, R.product(wn, wsn, q, s))
     assert out[:, 0].isnan().all() and out[:, 1 + rows:].isnan().all()
+
+
+@pytest.mark.parametrize("K", [1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 191, 200, 700])
+def test_many_tiles_along_a_short_axis(K):
+    """Checked where the rows and columns of tiles begin and end."""
+    r = np.random.RandomState(K)
+    rows, n = 5003, 7710
+    w, wn = _rows(r, rows, K, full=True)
+    ws, wsn = _scales(r, rows)
+    x, xn = _rows(r, n, K)
+    xs, xsn = _scales(r, n)
+    got = G.mul_mat_i8(w, ws, x, xs)
+    assert got.isfinite().all()
+    m = np.unique(np.concatenate([np.arange(b, b + 3) for b in range(0, rows - 2, 125)] + [np.arange(4864, rows)]))
+    c = np.unique(np.concatenate([np.arange(b, b + 3) for b in range(0, n - 2, 127)] + [np.arange(7680, n)]))
+    _near(got[torch.from_numpy(c).cuda()][:, torch.from_numpy(m).cuda()],
+          R.product(wn[m], wsn[m], np.ascontiguousarray(xn[c]), xsn[c]))
