@@ -148,7 +148,13 @@ __device__ __forceinline__ float inverse(float x) { return __builtin_amdgcn_rcpf
 // Two f32 scores that differ by more than SURE times the larger of 1 and their size have the order of the exact ones.
 // p is below 1 and off by the exponential (its argument's rounding, |l| 2^-24 relative, matters as x e^-x does, and its
 // own, 2^-23), the sum of at most 1024 (sums of 16 and then 6 more levels, 22 * 2^-24) and the reciprocal (2^-23): under
-// 2^-19; adding the bias is off by half a step of the sum.  A group's score is two of them.
+// 2^-19; adding the bias is off by half a step of the sum, 2^-24 of its size.
+//
+// A group's score is the sum of two of them and off by what both are and by half a step of its own.  Its two may be
+// large and of opposite signs, and it then small: its error goes by their size, not by its own.  With the larger of 1 and
+// their magnitudes as a unit it is below 2 * 2^-19 (p) + 2 * 2^-24 (biases) + 2 * 2^-24 (sum), little over half of SURE.
+// So a group comes before another for sure if its score less SURE units is above the other's and SURE of its own (whose
+// roundings are 2 * 2^-24 each).
 constexpr float SURE = 0x1p-17f;
 
 template <typename S>
@@ -252,10 +258,15 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const float (&l)[V], 
             __builtin_amdgcn_wave_barrier();
         }
         T mine = first;
-        if (sums && first != Key<S>::HIDDEN) {
-            S x = score_of<S>(first), y = score_of<S>(second);
-            if (!a.bias) x = p_of(a, m, (float)x), y = p_of(a, m, (float)y);
-            mine = key_of<S>(second != Key<S>::HIDDEN ? x + y : x);
+        float unit = 1.0f;  // of f32 scores' errors
+        if (first != Key<S>::HIDDEN) {
+            S x = score_of<S>(first), y = 0;
+            if (sums) {
+                if (second != Key<S>::HIDDEN) y = score_of<S>(second);
+                if (!a.bias) x = p_of(a, m, (float)x), y = second != Key<S>::HIDDEN ? p_of(a, m, (float)y) : y;
+                mine = key_of<S>(x + y);
+            }
+            unit = fmaxf(1.0f, fmaxf(fabsf((float)x), fabsf((float)y)));
         }
         if (group >= a.n_groups) mine = Key<S>::HIDDEN;
         int before = 0;  // groups that come before this lane's
@@ -265,9 +276,11 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const float (&l)[V], 
         }
         const bool kept = group < a.n_groups && before < a.n_keep;
         if constexpr (!EXACT) {
-            // The worst that is kept and the best that is not.
-            const T out = largest(kept ? Key<S>::HIDDEN : mine), in = ~largest(kept ? ~mine : Key<S>::HIDDEN);
-            if (out != Key<S>::HIDDEN && !apart(score_of<S>(in), score_of<S>(out))) sure = false;
+            // The worst that is kept at its lowest, and the best that is not at its highest.
+            const float score = score_of<S>(mine), reach = SURE * unit;
+            const T end = mine == Key<S>::HIDDEN ? mine : key_of<S>(kept ? score - reach : score + reach);
+            const T out = largest(kept ? Key<S>::HIDDEN : end), in = ~largest(kept ? ~end : Key<S>::HIDDEN);
+            if (out != Key<S>::HIDDEN && in <= out) sure = false;
         }
         if (aligned) {
 #pragma unroll

@@ -136,3 +136,41 @@ def test_many_tokens():
 def test_no_tokens():
     ids, w = G.route(torch.empty(0, 16, device="cuda"), 4)
     assert ids.shape == w.shape == (0, 4)
+
+
+def _balanced_groups(gating, n, groups, size, large, seed):
+    """Logits and a bias for which each group's two best are `large` above and below, and the sums of two nearly the
+    same for all groups: f32 scores of that size do not tell them apart."""
+    r = np.random.RandomState(seed)
+    p = r.uniform(0.1, 0.9, (n, groups, 1))
+    near = r.choice([-1, 1], (n, groups, 1)) * 10 ** r.uniform(-6, -4, (n, groups, 1))
+    rest = np.full((n, groups, size - 2), 0.01)
+    p = np.concatenate([p, 1 + near - p, rest], -1)
+    logits = {"softmax": np.log, "sigmoid": lambda x: np.log(x / (1 - x)), "softmax_chosen": lambda x: x}[gating](p)
+    bias = np.full((groups, size), -3.0 * large)
+    bias[:, 0], bias[:, 1] = large, -large
+    return logits.reshape(n, -1).astype(np.float32), bias.ravel().astype(np.float32)
+
+
+@pytest.mark.parametrize("gating", ["softmax", "sigmoid", "softmax_chosen"])
+@pytest.mark.parametrize("large", [30, 300, 1000, 4096, 1e5])
+@pytest.mark.parametrize("groups,size,keep", [(2, 2, 1), (8, 2, 4), (4, 3, 2), (8, 32, 4)])
+def test_groups_whose_two_best_cancel(gating, large, groups, size, keep):
+    logits, bias = _balanced_groups(gating, 500, groups, size, large, groups)
+    _check(logits, keep, gating=gating, bias=bias, groups=groups, keep=keep, top=2)
+
+
+@pytest.mark.parametrize("logits,large", [([0.47, 3.82, 2.17, 0.83], 1024), ([-0.6627474, -1.0630597, -1.5472649, -0.31719202], 300)])
+def test_the_better_of_two_groups(logits, large):
+    _check(np.array([logits], np.float32), 1, gating="sigmoid", bias=np.array([large, -large] * 2, np.float32), groups=2, top=2)
+
+
+@pytest.mark.parametrize("gating", ["softmax", "sigmoid", "softmax_chosen"])
+def test_groups_far_below_the_others(gating):
+    """Scores of a mask's size beside ordinary ones, and as many of them kept as there have to be."""
+    logits = _logits(40, 64, 7)
+    bias = (np.random.RandomState(3).randn(64) * 0.2).astype(np.float32)
+    bias[16:40] = -1e9
+    bias[40:44] = 1e9, -1e9, 1e4, -1e4
+    for keep in (1, 3, 5, 7, 8):
+        _check(logits, 6, gating=gating, bias=bias, groups=8, keep=keep, top=2)
