@@ -265,6 +265,7 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const float (&l)[V], 
                 if (second != Key<S>::HIDDEN) y = score_of<S>(second);
                 if (!a.bias) x = p_of(a, m, (float)x), y = second != Key<S>::HIDDEN ? p_of(a, m, (float)y) : y;
                 mine = key_of<S>(x + y);
+                sure = x + y - (x + y) == 0;  // else beyond f32: below it not to be taken for hidden
             }
             unit = fmaxf(1.0f, fmaxf(fabsf((float)x), fabsf((float)y)));
         }
@@ -280,7 +281,7 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const float (&l)[V], 
             const float score = score_of<S>(mine), reach = SURE * unit;
             const T end = mine == Key<S>::HIDDEN ? mine : key_of<S>(kept ? score - reach : score + reach);
             const T out = largest(kept ? Key<S>::HIDDEN : end), in = ~largest(kept ? ~end : Key<S>::HIDDEN);
-            if (out != Key<S>::HIDDEN && in <= out) sure = false;
+            sure = __all(sure) && (out == Key<S>::HIDDEN || in > out);
         }
         if (aligned) {
 #pragma unroll

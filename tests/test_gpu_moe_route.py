@@ -174,3 +174,29 @@ def test_groups_far_below_the_others(gating):
     bias[40:44] = 1e9, -1e9, 1e4, -1e4
     for keep in (1, 3, 5, 7, 8):
         _check(logits, 6, gating=gating, bias=bias, groups=8, keep=keep, top=2)
+
+
+@pytest.mark.parametrize("gating", ["softmax", "sigmoid", "softmax_chosen"])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("groups,size", [(2, 8), (4, 16), (6, 6), (8, 32)])
+def test_sums_beyond_f32_are_not_hidden(gating, biased, groups, size):
+    """Groups whose two best sum to less than f32 holds come before those without an expert."""
+    least = np.finfo(np.float32).min
+    logits = _logits(7, groups * size, 5).reshape(7, groups, size)
+    logits[:6, 0] = -np.inf
+    logits[1:, 1:] = least
+    logits[2, -1] = -0.9e38
+    logits[3, 1:, :2] = least / 2          # a sum that is just held
+    logits[4, 1:, 1:] = -np.inf            # one expert a group
+    logits[5, 1:] = np.abs(logits[5, 1:])  # and above what f32 holds
+    bias = None
+    if biased:
+        bias = np.full((groups, size), -3e38, np.float32)
+        bias[1, 1] = -2e38
+        if gating == "softmax_chosen":
+            logits[np.isfinite(logits)] /= 8  # some scores themselves are beyond f32, others their sums alone
+        bias = bias.ravel()
+    for keep in range(1, groups):
+        ids, _ = _check(logits.reshape(7, -1), 2, gating=gating, bias=bias, groups=groups, keep=keep, top=2)
+        if gating == "softmax_chosen":
+            assert (ids[:6, 0] >= size).all()
