@@ -93,10 +93,12 @@ struct Scale {
 };
 
 // A sum times its two scales: three f32 roundings (the sum's and two products'), of mantissas alone, so that no
-// product leaves the range of f32 unless the result does.
+// product leaves the range of f32 unless the result does.  The last product is exact in f64 and rounded once, to the
+// fewer bits that a subnormal result has too (f32 would round it to 24 bits before).
 __device__ __forceinline__ float scaled(int sum, float x_scale, float w_scale) {
-    return ldexpf((float)sum * __builtin_amdgcn_frexp_mantf(x_scale) * __builtin_amdgcn_frexp_mantf(w_scale),
-                  __builtin_amdgcn_frexp_expf(x_scale) + __builtin_amdgcn_frexp_expf(w_scale));
+    const float product = (float)sum * __builtin_amdgcn_frexp_mantf(x_scale);
+    return (float)ldexp((double)product * (double)__builtin_amdgcn_frexp_mantf(w_scale),
+                        __builtin_amdgcn_frexp_expf(x_scale) + __builtin_amdgcn_frexp_expf(w_scale));
 }
 
 // Scales with which the products may be taken as they are, with the same bits.

@@ -284,8 +284,10 @@ __device__ __forceinline__ void tile(const Product &a, uint8_t *ring, const int8
                 for (int u = 0; u < AT_ONCE; ++u) {
                     if (first + c0 + k + u * COLS + lane / CHUNKS >= end) continue;
                     float *o = out + (int64_t)row[u] * a.dst_stride;
-                    const v4f v = {scaled(s[u][0], xs[u], ws.x), scaled(s[u][1], xs[u], ws.y), scaled(s[u][2], xs[u], ws.z),
-                                   scaled(s[u][3], xs[u], ws.w)};
+                    const v4f v = plain ? (v4f){(float)s[u][0] * xs[u] * ws.x, (float)s[u][1] * xs[u] * ws.y,
+                                                (float)s[u][2] * xs[u] * ws.z, (float)s[u][3] * xs[u] * ws.w}
+                                        : (v4f){scaled(s[u][0], xs[u], ws.x), scaled(s[u][1], xs[u], ws.y),
+                                                scaled(s[u][2], xs[u], ws.z), scaled(s[u][3], xs[u], ws.w)};
                     if (left >= 4) {
                         *reinterpret_cast<v4f *>(o) = v;
                     } else {

@@ -423,3 +423,30 @@ def test_many_tiles_along_a_short_axis(K):
     c = np.unique(np.concatenate([np.arange(b, b + 3) for b in range(0, n - 2, 127)] + [np.arange(7680, n)]))
     _near(got[torch.from_numpy(c).cuda()][:, torch.from_numpy(m).cuda()],
           R.product(wn[m], wsn[m], np.ascontiguousarray(xn[c]), xsn[c]))
+
+
+def _rounded_thrice(w, w_scale, q, scale):
+    """The definition's bits: the sum to f32, the first product to 24 bits of any exponent, the second to f32."""
+    acc = (q.astype(np.float64) @ w.astype(np.float64).T).astype(np.float32).astype(np.float64)
+    mantissa, exponent = np.frexp(acc * scale.astype(np.float64)[:, None])  # products of two f32 are exact in f64
+    with np.errstate(all="ignore"):
+        return (np.ldexp(mantissa.astype(np.float32).astype(np.float64), exponent) * w_scale.astype(np.float64)).astype(np.float32)
+
+
+@pytest.mark.parametrize("n", [1, 3, 20, 60, 400])
+@pytest.mark.parametrize("w_power,x_power", [(-70, -68), (-140, 0), (0, -143), (-100, -47), (100, -110), (3, 5), (110, 6)])
+def test_bits_of_results(n, w_power, x_power):
+    """Subnormal results among them: of the fewer bits that they have, rounded once."""
+    r = np.random.RandomState(n)
+    rows, K = 300, 90
+    w, wn = _rows(r, rows, K)
+    x, xn = _rows(r, n, K)
+    wsn = np.ldexp(r.rand(rows) + 0.5, w_power).astype(np.float32)
+    xsn = np.ldexp(r.rand(n) + 0.5, x_power).astype(np.float32)
+    ws, xs = torch.from_numpy(wsn).cuda(), torch.from_numpy(xsn).cuda()
+    want = _rounded_thrice(wn, wsn, xn, xsn)
+    got = G.mul_mat_i8(w, ws, x, xs).cpu().numpy()
+    assert np.array_equal(got, want), (np.argwhere(got != want)[:3], (got != want).sum())
+    ids = torch.zeros(n, 2, dtype=torch.int32, device="cuda")
+    by_experts = G.mul_mat_id_i8(w[None], ws[None], x[:, None], ids, xs[:, None]).cpu().numpy()
+    assert np.array_equal(by_experts[:, 0], want) and np.array_equal(by_experts[:, 1], want)
