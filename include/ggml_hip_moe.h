@@ -8,9 +8,9 @@
  * Conventions are those of ggml_hip_qmm.h: device pointers, activations f32,
  * asynchronous on `stream`, no allocation, scratch from the caller, 0 or a
  * hipError_t back (hipErrorInvalidValue = 1 for what an entry does not take,
- * before anything is launched).  Strides are in elements; nothing that is
- * written overlaps what is read, but where a comment allows it.  All results
- * are deterministic.
+ * before anything is launched).  Strides are in elements, and f32 and int32
+ * tensors aligned to 4 bytes; nothing that is written overlaps what is read, but
+ * where a comment allows it.  All results are deterministic.
  */
 #ifndef GGML_HIP_MOE_H
 #define GGML_HIP_MOE_H

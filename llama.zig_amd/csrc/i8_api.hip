@@ -52,6 +52,9 @@ bool operand_ok(const void *p, int64_t stride, int64_t K, bool bytes) {
     return bytes ? !((uintptr_t)p % 16 || stride % 16) : !((uintptr_t)p % 4);
 }
 
+// Tensors of 4-byte values.
+bool words_ok(const void *p) { return p && !((uintptr_t)p % 4); }
+
 bool workspace_ok(const void *ws, size_t have, size_t need) {
     return need == 0 || (ws && !((uintptr_t)ws % 256) && have >= need);
 }
@@ -76,8 +79,8 @@ extern "C" int hip_qmm_mul_mat_i8(const int8_t *w, const float *w_scale, int64_t
     if (!sizes_ok(K, nrows) || ncols < 0 || ncols > MAX_ROWS) return (int)hipErrorInvalidValue;
     if (ncols == 0) return 0;
     if (nrows > MAX_RESULTS / ncols) return (int)hipErrorInvalidValue;
-    if (!w_scale || !dst || dst_stride < nrows || dst_stride > MAX_STRIDE || !operand_ok(w, w_stride, K, true) ||
-        !operand_ok(x, x_stride, K, x_scale != nullptr) ||
+    if (!words_ok(w_scale) || !words_ok(dst) || (x_scale && !words_ok(x_scale)) || dst_stride < nrows ||
+        dst_stride > MAX_STRIDE || !operand_ok(w, w_stride, K, true) || !operand_ok(x, x_stride, K, x_scale != nullptr) ||
         !workspace_ok(workspace, workspace_size, hip_qmm_mul_mat_i8_workspace_size(K, nrows, ncols, x_scale != nullptr)))
         return (int)hipErrorInvalidValue;
     hipStream_t s = (hipStream_t)stream;
@@ -122,7 +125,8 @@ extern "C" int hip_qmm_mul_mat_id_i8(const int8_t *w, const float *w_scale, int6
     if (n_tokens == 0 || n_ids == 0) return 0;
     if (nrows > MAX_RESULTS / (n_tokens * n_ids)) return (int)hipErrorInvalidValue;
     const bool quantized = x_scale != nullptr;
-    if (!w_scale || !dst || !ids || ids_stride < n_ids || ids_stride > MAX_STRIDE || dst_stride < nrows ||
+    if (!words_ok(w_scale) || !words_ok(dst) || !words_ok(ids) || (quantized && !words_ok(x_scale)) || ids_stride < n_ids ||
+        ids_stride > MAX_STRIDE || dst_stride < nrows ||
         dst_stride > MAX_STRIDE || !operand_ok(w, w_stride, K, true) || expert_stride % 16 ||
         expert_stride < (nrows - 1) * w_stride + K || expert_stride > MAX_STRIDE ||
         !operand_ok(x, x_stride, K, quantized) ||

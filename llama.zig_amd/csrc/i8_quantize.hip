@@ -270,7 +270,8 @@ extern "C" int hip_qmm_quantize_i8(const float *x, int64_t K, int64_t n_rows, in
                                    int64_t q_stride, float *scale, void *stream) {
     if (K < 1 || K > MAX_K || n_rows < 0 || n_rows > (1 << 24)) return (int)hipErrorInvalidValue;
     if (n_rows == 0) return 0;
-    if (!x || !q || !scale || x_stride < K || q_stride < K || x_stride > MAX_STRIDE || q_stride > MAX_STRIDE)
+    if (!x || !q || !scale || ((uintptr_t)x | (uintptr_t)scale) % 4 || x_stride < K || q_stride < K ||
+        x_stride > MAX_STRIDE || q_stride > MAX_STRIDE)
         return (int)hipErrorInvalidValue;
     return quantize(x, K, n_rows, x_stride, q, q_stride, scale, (hipStream_t)stream);
 }

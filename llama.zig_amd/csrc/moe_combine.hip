@@ -80,6 +80,8 @@ extern "C" int hip_qmm_moe_combine(const float *y, int64_t n_tokens, int64_t n_i
     if (n_tokens < 0 || n_tokens > INT32_MAX || n_ids < 0 || n_ids > 65535 || nrows < 0 || nrows > INT32_MAX)
         return (int)hipErrorInvalidValue;
     if (n_tokens == 0 || nrows == 0) return 0;
+    if (((uintptr_t)y | (uintptr_t)weights | (uintptr_t)ids | (uintptr_t)add | (uintptr_t)dst) % 4)
+        return (int)hipErrorInvalidValue;
     if (!dst || dst_stride < nrows || dst_stride > lim || (add && (add_stride < nrows || add_stride > lim)))
         return (int)hipErrorInvalidValue;
     if (n_ids > 0 && (!y || !weights || y_token_stride < 0 || y_row_stride < 0 || y_token_stride > lim ||

@@ -437,7 +437,8 @@ extern "C" int hip_qmm_moe_route(const float *logits, int64_t n_tokens, int64_t 
         !isfinite(scale))
         return (int)hipErrorInvalidValue;
     if (n_tokens == 0) return 0;
-    if (!logits || !ids || !weights || logits_stride < n_experts || ids_stride < k || weights_stride < k ||
+    if (!logits || !ids || !weights || ((uintptr_t)logits | (uintptr_t)bias | (uintptr_t)ids | (uintptr_t)weights) % 4 ||
+        logits_stride < n_experts || ids_stride < k || weights_stride < k ||
         logits_stride > lim || ids_stride > lim || weights_stride > lim)
         return (int)hipErrorInvalidValue;
     const RouteArgs a = {logits, bias, logits_stride, ids_stride, weights_stride, ids, weights, (int)n_tokens,

@@ -121,3 +121,12 @@ def test_python_refusals_without_a_gpu():
                  lambda: G.mul_mat_id_i8(b[None], f[:1, :2], f[:, None], i), lambda: G.combine(f[:, None], f[:, :1])):
         with pytest.raises(G.HipQmmError):
             call()
+
+
+@pytest.mark.parametrize("call,names", [(_route, ("logits", "bias", "ids", "w")), (_quantize, ("x", "scale")),
+                                        (_product, ("ws", "xs", "dst")), (_by_experts, ("ws", "xs", "ids", "dst")),
+                                        (_combine, ("y", "w", "ids", "add", "dst"))])
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_tensors_at_odd_bytes(call, names, off):
+    for name in names:
+        assert call(**{name: P + off}) == BAD, name
