@@ -223,7 +223,9 @@ def mul_mat_id_i8(w: torch.Tensor, w_scale: torch.Tensor, x: torch.Tensor, ids: 
     e, rows, K = size
     n, ne11, _ = xsize
     n_ids = isize[1]
-    ws = _i8_rows(w, _rows(w, size, _I8, "w", device), "w")
+    ws = _rows(w, size, _I8, "w", device)
+    # One row an expert: what lies between two is the experts' stride (w[:, None]'s own is the row's length).
+    ws = _i8_rows(w, w.stride(0) if rows == 1 and e > 1 else ws, "w")
     es = w.stride(0) if e > 1 else rows * ws
     sp = _flat(w_scale, e * rows, _F32, "w_scale", device)
     if x_scale is None:

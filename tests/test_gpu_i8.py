@@ -450,3 +450,15 @@ def test_bits_of_results(n, w_power, x_power):
     ids = torch.zeros(n, 2, dtype=torch.int32, device="cuda")
     by_experts = G.mul_mat_id_i8(w[None], ws[None], x[:, None], ids, xs[:, None]).cpu().numpy()
     assert np.array_equal(by_experts[:, 0], want) and np.array_equal(by_experts[:, 1], want)
+
+
+@pytest.mark.parametrize("n", [1, 30, 700])
+def test_one_row_an_expert(n):
+    r = np.random.RandomState(n)
+    e, k, K = 6, 2, 90
+    w, wn = _rows(r, e, K)
+    ws, wsn = _scales(r, e, 1)
+    ids = r.randint(-1, e, (n, k)).astype(np.int32)
+    x = r.randn(n, 1, K).astype(np.float32)
+    got = G.mul_mat_id_i8(w[:, None], ws, torch.from_numpy(x).cuda(), torch.from_numpy(ids).cuda())
+    _near(got, R.product_id(wn[:, None], wsn, *R.quantize(x), ids))

@@ -187,3 +187,15 @@ def test_unknown_gating(library):
     with pytest.raises(G.HipQmmError):
         G.route(On(_t(2, 8)), 0)
     assert not library.calls
+
+
+def test_one_row_an_expert(library):
+    """Rows of quantize_i8 as weights of experts with one row each, by indexing: 16-byte aligned and as far apart."""
+    ids, x = On(_t(3, 2, dtype=I32)), On(_t(3, 1, 20))
+    for w in (_rows(4, 32)[:, :20][:, None], _rows(4, 1, 32)[..., :20], _rows(4, 5, 32)[:, 2:3, :20]):
+        assert G.mul_mat_id_i8(On(w), On(_t(4, 1)), x, ids).shape == (3, 2, 1)
+    assert len(library.calls) == 3
+    for w in (_rows(4, 20)[:, None], _rows(4, 40)[:, :20][:, None]):
+        with pytest.raises(G.HipQmmError):
+            G.mul_mat_id_i8(On(w), On(_t(4, 1)), x, ids)
+    assert len(library.calls) == 3
