@@ -148,7 +148,7 @@ def quantize_i8(x: torch.Tensor, out=None, scale=None):
     if x.dim() > 2:
         if not x.is_contiguous():
             raise HipQmmError("x of more than two dimensions must be contiguous")
-        flat = x.view(-1, K)
+        flat = x.view(lead.numel(), K)
     else:
         flat = x
     n = flat.shape[0]

@@ -199,3 +199,13 @@ def test_one_row_an_expert(library):
         with pytest.raises(G.HipQmmError):
             G.mul_mat_id_i8(On(w), On(_t(4, 1)), x, ids)
     assert len(library.calls) == 3
+
+
+@pytest.mark.parametrize("shape", [(3, 0), (2, 3, 0), (1, 1, 0)])
+def test_rows_without_values(shape, monkeypatch):
+    """The library's refusal (a row has 1 to 131071 values), whatever the dimensions."""
+    real = M._lib()
+    monkeypatch.setattr(M, "_lib", lambda: real)
+    monkeypatch.setattr(M, "_raw_stream", lambda *_: 0)
+    with pytest.raises(G.HipQmmError):
+        G.quantize_i8(On(torch.zeros(shape)))
