@@ -1,6 +1,8 @@
 """Weighted sums of experts' rows against f64: n + 1 terms summed by fused
 multiply-adds, each off by half a step of a partial sum, which is at most the sum
 of magnitudes."""
+import math
+
 import numpy as np
 import pytest
 
@@ -91,3 +93,30 @@ def test_ends_of_rows(rows, off):
     got = G.combine(y, w, add=add, out=out[:, off:off + rows])
     _check(y, w, add=add, got=got)
     assert (out[:, :off] == 7).all() and (out[:, off + rows:] == 7).all()
+
+
+@pytest.mark.parametrize("n,k,rows", [(3, 1, 50), (5, 8, 130), (4, 16, 70), (2, 64, 41)])
+@pytest.mark.parametrize("add", [False, True])
+def test_one_rounding(n, k, rows, add):
+    """Sums that nearly cancel, against the exact ones: half a step of the result, and what k f64 terms and the
+    reference's own rounding leave of their magnitudes."""
+    r = np.random.RandomState(k + rows)
+    y, w = r.randn(n, k, rows).astype(np.float32), r.randn(n, k).astype(np.float32)
+    terms = y.astype(np.float64) * w[..., None].astype(np.float64)  # exact
+    base = np.zeros((n, rows))
+    if add:
+        base = (-terms.sum(1) * (1 + r.randn(n, rows) * 1e-4)).astype(np.float32).astype(np.float64)
+    elif k > 1:
+        y[:, -1] = -(terms[:, :-1].sum(1) / w[:, -1:]) * (1 + r.randn(n, rows) * 1e-4)
+        terms = y.astype(np.float64) * w[..., None].astype(np.float64)
+    want = np.array([[math.fsum([base[t, m], *terms[t, :, m]]) for m in range(rows)] for t in range(n)])
+    bound = R.U * np.abs(want) + (k + 2) * 2.0 ** -53 * (np.abs(base) + np.abs(terms).sum(1)) + 2.0 ** -150
+    got = G.combine(torch.from_numpy(y).cuda(), torch.from_numpy(w).cuda(),
+                    add=torch.from_numpy(base.astype(np.float32)).cuda() if add else None).cpu().numpy()
+    assert np.all(np.abs(got.astype(np.float64) - want) <= bound)
+    # What the bound is for: sums in f32 would not keep it.
+    f32 = base.astype(np.float32)
+    for s in range(k):
+        f32 = f32 + y[:, s] * w[:, s:s + 1]
+    if k > 1 or add:
+        assert np.any(np.abs(f32.astype(np.float64) - want) > bound)
