@@ -8,9 +8,10 @@
 // The order is that of f64 scores.  Where a score is the logit itself f32 holds
 // it.  Else f32 scores are tried: their errors are below SURE, so two that are
 // further apart have the right order, and only a token of which some that matter
-// are not is done again in f64 (a few in a thousand).
+// are not is done again in f64 (a few in a thousand), and so is one whose scores
+// leave the range of f32.
 //
-// Bound by the issue of instructions, 650 vector and 350 scalar ones a token of
+// Bound by the issue of instructions, 670 vector and 350 scalar ones a token of
 // 256 experts in groups: 8192 such tokens take 14.4 us, where their logits could
 // be read in 1.8, 61 tokens 5.4; one of 128 experts 3.4.  Several tokens a wave,
 // one after the other, took longer.
